@@ -24,3 +24,9 @@ from .moe import (  # noqa: F401
     plan_residency,
     workspace_bytes,
 )
+from .ffn import (  # noqa: F401
+    LowRankAdapters,
+    adapter_linear,
+    gated_ffn,
+    gated_ffn_backward,
+)

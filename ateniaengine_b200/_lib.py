@@ -57,6 +57,15 @@ class HostMoeLayer(C.Structure):
     ]
 
 
+class LowRank(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("rank", C.c_int32), ("reserved", C.c_int32)]
+
+
+class FfnAdapters(C.Structure):
+    _fields_ = [("gate", LowRank), ("up", LowRank), ("down", LowRank), ("ids", C.c_void_p), ("n", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
 EXPORTS = [
     "atenia_moe_create", "atenia_moe_destroy", "atenia_moe_set_weights", "atenia_moe_forward",
     "atenia_moe_forward_sync", "atenia_moe_check", "atenia_moe_route_from_logits",
@@ -75,6 +84,8 @@ EXPORTS = [
     "atenia_numeric_policy_ffn_uses_f32", "atenia_numeric_policy_ffn_uses_cuda", "atenia_numeric_policy_gate",
     "atenia_moe_block_forward", "atenia_moe_stack_set_norm", "atenia_moe_last_phase_ms", "atenia_moe_last_recv_rows", "atenia_moe_plan_residency", "atenia_auto_expert_cache_capacity", "atenia_moe_workspace_bytes",
     "atenia_moe_plan_exec_pieces", "atenia_moe_plan_exec_pieces_measured",
+    "atenia_gated_ffn_workspace_bytes", "atenia_gated_ffn_forward", "atenia_gated_ffn_backward",
+    "atenia_adapter_linear_workspace_bytes", "atenia_adapter_linear", "atenia_ffn_check",
 ]
 
 _lib = None
@@ -174,6 +185,17 @@ def lib():
         l.atenia_moe_plan_exec_pieces.argtypes = [C.POINTER(MoeConfig), C.c_uint64, C.POINTER(C.c_uint64), C.c_int]
         l.atenia_moe_plan_exec_pieces_measured.argtypes = [C.POINTER(MoeConfig), C.c_uint64, C.c_double, C.c_double,
                                                             C.c_double, C.POINTER(C.c_uint64), C.c_int]
+        vp = C.c_void_p
+        l.atenia_gated_ffn_workspace_bytes.argtypes = [C.c_int] * 3 + [C.POINTER(FfnAdapters), C.c_int]
+        l.atenia_gated_ffn_workspace_bytes.restype = C.c_uint64
+        l.atenia_gated_ffn_forward.argtypes = ([vp] * 4 + [C.c_int] * 3 + [C.POINTER(FfnAdapters)] + [vp] * 4
+                                               + [C.c_uint64, vp])
+        l.atenia_gated_ffn_backward.argtypes = [vp] * 7 + [C.c_int] * 3 + [vp] * 5 + [C.c_uint64, vp]
+        l.atenia_adapter_linear_workspace_bytes.argtypes = [C.c_int, C.c_int]
+        l.atenia_adapter_linear_workspace_bytes.restype = C.c_uint64
+        l.atenia_adapter_linear.argtypes = ([vp, vp] + [C.c_int] * 3 + [C.POINTER(LowRank), vp, C.c_int, vp, vp, C.c_uint64,
+                                                                         vp])
+        l.atenia_ffn_check.argtypes = [vp]
         _lib = l
     return _lib
 

@@ -5,7 +5,7 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["grouped_gemm.cu", "w8_gemm.cu", "w8_gemm_m256.cu", "bf16_decode_gemm.cu", "decode_gemv.cu", "grouped_gemm_2cta.cu", "grouped_gemm_pair_rows.cu", "router.cu", "router_dmma.cu", "router_splitk.cu", "router_i8.cu", "dispatch.cu", "combine.cu", "moe_layer.cu", "ep.cu", "registry.cu", "noalloc.cu", "planner.cu", "stack.cu", "tier.cu", "dense_int8.cu"]
+SOURCES = ["grouped_gemm.cu", "w8_gemm.cu", "w8_gemm_m256.cu", "bf16_decode_gemm.cu", "decode_gemv.cu", "grouped_gemm_2cta.cu", "grouped_gemm_pair_rows.cu", "router.cu", "router_dmma.cu", "router_splitk.cu", "router_i8.cu", "dispatch.cu", "combine.cu", "moe_layer.cu", "ep.cu", "registry.cu", "noalloc.cu", "planner.cu", "stack.cu", "tier.cu", "dense_int8.cu", "dense_gemm.cu", "adapters.cu", "gated_ffn.cu"]
 LIB = os.path.join(HERE, "libatenia_moe.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-ccbin", "g++",
@@ -20,7 +20,7 @@ def _stale(out, deps):
 
 
 def build(force=False, verbose=False):
-    headers = [os.path.join(HERE, h) for h in ("common.cuh", "layer.cuh", "tc_common.cuh", "v3_route.cuh", "route_warp.cuh", "dmma.cuh", "router_digits.cuh", "round_codes.cuh", "ep_plan.cuh", "pair_tiles.cuh", "kernel_choice.cuh")] + [
+    headers = [os.path.join(HERE, h) for h in ("common.cuh", "layer.cuh", "tc_common.cuh", "v3_route.cuh", "route_warp.cuh", "dmma.cuh", "router_digits.cuh", "round_codes.cuh", "ep_plan.cuh", "pair_tiles.cuh", "kernel_choice.cuh", "dense_gemm.cuh")] + [
         os.path.join(HERE, "..", "..", "include", "atenia_moe.h")]
     objs = []
     jobs = []

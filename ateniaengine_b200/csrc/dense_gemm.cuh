@@ -1,0 +1,267 @@
+// Products of the dense feed-forward block and of the low-rank adapters: what the kernels (dense_gemm.cu, adapters.cu) and the
+// entry points (gated_ffn.cu) share.
+//
+// Every product is D[m, n] = sum_k A[m, k] B[n, k] with D row-major.  An operand lies in memory either with k contiguous
+// ("K-major": activations times weights as the models store them) or with its own rows contiguous ("MN-major": the transposed
+// reads of the backward pass, where the reduction runs over the rows of a row-major matrix).  Both come through TMA into
+// 128-byte-swizzled tiles and the MMA reads either, so nothing is transposed in memory.
+#pragma once
+#include "tc_common.cuh"
+
+namespace atenia {
+
+enum DenseEpilogue {
+  kDensePlain = 0,     // out[m, n] = D
+  kDenseSwiGLU = 1,    // B = gate and up rows of the same features: out[m, f] = silu(g) u, optionally g and u in f32
+  kDenseGateGrad = 2,  // D = dh: dg, du and h from the saved g and u
+};
+
+struct DenseProblem {
+  CUtensorMap a[2], b[2];  // kDenseSwiGLU: b[0] gate, b[1] up.  Else the k-blocks from kb0 on come through a[1] and b[1]
+  int M, N, kb, kb0;       // N: columns of `out`; kb: k-blocks of 64 in all
+  __nv_bfloat16* out;      // [M, N]
+  float* gate;             // kDenseSwiGLU: g and u [M, N] to be saved, or null; kDenseGateGrad: the saved ones
+  float* up;
+  __nv_bfloat16* out_du;   // kDenseGateGrad: du and h [M, N] (dg is `out`)
+  __nv_bfloat16* out_h;
+};
+
+// One projection's adapters beside the product: D[m, :] += B_a v[m, :] for a = ids[m].  (kDenseSwiGLU: segment 0 acts on the
+// gate columns, segment 1 on the up columns; a segment of rank 0 adds nothing.)
+struct AdapterSegment {
+  CUtensorMap v;  // [M, rank] bf16, box {16, rows}, 32-byte swizzle
+  CUtensorMap b;  // [n, N, rank] bf16, box {16, 64, 1}, 32-byte swizzle
+  int rank;
+};
+struct DenseAdapters {
+  AdapterSegment seg[2];
+  const int32_t* ids;  // [M]; an id outside [0, n) means none
+  int n;
+};
+
+constexpr int kMaxDenseProblems = 3;
+struct DenseGemm {
+  DenseProblem p[kMaxDenseProblems];
+  int problems;
+  int epilogue;
+  bool a_mn, b_mn;               // MN-major operands
+  const DenseAdapters* adapters;  // or null (host pointer, copied at the launch)
+  int a_rows;                    // K-major A: rows of its box (dense_a_rows)
+  bool chained;                  // see launch_chained
+  bool b_early;                  // B is not written by the kernel before: its first tiles are requested before the wait
+  bool a_early;                  // neither is A: only the adapters' v is waited for
+};
+int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);
+
+// Rows of a K-major A box: all of a small batch, so that a call of few tokens moves few token rows.
+inline int dense_a_rows(int64_t rows) { return rows >= 128 ? 128 : (int)((rows + 7) / 8 * 8); }
+
+// v[t, :] = scale[a] * (A_a x[t, :]), a = ids[t], for up to two projections of the same rows
+struct AdapterReduce {
+  struct Projection {
+    CUtensorMap a;  // [n, rank, K] bf16, box {64, rank, 1}, 128-byte swizzle
+    const float* scale;  // [n]
+    __nv_bfloat16* v;    // [M, rank]
+    int rank;
+  } p[2];
+  int projections;
+  CUtensorMap x;  // [M, K], box {64, a_rows}
+  const int32_t* ids;
+  int M, kb, n, a_rows;
+  bool chained;
+};
+int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s);
+constexpr int kAdapterMaxRank = 128;
+
+// Where kernels of these files record a wait that gave up: one word per device, read by atenia_ffn_check.
+int dense_error_word(DeviceError** out);
+
+// bf16 map of up to three dimensions (innermost first, contiguous); dims[2] = 0: two
+int encode_tmap_bf16(CUtensorMap* out, const void* base, const uint64_t (&dims)[3], const uint32_t (&box)[3], int swizzle_bytes);
+
+// ---- device side -------------------------------------------------------------------------------
+#ifdef __CUDACC__
+namespace tc {
+// Descriptor of an MN-major operand under the 128-byte swizzle: atoms of 64 elements x 8 k; the next 8 k 1024 bytes on
+// (stride offset), the next 64 elements 8192 bytes on (leading offset; a box of 64 k x 64 elements).
+__device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t smem_addr) {
+  uint64_t d = static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(8192 >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// K-major, 32-byte swizzle: rows of 32 bytes (one K = 16 step), eight-row groups 256 bytes apart.
+__device__ __forceinline__ uint64_t make_smem_desc_k16(uint32_t smem_addr) {
+  uint64_t d = static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(256 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(6) << 61;
+  return d;
+}
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
+  return MN ? make_smem_desc_mn(smem_addr) : make_smem_desc(smem_addr);
+}
+// K = 16 further inside the tile: 32 bytes of the swizzle row, or 16 rows of 128 bytes
+template <bool MN>
+constexpr uint64_t kOperandStep = MN ? (2048 >> 4) : (32 >> 4);
+
+__device__ __forceinline__ void tma_load_3d_one(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// An accumulating MMA that leaves the lanes whose bit is set in `off` as they are.
+__device__ __forceinline__ void tc_mma_bf16_lanes_one(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                      const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n\t.reg .pred e, t;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, t;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
+__device__ __forceinline__ void tc_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float at this offset of the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %1, %2;\n\t"
+      "ld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank));
+  return v;
+}
+
+constexpr int kNoAdapter = 0x7fffffff;
+// The ids of 32 * W token rows from `row0` on, W per lane; kNoAdapter where a row is past the end or has none.
+template <int W>
+__device__ __forceinline__ void load_ids(int32_t (&id)[W], const int32_t* __restrict__ ids, int64_t row0, int rows, int n, int lane) {
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const int r = 32 * w + lane;
+    const int32_t v = r < rows ? ids[row0 + r] : -1;
+    id[w] = v >= 0 && v < n ? v : kNoAdapter;
+  }
+}
+// The smallest id above `last` that some row has, kNoAdapter if there is none: the adapters of a tile in ascending order, found
+// alike by every warp that walks them.
+template <int W>
+__device__ __forceinline__ int32_t next_adapter(const int32_t (&id)[W], int32_t last) {
+  int32_t m = kNoAdapter;
+#pragma unroll
+  for (int w = 0; w < W; ++w) m = id[w] > last && id[w] < m ? id[w] : m;
+  return __reduce_min_sync(0xffffffffu, m);
+}
+// Bit set: the row does not have adapter `a`.
+template <int W>
+__device__ __forceinline__ void lanes_off(uint32_t (&off)[W], const int32_t (&id)[W], int32_t a) {
+#pragma unroll
+  for (int w = 0; w < W; ++w) off[w] = __ballot_sync(0xffffffffu, id[w] != a);
+}
+
+// dg, du and h of one element
+__device__ __forceinline__ void gate_grad(float dh, float g, float u, float& dg, float& du, float& h) {
+  const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+  dg = dh * u * (s * (1.0f + g * (1.0f - s)));
+  du = dh * (g * s);
+  h = silu_mul(g, u);
+}
+// 16 values of one row to consecutive bf16 (32 bytes; 16-byte aligned)
+__device__ __forceinline__ void store16_bf16(__nv_bfloat16* dst, const float (&v)[16]) {
+  uint4 a, b;
+  a.x = pack_bf16x2(v[0], v[1]);
+  a.y = pack_bf16x2(v[2], v[3]);
+  a.z = pack_bf16x2(v[4], v[5]);
+  a.w = pack_bf16x2(v[6], v[7]);
+  b.x = pack_bf16x2(v[8], v[9]);
+  b.y = pack_bf16x2(v[10], v[11]);
+  b.z = pack_bf16x2(v[12], v[13]);
+  b.w = pack_bf16x2(v[14], v[15]);
+  reinterpret_cast<uint4*>(dst)[0] = a;
+  reinterpret_cast<uint4*>(dst)[1] = b;
+}
+__device__ __forceinline__ void store16_f32(float* dst, const float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+__device__ __forceinline__ void load16_f32(const float* src, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 q = reinterpret_cast<const float4*>(src)[i];
+    v[4 * i] = q.x;
+    v[4 * i + 1] = q.y;
+    v[4 * i + 2] = q.z;
+    v[4 * i + 3] = q.w;
+  }
+}
+// What becomes of 16 neighbouring columns of one row (acc1: the up columns of kDenseSwiGLU)
+template <int EPI>
+__device__ __forceinline__ void dense_emit16(const DenseProblem& p, int64_t at, const float (&acc)[16], const float (&acc1)[16]) {
+  float o[16];
+  if constexpr (EPI == kDensePlain) {
+    store16_bf16(p.out + at, acc);
+  } else if constexpr (EPI == kDenseSwiGLU) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = silu_mul(acc[j], acc1[j]);
+    store16_bf16(p.out + at, o);
+    if (p.gate) {
+      store16_f32(p.gate + at, acc);
+      store16_f32(p.up + at, acc1);
+    }
+  } else {
+    float g[16], u[16], du[16], h[16];
+    load16_f32(p.gate + at, g);
+    load16_f32(p.up + at, u);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) gate_grad(acc[j], g[j], u[j], o[j], du[j], h[j]);
+    store16_bf16(p.out + at, o);
+    store16_bf16(p.out_du + at, du);
+    store16_bf16(p.out_h + at, h);
+  }
+}
+// ... of one element
+template <int EPI>
+__device__ __forceinline__ void dense_emit1(const DenseProblem& p, int64_t at, float acc, float acc1) {
+  if constexpr (EPI == kDensePlain) {
+    p.out[at] = __float2bfloat16(acc);
+  } else if constexpr (EPI == kDenseSwiGLU) {
+    p.out[at] = __float2bfloat16(silu_mul(acc, acc1));
+    if (p.gate) {
+      p.gate[at] = acc;
+      p.up[at] = acc1;
+    }
+  } else {
+    float dg, du, h;
+    gate_grad(acc, p.gate[at], p.up[at], dg, du, h);
+    p.out[at] = __float2bfloat16(dg);
+    p.out_du[at] = __float2bfloat16(du);
+    p.out_h[at] = __float2bfloat16(h);
+  }
+}
+}  // namespace tc
+#endif
+
+}  // namespace atenia

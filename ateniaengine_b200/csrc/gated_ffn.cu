@@ -1,0 +1,348 @@
+// Entry points of the dense gated feed-forward block, its backward pass and the low-rank adapters, and their host side.
+//
+//   forward   g = x Wg^T, u = x Wu^T, h = silu(g) u (one kernel); y = h Wd^T
+//   backward  dh = dy Wd, from it with the saved g and u: dg, du and h again (one kernel);
+//             dx = dg Wg + du Wu (one reduction of 2 d_ff); dWg = dg^T x, dWu = du^T x, dWd = dy^T h (one launch)
+//   adapters  v = scale A x of the rows' own adapters, then their B v inside the projection's kernel
+//
+// The calls keep no state: the caller passes the workspace, so that two calls, streams or captured graphs share nothing but
+// what the caller lets them share.  g and u are saved in f32 (8 bytes per token and feature): rounded to bf16 they would
+// add as much to the gradients' error as the two roundings that the operands of the second products need anyway.
+#include <mutex>
+
+#include "dense_gemm.cuh"
+
+namespace atenia {
+
+namespace {
+
+static __device__ DeviceError g_dense_error;
+std::mutex g_mu;
+DeviceError* g_error_addr[kMaxDevices] = {};
+int g_sms[kMaxDevices] = {};
+
+int num_sms_of_current_device(int* out) {
+  int dev = -1;
+  ATENIA_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return ATENIA_ERR_UNSUPPORTED;
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_sms[dev]) ATENIA_CUDA_TRY(cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev));
+  *out = g_sms[dev];
+  return ATENIA_OK;
+}
+
+constexpr int64_t kMaxRows = 1 << 24, kMaxWidth = 1 << 20;
+
+uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+int kblocks(int64_t k) { return (int)((k + tc::BK - 1) / tc::BK); }
+
+// [rows, cols] row-major in boxes of `box_rows` rows x 64 columns
+int matrix_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
+  return encode_tmap_bf16(m, base, {(uint64_t)cols, (uint64_t)rows, 0}, {64, (uint32_t)box_rows, 1}, 128);
+}
+
+bool rank_ok(int r) { return r >= 8 && r <= kAdapterMaxRank && r % 8 == 0; }
+int check_adapter(const AteniaLowRank& a) {
+  if (!rank_ok(a.rank)) return ATENIA_ERR_SHAPE;
+  if (!a.a || !a.b || !a.scale) return ATENIA_ERR_NULL;
+  if (!aligned16(a.a) || !aligned16(a.b)) return ATENIA_ERR_SHAPE;
+  return ATENIA_OK;
+}
+uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64_t)T * rank * 2) : 0; }
+
+// One projection's adapters: the first half's projection and the second half's segment, with v at `v`.
+int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, void* v,
+                   AdapterReduce::Projection* red, AdapterSegment* seg) {
+  const uint64_t r = (uint64_t)a.rank;
+  int rc = encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
+  if (!rc) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {16, (uint32_t)a_rows, 1}, 32);
+  if (!rc) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {16, 64, 1}, 32);
+  red->scale = a.scale;
+  red->v = static_cast<__nv_bfloat16*>(v);
+  red->rank = seg->rank = a.rank;
+  return rc;
+}
+
+// The reduced rows of up to two projections of the same input, and what the product needs of them.
+struct AdapterPlan {
+  AdapterReduce red{};
+  DenseAdapters add{};
+};
+int plan_adapters(AdapterPlan* p, const AteniaLowRank* const (&sets)[2], const int32_t* ids, int n, const void* x, int64_t T,
+                  int64_t in, int64_t out, uint8_t** ws, bool chained) {
+  const int a_rows = dense_a_rows(T);
+  p->red.ids = p->add.ids = ids;
+  p->red.n = p->add.n = n;
+  p->red.M = (int)T;
+  p->red.kb = kblocks(in);
+  p->red.a_rows = a_rows;
+  p->red.chained = chained;
+  int rc = matrix_map(&p->red.x, x, T, in, a_rows);
+  for (int i = 0; i < 2 && !rc; ++i) {
+    if (!sets[i] || sets[i]->rank == 0) continue;
+    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
+    p->red.projections += 1;
+    *ws += reduced_bytes(T, sets[i]->rank);
+  }
+  return rc;
+}
+
+int check_sizes(int64_t T, int64_t d, int64_t f) {
+  if (T < 0 || T > kMaxRows || d < 16 || f < 16 || d > kMaxWidth || f > kMaxWidth || d % 16 || f % 16) return ATENIA_ERR_SHAPE;
+  return ATENIA_OK;
+}
+
+int check_ffn_adapters(const AteniaFfnAdapters* ad) {
+  if (!ad->ids) return ATENIA_ERR_NULL;
+  if (ad->n < 1) return ATENIA_ERR_SHAPE;
+  const AteniaLowRank* sets[3] = {&ad->gate, &ad->up, &ad->down};
+  for (const AteniaLowRank* a : sets) {
+    if (a->rank == 0) continue;
+    int rc = check_adapter(*a);
+    if (rc) return rc;
+  }
+  return ATENIA_OK;
+}
+
+}  // namespace
+
+int dense_error_word(DeviceError** out) {
+  int dev = -1;
+  ATENIA_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return ATENIA_ERR_UNSUPPORTED;
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_error_addr[dev]) {
+    void* p = nullptr;
+    ATENIA_CUDA_TRY(cudaGetSymbolAddress(&p, g_dense_error));
+    if (!p) return ATENIA_ERR_DRIVER;
+    g_error_addr[dev] = static_cast<DeviceError*>(p);
+  }
+  *out = g_error_addr[dev];
+  return ATENIA_OK;
+}
+
+}  // namespace atenia
+
+extern "C" {
+
+uint64_t atenia_gated_ffn_workspace_bytes(int T, int d_model, int d_ff, const AteniaFfnAdapters* adapters, int backward) {
+  using namespace atenia;
+  if (check_sizes(T, d_model, d_ff)) return 0;
+  const uint64_t rows = align256((uint64_t)T * d_ff * 2);
+  if (backward) return 3 * rows;  // dg, du, h
+  uint64_t n = rows;              // h
+  if (adapters) n += reduced_bytes(T, adapters->gate.rank) + reduced_bytes(T, adapters->up.rank) + reduced_bytes(T, adapters->down.rank);
+  return n;
+}
+
+uint64_t atenia_adapter_linear_workspace_bytes(int T, int rank) {
+  return T < 0 || !atenia::rank_ok(rank) ? 0 : atenia::reduced_bytes(T, rank);
+}
+
+int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up, const void* w_down, int T, int d_model, int d_ff,
+                             const AteniaFfnAdapters* adapters, void* y, float* saved_gate, float* saved_up, void* workspace,
+                             uint64_t workspace_bytes, void* stream) {
+  using namespace atenia;
+  int rc = check_sizes(T, d_model, d_ff);
+  if (rc) return rc;
+  if (!w_gate || !w_up || !w_down || !saved_gate != !saved_up) return ATENIA_ERR_NULL;
+  if (adapters && (rc = check_ffn_adapters(adapters))) return rc;
+  if (T == 0) return ATENIA_OK;
+  if (!x || !y || !workspace) return ATENIA_ERR_NULL;
+  for (const void* p : {x, w_gate, w_up, w_down, (const void*)y, (const void*)saved_gate, (const void*)saved_up, (const void*)workspace})
+    if (!aligned16(p)) return ATENIA_ERR_SHAPE;
+  if (workspace_bytes < atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, adapters, 0)) return ATENIA_ERR_CAPACITY;
+  int sms = 0;
+  if ((rc = num_sms_of_current_device(&sms))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(ws);
+  ws += align256((uint64_t)T * d_ff * 2);
+  const int64_t d = d_model, F = d_ff;
+
+  AdapterPlan first, second;
+  const bool ad1 = adapters && (adapters->gate.rank || adapters->up.rank), ad2 = adapters && adapters->down.rank;
+  DenseGemm g1{};
+  g1.problems = 1;
+  g1.epilogue = kDenseSwiGLU;
+  g1.a_rows = dense_a_rows(T);
+  DenseProblem& p1 = g1.p[0];
+  p1.M = T;
+  p1.N = d_ff;
+  p1.kb = p1.kb0 = kblocks(d);
+  p1.out = h;
+  p1.gate = saved_gate;
+  p1.up = saved_up;
+  rc = matrix_map(&p1.a[0], x, T, d, g1.a_rows);
+  if (!rc) rc = matrix_map(&p1.b[0], w_gate, F, d, 64);
+  if (!rc) rc = matrix_map(&p1.b[1], w_up, F, d, 64);
+  DenseGemm g2{};
+  g2.problems = 1;
+  g2.epilogue = kDensePlain;
+  g2.a_rows = g1.a_rows;
+  g2.chained = g2.b_early = true;
+  DenseProblem& p2 = g2.p[0];
+  p2.M = T;
+  p2.N = d_model;
+  p2.kb = p2.kb0 = kblocks(F);
+  p2.out = static_cast<__nv_bfloat16*>(y);
+  if (!rc) rc = matrix_map(&p2.a[0], h, T, F, g2.a_rows);
+  if (!rc) rc = matrix_map(&p2.b[0], w_down, d, F, 64);
+  if (!rc && ad1) {
+    rc = plan_adapters(&first, {&adapters->gate, &adapters->up}, adapters->ids, adapters->n, x, T, d, F, &ws, false);
+    g1.adapters = &first.add;
+    g1.chained = true;
+  }
+  g1.b_early = g1.a_early = true;  // (only the adapters' rows come from a kernel of this call)
+  if (!rc && ad2) {
+    rc = plan_adapters(&second, {&adapters->down, nullptr}, adapters->ids, adapters->n, h, T, F, d, &ws, true);
+    g2.adapters = &second.add;
+  }
+  if (!rc && ad1) rc = launch_adapter_reduce(first.red, sms, s);
+  if (!rc) rc = launch_dense_gemm(g1, sms, s);
+  if (!rc && ad2) rc = launch_adapter_reduce(second.red, sms, s);
+  if (!rc) rc = launch_dense_gemm(g2, sms, s);
+  return rc;
+}
+
+int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                              const float* saved_gate, const float* saved_up, int T, int d_model, int d_ff, void* dx, void* dw_gate,
+                              void* dw_up, void* dw_down, void* workspace, uint64_t workspace_bytes, void* stream) {
+  using namespace atenia;
+  int rc = check_sizes(T, d_model, d_ff);
+  if (rc) return rc;
+  if (!w_gate || !w_up || !w_down || !dw_gate || !dw_up || !dw_down) return ATENIA_ERR_NULL;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t d = d_model, F = d_ff;
+  if (T == 0) {  // sums over no token
+    for (void* p : {dw_gate, dw_up, dw_down}) ATENIA_CUDA_TRY(cudaMemsetAsync(p, 0, (size_t)(d * F * 2), s));
+    return ATENIA_OK;
+  }
+  if (!dy || !x || !dx || !saved_gate || !saved_up || !workspace) return ATENIA_ERR_NULL;
+  for (const void* p : {dy, x, w_gate, w_up, w_down, (const void*)saved_gate, (const void*)saved_up, (const void*)dx, (const void*)dw_gate,
+                        (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
+    if (!aligned16(p)) return ATENIA_ERR_SHAPE;
+  if (workspace_bytes < atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, nullptr, 1)) return ATENIA_ERR_CAPACITY;
+  int sms = 0;
+  if ((rc = num_sms_of_current_device(&sms))) return rc;
+  const uint64_t rows = align256((uint64_t)T * F * 2);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  __nv_bfloat16* dg = reinterpret_cast<__nv_bfloat16*>(ws);
+  __nv_bfloat16* du = reinterpret_cast<__nv_bfloat16*>(ws + rows);
+  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(ws + 2 * rows);
+
+  DenseGemm g1{};  // dh = dy Wd: the reduction runs over the rows of Wd [d, F]
+  g1.problems = 1;
+  g1.epilogue = kDenseGateGrad;
+  g1.b_mn = true;
+  g1.a_rows = dense_a_rows(T);
+  g1.b_early = g1.a_early = true;
+  DenseProblem& p1 = g1.p[0];
+  p1.M = T;
+  p1.N = d_ff;
+  p1.kb = p1.kb0 = kblocks(d);
+  p1.out = dg;
+  p1.out_du = du;
+  p1.out_h = h;
+  p1.gate = const_cast<float*>(saved_gate);
+  p1.up = const_cast<float*>(saved_up);
+  rc = matrix_map(&p1.a[0], dy, T, d, g1.a_rows);
+  if (!rc) rc = matrix_map(&p1.b[0], w_down, d, F, 64);
+
+  DenseGemm g2{};  // dx = dg Wg + du Wu
+  g2.problems = 1;
+  g2.epilogue = kDensePlain;
+  g2.b_mn = true;
+  g2.a_rows = g1.a_rows;
+  g2.chained = g2.b_early = true;
+  DenseProblem& p2 = g2.p[0];
+  p2.M = T;
+  p2.N = d_model;
+  p2.kb0 = kblocks(F);
+  p2.kb = 2 * p2.kb0;
+  p2.out = static_cast<__nv_bfloat16*>(dx);
+  if (!rc) rc = matrix_map(&p2.a[0], dg, T, F, g2.a_rows);
+  if (!rc) rc = matrix_map(&p2.a[1], du, T, F, g2.a_rows);
+  if (!rc) rc = matrix_map(&p2.b[0], w_gate, F, d, 64);
+  if (!rc) rc = matrix_map(&p2.b[1], w_up, F, d, 64);
+
+  DenseGemm g3{};  // the weights' gradients: reductions over the tokens
+  g3.problems = 3;
+  g3.epilogue = kDensePlain;
+  g3.a_mn = g3.b_mn = true;
+  g3.chained = true;
+  const void* lhs[3] = {dg, du, dy};
+  const void* rhs[3] = {x, x, h};
+  void* out[3] = {dw_gate, dw_up, dw_down};
+  for (int i = 0; i < 3; ++i) {
+    DenseProblem& p = g3.p[i];
+    p.M = i < 2 ? d_ff : d_model;
+    p.N = i < 2 ? d_model : d_ff;
+    p.kb = p.kb0 = kblocks(T);
+    p.out = static_cast<__nv_bfloat16*>(out[i]);
+    if (!rc) rc = matrix_map(&p.a[0], lhs[i], T, p.M, 64);
+    if (!rc) rc = matrix_map(&p.b[0], rhs[i], T, p.N, 64);
+  }
+  if (!rc) rc = launch_dense_gemm(g1, sms, s);
+  if (!rc) rc = launch_dense_gemm(g2, sms, s);
+  if (!rc) rc = launch_dense_gemm(g3, sms, s);
+  return rc;
+}
+
+int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, int d_out, const AteniaLowRank* adapter,
+                          const int32_t* ids, int n, void* y, void* workspace, uint64_t workspace_bytes, void* stream) {
+  using namespace atenia;
+  int rc = check_sizes(T, d_in, d_out);
+  if (rc) return rc;
+  if (!weight || !adapter) return ATENIA_ERR_NULL;
+  if (n < 1) return ATENIA_ERR_SHAPE;
+  if ((rc = check_adapter(*adapter))) return rc;
+  if (T == 0) return ATENIA_OK;
+  if (!x || !ids || !y || !workspace) return ATENIA_ERR_NULL;
+  for (const void* p : {x, weight, (const void*)y, (const void*)workspace})
+    if (!aligned16(p)) return ATENIA_ERR_SHAPE;
+  if (overlap(x, (uint64_t)T * d_in * 2, y, (uint64_t)T * d_out * 2)) return ATENIA_ERR_SHAPE;
+  if (workspace_bytes < atenia_adapter_linear_workspace_bytes(T, adapter->rank)) return ATENIA_ERR_CAPACITY;
+  int sms = 0;
+  if ((rc = num_sms_of_current_device(&sms))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  AdapterPlan plan;
+  rc = plan_adapters(&plan, {adapter, nullptr}, ids, n, x, T, d_in, d_out, &ws, false);
+  DenseGemm g{};
+  g.problems = 1;
+  g.epilogue = kDensePlain;
+  g.a_rows = dense_a_rows(T);
+  g.adapters = &plan.add;
+  g.chained = g.b_early = g.a_early = true;
+  DenseProblem& p = g.p[0];
+  p.M = T;
+  p.N = d_out;
+  p.kb = p.kb0 = kblocks(d_in);
+  p.out = static_cast<__nv_bfloat16*>(y);
+  if (!rc) rc = matrix_map(&p.a[0], x, T, d_in, g.a_rows);
+  if (!rc) rc = matrix_map(&p.b[0], weight, d_out, d_in, 64);
+  if (!rc) rc = launch_adapter_reduce(plan.red, sms, s);
+  if (!rc) rc = launch_dense_gemm(g, sms, s);
+  return rc;
+}
+
+int atenia_ffn_check(void* stream) {
+  using namespace atenia;
+  DeviceError* err = nullptr;
+  int rc = dense_error_word(&err);
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceError e{};
+  ATENIA_CUDA_TRY(cudaMemcpyAsync(&e, err, sizeof e, cudaMemcpyDeviceToHost, s));
+  ATENIA_CUDA_TRY(cudaStreamSynchronize(s));
+  if (e.code) ATENIA_CUDA_TRY(cudaMemsetAsync(err, 0, sizeof e, s));
+  return e.code;
+}
+
+}  // extern "C"

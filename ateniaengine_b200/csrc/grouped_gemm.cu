@@ -26,7 +26,7 @@
 //
 // Every wait is bounded: a wait that runs out records ATENIA_ERR_DEVICE_TIMEOUT with a site id and
 // the CTA leaves its loops, waits (bounded) for its own TMA copies, frees TMEM and returns.
-#include "tc_common.cuh"
+#include "dense_gemm.cuh"
 
 namespace atenia {
 namespace {
@@ -507,6 +507,21 @@ int encode_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint6
   CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
+}
+
+int encode_tmap_bf16(CUtensorMap* out, const void* base, const uint64_t (&dims)[3], const uint32_t (&box)[3], int swizzle_bytes) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return ATENIA_ERR_DRIVER;
+  const int rank = dims[2] ? 3 : 2;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (dims[0] * 2) % 16 != 0) return ATENIA_ERR_SHAPE;
+  cuuint64_t size[3] = {dims[0], dims[1], dims[2]};
+  cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
+  cuuint32_t boxes[3] = {box[0], box[1], box[2]};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), size, strides, boxes, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
 }
 

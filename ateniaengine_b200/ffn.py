@@ -1,0 +1,177 @@
+"""The dense gated feed-forward block, its backward pass, and low-rank adapters of many requests beside shared projections.
+
+The dense counterpart of an MoE layer's expert (gate, up, SwiGLU, down) for the layers of a model that have no router, for training
+it, and for serving it with one adapter per request.  Every computation runs in the CUDA library; torch owns the memory (the
+calls take their workspace from its allocator, on the current stream) and nothing is recorded for torch's autograd: a training
+step calls `gated_ffn_backward` itself.
+"""
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .moe import _launching
+
+BF16 = torch.bfloat16
+
+
+class LowRankAdapters(NamedTuple):
+    """n adapters of one projection [out, in]: token t of adapter i adds scale[i] * (x_t A_i^T) B_i^T.
+
+    a: CUDA bf16 [n, rank, in]; b: CUDA bf16 [n, out, rank]; scale: CUDA f32 [n].  rank: a multiple of 8 up to 128 (zero-pad a's rows
+    and b's columns otherwise)."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: torch.Tensor
+
+
+def _operand(t, name, shape, dtype, device):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, x on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows(x, name="x"):
+    if not isinstance(x, torch.Tensor) or x.dtype != BF16:
+        raise TypeError(f"{name} must be a bf16 tensor")
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be [tokens, width], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def _output(out, shape, x):
+    if out is None:
+        return torch.empty(shape, dtype=BF16, device=x.device)
+    if not isinstance(out, torch.Tensor) or out.dtype != BF16 or tuple(out.shape) != shape or out.device != x.device:
+        raise ValueError(f"out must be a bf16 tensor of shape {shape} on {x.device}")
+    if not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    return out
+
+
+def _low_rank(set_, name, n_in, n_out, device, keep):
+    """The C description of one projection's adapters; what it points to goes into `keep`."""
+    a, b, scale = set_
+    if not isinstance(a, torch.Tensor) or a.dim() != 3:
+        raise ValueError(f"{name}.a must be [n, rank, {n_in}]")
+    n, rank = a.shape[0], a.shape[1]
+    if n < 1 or rank < 8 or rank > 128 or rank % 8:
+        raise ValueError(f"{name}: at least one adapter, of a rank that is a multiple of 8 up to 128, got {tuple(a.shape)}")
+    a = _operand(a, name + ".a", (n, rank, n_in), BF16, device)
+    b = _operand(b, name + ".b", (n, n_out, rank), BF16, device)
+    scale = _operand(scale, name + ".scale", (n,), torch.float32, device)
+    keep += [a, b, scale]
+    return _lib.LowRank(a.data_ptr(), b.data_ptr(), scale.data_ptr(), rank, 0), n
+
+
+def _workspace(nbytes, device):
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+def _block(x, gate, up, down):
+    if not isinstance(gate, torch.Tensor) or gate.dim() != 2:
+        raise ValueError("gate must be [d_ff, d_model]")
+    T, d = x.shape
+    F = gate.shape[0]
+    if d < 16 or F < 16 or d % 16 or F % 16:
+        raise ValueError(f"d_model and d_ff must be multiples of 16, got {d} and {F}")
+    return (T, d, F, _operand(gate, "gate", (F, d), BF16, x.device), _operand(up, "up", (F, d), BF16, x.device),
+            _operand(down, "down", (d, F), BF16, x.device))
+
+
+def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, out=None, sync=False):
+    """y = (silu(x gate^T) * (x up^T)) down^T.  x: CUDA bf16 [T, d], any T; gate, up: bf16 [F, d]; down: bf16 [d, F].
+
+    `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
+    the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
+    [2, T, F], the two projections before the activation.  `sync=True` waits and raises what the kernels recorded."""
+    x = _rows(x)
+    T, d, F, gate, up, down = _block(x, gate, up, down)
+    keep, ad = [], None
+    if adapters:
+        if save:
+            raise ValueError("the backward pass is that of the block without adapters: save=True takes none")
+        if set(adapters) - {"gate", "up", "down"}:
+            raise ValueError(f"adapters of {sorted(set(adapters) - {'gate', 'up', 'down'})}: the block has gate, up and down")
+        ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, x.device)
+        ad = _lib.FfnAdapters(ids=ids.data_ptr())
+        for name, set_ in adapters.items():
+            n_in, n_out = (F, d) if name == "down" else (d, F)
+            low, n = _low_rank(set_, name, n_in, n_out, x.device, keep)
+            if ad.n not in (0, n):
+                raise ValueError("the projections have different numbers of adapters")
+            ad.n = n
+            setattr(ad, name, low)
+        keep.append(ids)
+    elif adapter_ids is not None:
+        raise ValueError("adapter_ids without adapters")
+    y = _output(out, (T, d), x)
+    saved = torch.empty((2, T, F), dtype=torch.float32, device=x.device) if save else None
+    lib = _lib.lib()
+    pad = C.byref(ad) if ad is not None else None
+    with _launching(x.device) as st:
+        nbytes = lib.atenia_gated_ffn_workspace_bytes(T, d, F, pad, 0)
+        ws = _workspace(nbytes, x.device)
+        _lib.check(lib.atenia_gated_ffn_forward(x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), T, d, F, pad,
+                                                y.data_ptr(), saved[0].data_ptr() if save else None,
+                                                saved[1].data_ptr() if save else None, ws.data_ptr(), ws.numel(), st), "gated_ffn")
+        if sync:
+            _lib.check(lib.atenia_ffn_check(st), "gated_ffn")
+    return (y, saved) if save else y
+
+
+def gated_ffn_backward(dy, x, gate, up, down, saved, sync=False):
+    """Gradients of gated_ffn(x, gate, up, down) for the gradient dy [T, d] of its output, from what save=True returned:
+    (dx [T, d], dgate [F, d], dup [F, d], ddown [d, F]), bf16.  `saved` is left as it is."""
+    x = _rows(x)
+    T, d, F, gate, up, down = _block(x, gate, up, down)
+    dy = _operand(dy, "dy", (T, d), BF16, x.device)
+    saved = _operand(saved, "saved", (2, T, F), torch.float32, x.device)
+    dx = torch.empty_like(x)
+    dgate, dup, ddown = torch.empty_like(gate), torch.empty_like(up), torch.empty_like(down)
+    lib = _lib.lib()
+    with _launching(x.device) as st:
+        nbytes = lib.atenia_gated_ffn_workspace_bytes(T, d, F, None, 1)
+        ws = _workspace(nbytes, x.device)
+        _lib.check(lib.atenia_gated_ffn_backward(dy.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(),
+                                                 saved[0].data_ptr(), saved[1].data_ptr(), T, d, F, dx.data_ptr(), dgate.data_ptr(),
+                                                 dup.data_ptr(), ddown.data_ptr(), ws.data_ptr(), ws.numel(), st),
+                   "gated_ffn_backward")
+        if sync:
+            _lib.check(lib.atenia_ffn_check(st), "gated_ffn_backward")
+    return dx, dgate, dup, ddown
+
+
+def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
+    """y = x weight^T + scale[i] * (x A_i^T) B_i^T with i = adapter_ids[t], outside [0, n) for none: one shared projection with the
+    adapters of many requests.  x: CUDA bf16 [T, in]; weight: bf16 [out, in]; adapters: LowRankAdapters; adapter_ids: int32 [T].
+    `out` must not overlap x."""
+    x = _rows(x)
+    T, n_in = x.shape
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be [out, in]")
+    n_out = weight.shape[0]
+    if n_in < 16 or n_out < 16 or n_in % 16 or n_out % 16:
+        raise ValueError(f"the projection's sizes must be multiples of 16, got {n_out} x {n_in}")
+    weight = _operand(weight, "weight", (n_out, n_in), BF16, x.device)
+    ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, x.device)
+    keep = []
+    low, n = _low_rank(adapters, "adapters", n_in, n_out, x.device, keep)
+    y = _output(out, (T, n_out), x)
+    lib = _lib.lib()
+    with _launching(x.device) as st:
+        ws = _workspace(lib.atenia_adapter_linear_workspace_bytes(T, low.rank), x.device)
+        _lib.check(lib.atenia_adapter_linear(x.data_ptr(), weight.data_ptr(), T, n_in, n_out, C.byref(low), ids.data_ptr(), n,
+                                             y.data_ptr(), ws.data_ptr(), ws.numel(), st), "adapter_linear")
+        if sync:
+            _lib.check(lib.atenia_ffn_check(st), "adapter_linear")
+    return y

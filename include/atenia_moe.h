@@ -424,6 +424,56 @@ ATENIA_API int atenia_moe_stack_set_norm(AteniaMoeStack* stack, const float* con
 ATENIA_API int atenia_moe_stack_check(AteniaMoeStack* stack, void* stream);
 ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
 
+/* ---- dense gated feed-forward block, its backward pass, low-rank adapters ------------------- */
+
+/* y = (silu(x Wg^T) * (x Wu^T)) Wd^T for the dense layers beside the MoE ones.  x [T, d_model], w_gate and w_up [d_ff, d_model],
+ * w_down [d_model, d_ff], y [T, d_model]: device, bf16, row-major.  The sums are f32; h = silu(g) u is rounded to bf16 between
+ * the products.  d_model and d_ff are multiples of 16 (at most 2^20), T at most 2^24 (0 is allowed); matrices and the workspace are
+ * 16-byte aligned (else ATENIA_ERR_SHAPE).  `workspace` (device) has at least the bytes the size function returns (else
+ * ATENIA_ERR_CAPACITY); its content need not be kept between calls, and calls that may run at the same time, captured ones
+ * included, need one each.  Asynchronous on `stream`; the calls allocate nothing and can be captured in a graph (make the first call
+ * per device outside of a capture).
+ * saved_gate, saved_up (device, f32 [T, d_ff], both or neither): g = x Wg^T and u = x Wu^T are stored for the backward pass.
+ *
+ * Adapters: token t adds scale[a] * B_a (A_a x_t) to a projection W x_t, where a = ids[t]; an id outside [0, n) means none.
+ * A is [n, rank, in], B [n, out, rank] (device, bf16, 16-byte aligned), scale [n] and ids [T] device.  A rank is a multiple of 8
+ * up to ATENIA_ADAPTER_MAX_RANK (zero-pad A's rows and B's columns otherwise); rank 0 = this projection has none.  The reduced
+ * rows scale A x are rounded to bf16.  A token reads its own adapter only: infinities and NaN in another one's do not reach it. */
+#define ATENIA_ADAPTER_MAX_RANK 128
+typedef struct AteniaLowRank {
+  const void* a;      /* device bf16 [n, rank, in] */
+  const void* b;      /* device bf16 [n, out, rank] */
+  const float* scale; /* device f32 [n] */
+  int32_t rank;
+  int32_t reserved;
+} AteniaLowRank;
+typedef struct AteniaFfnAdapters {
+  AteniaLowRank gate, up, down;
+  const int32_t* ids; /* device [T] */
+  int32_t n;          /* adapters, the same for all three projections */
+  int32_t reserved;
+} AteniaFfnAdapters;
+/* Bytes of workspace of the forward call (adapters may be NULL; only their ranks are read), or of the backward call
+ * (backward != 0).  0 for sizes the calls refuse. */
+ATENIA_API uint64_t atenia_gated_ffn_workspace_bytes(int T, int d_model, int d_ff, const AteniaFfnAdapters* adapters, int backward);
+ATENIA_API int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up, const void* w_down, int T, int d_model,
+                                        int d_ff, const AteniaFfnAdapters* adapters, void* y, float* saved_gate, float* saved_up,
+                                        void* workspace, uint64_t workspace_bytes, void* stream);
+/* Gradients of the block without adapters, from dy [T, d_model] and what the forward call saved: dx [T, d_model], dw_gate and
+ * dw_up [d_ff, d_model], dw_down [d_model, d_ff], bf16, all written (none is added to; zero for T = 0).  dg, du and h are rounded
+ * to bf16 as operands of the second products.  Nothing saved is changed: the call can be repeated.  No output overlaps an input. */
+ATENIA_API int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                                         const float* saved_gate, const float* saved_up, int T, int d_model, int d_ff, void* dx,
+                                         void* dw_gate, void* dw_up, void* dw_down, void* workspace, uint64_t workspace_bytes,
+                                         void* stream);
+/* y = x W^T plus the tokens' adapters: any one projection (W [d_out, d_in]).  y does not overlap x (ATENIA_ERR_SHAPE). */
+ATENIA_API uint64_t atenia_adapter_linear_workspace_bytes(int T, int rank);
+ATENIA_API int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, int d_out, const AteniaLowRank* adapter,
+                                     const int32_t* ids, int n, void* y, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Waits for the stream and returns the first error that kernels of the calls above recorded on this device since the last check
+ * (ATENIA_ERR_DEVICE_TIMEOUT: a bounded wait gave up); the word is cleared. */
+ATENIA_API int atenia_ffn_check(void* stream);
+
 /* ---- expert parallelism ------------------------------------------------------------------- */
 
 /* Size of the opaque NCCL unique id, and a fresh id (rank 0 creates it, the host program
