@@ -18,7 +18,8 @@ constexpr int kRedStages = 6;       // at most
 constexpr int kRedThreads = 192;
 constexpr int kRedTmemCols = 128;
 constexpr int kRedRingBytes = 100 * 1024;
-constexpr int kRedPartBytes = kAdapterMaxRank * 129 * 4;
+constexpr int kRedPitch = kAdapterMaxRank + 4;  // floats (see kPartPitch)
+constexpr int kRedPartBytes = BM * kRedPitch * 4;  // f32 sums [row][rank row]
 static_assert(kRedPartBytes <= kRedRingBytes, "");
 
 struct __align__(8) RedBars {
@@ -28,6 +29,28 @@ struct __align__(8) RedBars {
   uint32_t tmem_base;
   int abort_flag;
 };
+
+// This rank's share of the tile's sums, four rank rows a thread, added in rank order.
+template <int S>
+__device__ __forceinline__ void add_rows(const AdapterReduce& ar, int proj, int m0, int rows, uint32_t part, const int32_t* row_id,
+                                         int rank) {
+  const int r = ar.p[proj].rank, quads = r / 4, total = rows * quads;
+  const int begin = total * rank / S, end = total * (rank + 1) / S;
+  for (int i = begin + (int)threadIdx.x; i < end; i += kRedThreads) {
+    const int t = i / quads, j = 4 * (i - t * quads);
+    const int32_t a = row_id[t];
+    if (a == kNoAdapter) continue;
+    const float scale = ar.p[proj].scale[a];
+    float4 v[S];
+#pragma unroll
+    for (int q = 0; q < S; ++q) v[q] = ld_cluster_f32x4(part + (t * kRedPitch + j) * 4, q);
+    float4 sum = v[0];
+#pragma unroll
+    for (int q = 1; q < S; ++q) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
+    *reinterpret_cast<uint2*>(ar.p[proj].v + (int64_t)(m0 + t) * r + j) =
+        make_uint2(pack_bf16x2(sum.x * scale, sum.y * scale), pack_bf16x2(sum.z * scale, sum.w * scale));
+  }
+}
 
 __global__ void __launch_bounds__(kRedThreads)
 adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int passes, int stages, DeviceError* err) {
@@ -152,7 +175,6 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int p
   } else {
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const int pitch = rows | 1;
     const int32_t all = quarter == 0 ? id[0] : quarter == 1 ? id[1] : quarter == 2 ? id[2] : id[3];
     const int32_t mine = all >= first && all <= last ? all : kNoAdapter;  // (ascending ids: the pass has all between)
     row_id[row] = mine;
@@ -171,8 +193,9 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int p
           tc_ld8(taddr + i * r + j, v);
           tc_ld_wait();
           if (mine == list[i]) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) part[(j + q) * pitch + row] = __uint_as_float(v[q]);
+            uint4* dst = reinterpret_cast<uint4*>(part + row * kRedPitch + j);
+            dst[0] = make_uint4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_uint4(v[4], v[5], v[6], v[7]);
           }
         }
       }
@@ -183,23 +206,10 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int p
   __syncthreads();
   if (split > 1) cluster_barrier();
   if (!*abort_flag) {
-    const int pitch = rows | 1;
-    const int total = rows * r;
-    const int begin = (int)((int64_t)total * rank / split), end = (int)((int64_t)total * (rank + 1) / split);
-    const uint32_t part_s = smem_u32(part);
-    for (int i = begin + threadIdx.x; i < end; i += kRedThreads) {
-      const int t = i / r, j = i - t * r;
-      const int32_t a = row_id[t];
-      if (a == kNoAdapter) continue;
-      const uint32_t at = part_s + (j * pitch + t) * 4;
-      float acc = 0.f;
-      if (split == 1) {
-        acc = part[j * pitch + t];
-      } else {
-        for (int q = 0; q < split; ++q) acc += ld_cluster_f32(at, q);
-      }
-      ar.p[proj].v[(int64_t)(m0 + t) * r + j] = __float2bfloat16(acc * ar.p[proj].scale[a]);
-    }
+    if (split == 1) add_rows<1>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
+    else if (split == 2) add_rows<2>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
+    else if (split == 4) add_rows<4>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
+    else add_rows<8>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
   }
   __syncthreads();
   if (split > 1) cluster_barrier();  // no CTA leaves while another reads its sums

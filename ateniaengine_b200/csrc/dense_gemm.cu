@@ -25,7 +25,8 @@ constexpr int kTmemCols = 128;
 constexpr int kBBytes = kTileN * BK * 2;
 constexpr int kMaxSplit = 8;
 constexpr int kRingBytes = 100 * 1024;  // two CTAs per SM
-constexpr int kPartBytes = kTileN * 129 * 4;  // f32 sums of a tile [column][row], odd pitch
+constexpr int kPartPitch = kTileN + 4;         // floats: eight lanes' 16-byte accesses fall into different banks
+constexpr int kPartBytes = BM * kPartPitch * 4;  // f32 sums of a tile [row][column]
 static_assert(kPartBytes <= kRingBytes, "the sums take the ring's place");
 
 struct __align__(8) TileBars {
@@ -48,6 +49,33 @@ struct Problems {
 };
 
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 4) << 24);
+
+// This rank's share of a tile whose sums lie in the shared memory of the S CTAs: four columns a thread, columns fastest, all S loads
+// on their way before the first is added; added in rank order.
+template <int EPI, int S>
+__device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, int rows, int cols, uint32_t part, int rank) {
+  constexpr int N_OUT = EPI == kDenseSwiGLU ? kTileN / 2 : kTileN;
+  const int quads = cols / 4, total = rows * quads;
+  const int begin = total * rank / S, end = total * (rank + 1) / S;
+#pragma unroll 1
+  for (int i = begin + (int)threadIdx.x; i < end; i += kTileThreads) {
+    const int r = i / quads, c = 4 * (i - r * quads);
+    const uint32_t at = part + (r * kPartPitch + c) * 4;
+    float4 v[S], v1[EPI == kDenseSwiGLU ? S : 1];
+#pragma unroll
+    for (int q = 0; q < S; ++q) {
+      v[q] = ld_cluster_f32x4(at, q);
+      if constexpr (EPI == kDenseSwiGLU) v1[q] = ld_cluster_f32x4(at + N_OUT * 4, q);
+    }
+    float acc[4] = {}, acc1[4] = {};
+#pragma unroll
+    for (int q = 0; q < S; ++q) {
+      acc[0] += v[q].x, acc[1] += v[q].y, acc[2] += v[q].z, acc[3] += v[q].w;
+      if constexpr (EPI == kDenseSwiGLU) acc1[0] += v1[q].x, acc1[1] += v1[q].y, acc1[2] += v1[q].z, acc1[3] += v1[q].w;
+    }
+    dense_emit4<EPI>(p, at0 + (int64_t)r * p.N + c, acc, acc1);
+  }
+}
 
 template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
 __global__ void __launch_bounds__(kTileThreads)
@@ -286,15 +314,15 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           if (row < rows) dense_emit16<EPI>(p, (int64_t)(m0 + row) * p.N + n0 + c, f, f1);
         }
       } else {
-        const int pitch = rows | 1;
-#pragma unroll 1
+#pragma unroll 2
         for (int c = 0; c < kTileN; c += 16) {
           uint32_t v[16];
           tc_ld16(taddr + c, v);
           tc_ld_wait();
           if (row < rows) {
+            uint4* dst = reinterpret_cast<uint4*>(part + row * kPartPitch + c);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) part[(c + j) * pitch + row] = __uint_as_float(v[j]);
+            for (int j = 0; j < 4; ++j) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
         }
       }
@@ -305,22 +333,11 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   if (split > 1) {
     __syncthreads();
     cluster_barrier();
-    // this rank's share of the tile's elements, columns fastest
     if (!*abort_flag) {
-      const int pitch = rows | 1;
-      const int total = rows * cols;
-      const int begin = (int)((int64_t)total * rank / split), end = (int)((int64_t)total * (rank + 1) / split);
-      const uint32_t part_s = smem_u32(part);
-      for (int i = begin + threadIdx.x; i < end; i += kTileThreads) {
-        const int r = i / cols, c = i - r * cols;
-        const uint32_t at = part_s + (c * pitch + r) * 4;
-        float acc = 0.f, acc1 = 0.f;
-        for (int q = 0; q < split; ++q) {
-          acc += ld_cluster_f32(at, q);
-          if constexpr (EPI == kDenseSwiGLU) acc1 += ld_cluster_f32(at + N_OUT * pitch * 4, q);
-        }
-        dense_emit1<EPI>(p, (int64_t)(m0 + r) * p.N + n0 + c, acc, acc1);
-      }
+      const int64_t at0 = (int64_t)m0 * p.N + n0;
+      if (split == 2) add_parts<EPI, 2>(p, at0, rows, cols, smem_u32(part), rank);
+      else if (split == 4) add_parts<EPI, 4>(p, at0, rows, cols, smem_u32(part), rank);
+      else add_parts<EPI, 8>(p, at0, rows, cols, smem_u32(part), rank);
     }
     __syncthreads();
     cluster_barrier();  // no CTA leaves while another reads its sums
@@ -384,9 +401,9 @@ int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   ta.a_rows = g.a_rows;
   ta.b_early = g.b_early;
   ta.a_early = g.a_early && g.b_early;
-  // clusters until every SM has two CTAs, each with four k-blocks at least
+  // clusters until every SM has a CTA, each with four k-blocks at least
   ta.split = 1;
-  while (ta.split < kMaxSplit && tiles * ta.split < 2 * num_sms && min_kb >= 8 * ta.split) ta.split *= 2;
+  while (ta.split < kMaxSplit && tiles * ta.split < num_sms && min_kb >= 8 * ta.split) ta.split *= 2;
   const int stage_bytes = (g.a_mn ? BM * BK * 2 : g.a_rows * BK * 2) + kBBytes;
   ta.stages = kRingBytes / stage_bytes;
   if (ta.stages > kTileStages) ta.stages = kTileStages;

@@ -143,14 +143,14 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The float at this offset of the shared memory of CTA `rank` of the cluster.
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
-  float v;
+// Four floats at this offset of the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank) {
+  float4 v;
   asm volatile(
       "{\n\t.reg .b32 a;\n\t"
-      "mapa.shared::cluster.u32 a, %1, %2;\n\t"
-      "ld.shared::cluster.f32 %0, [a];\n\t}"
-      : "=f"(v)
+      "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
       : "r"(addr), "r"(rank));
   return v;
 }
@@ -242,23 +242,30 @@ __device__ __forceinline__ void dense_emit16(const DenseProblem& p, int64_t at, 
     store16_bf16(p.out_h + at, h);
   }
 }
-// ... of one element
+// ... of four
 template <int EPI>
-__device__ __forceinline__ void dense_emit1(const DenseProblem& p, int64_t at, float acc, float acc1) {
+__device__ __forceinline__ void dense_emit4(const DenseProblem& p, int64_t at, const float (&acc)[4], const float (&acc1)[4]) {
+  auto store = [&](__nv_bfloat16* dst, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(dst + at) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+  };
   if constexpr (EPI == kDensePlain) {
-    p.out[at] = __float2bfloat16(acc);
+    store(p.out, acc[0], acc[1], acc[2], acc[3]);
   } else if constexpr (EPI == kDenseSwiGLU) {
-    p.out[at] = __float2bfloat16(silu_mul(acc, acc1));
+    store(p.out, silu_mul(acc[0], acc1[0]), silu_mul(acc[1], acc1[1]), silu_mul(acc[2], acc1[2]), silu_mul(acc[3], acc1[3]));
     if (p.gate) {
-      p.gate[at] = acc;
-      p.up[at] = acc1;
+      *reinterpret_cast<float4*>(p.gate + at) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(p.up + at) = make_float4(acc1[0], acc1[1], acc1[2], acc1[3]);
     }
   } else {
-    float dg, du, h;
-    gate_grad(acc, p.gate[at], p.up[at], dg, du, h);
-    p.out[at] = __float2bfloat16(dg);
-    p.out_du[at] = __float2bfloat16(du);
-    p.out_h[at] = __float2bfloat16(h);
+    const float4 g = *reinterpret_cast<const float4*>(p.gate + at), u = *reinterpret_cast<const float4*>(p.up + at);
+    float dg[4], du[4], h[4];
+    gate_grad(acc[0], g.x, u.x, dg[0], du[0], h[0]);
+    gate_grad(acc[1], g.y, u.y, dg[1], du[1], h[1]);
+    gate_grad(acc[2], g.z, u.z, dg[2], du[2], h[2]);
+    gate_grad(acc[3], g.w, u.w, dg[3], du[3], h[3]);
+    store(p.out, dg[0], dg[1], dg[2], dg[3]);
+    store(p.out_du, du[0], du[1], du[2], du[3]);
+    store(p.out_h, h[0], h[1], h[2], h[3]);
   }
 }
 }  // namespace tc
