@@ -382,7 +382,7 @@ int launch_tiles(const DenseGemm& g, const TileArgs& ta, int grid, int smem, cud
 
 }  // namespace
 
-int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
+int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s) {
   TileArgs ta{};
   int rc = dense_error_word(&ta.err);
   if (rc) return rc;
@@ -426,6 +426,15 @@ int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   if (g.epilogue == kDensePlain && g.a_mn && g.b_mn && g.problems == 3)
     return launch_tiles<kDensePlain, true, true, 3, false>(g, ta, grid, smem, s);
   return ATENIA_ERR_UNSUPPORTED;
+}
+
+int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
+  // pairs where every pair of SMs has a tile
+  const int n_out = g.epilogue == kDenseSwiGLU ? 128 : 256;
+  int64_t tiles = 0;
+  for (int i = 0; i < g.problems; ++i) tiles += (int64_t)((g.p[i].M + 255) / 256) * ((g.p[i].N + n_out - 1) / n_out);
+  if ((g.a_mn || g.a_rows == BM) && tiles >= num_sms / 2) return launch_dense_pairs(g, num_sms, s);
+  return launch_dense_tiles(g, num_sms, s);
 }
 
 }  // namespace atenia

@@ -51,7 +51,9 @@ struct DenseGemm {
   bool b_early;                  // B is not written by the kernel before: its first tiles are requested before the wait
   bool a_early;                  // neither is A: only the adapters' v is waited for
 };
-int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);
+int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between the two
+int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_gemm.cu
+int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_pair.cu
 
 // Rows of a K-major A box: all of a small batch, so that a call of few tokens moves few token rows.
 inline int dense_a_rows(int64_t rows) { return rows >= 128 ? 128 : (int)((rows + 7) / 8 * 8); }

@@ -1,0 +1,461 @@
+// Dense products on CTA pairs (tcgen05 cta_group::2): tiles of 256 rows x 256 columns, for calls of many rows.
+//
+// Two CTAs on the two SMs of a TPC stage 128 A rows and half of the 256 B rows each (kDenseSwiGLU: rank 0 the gate rows of 128
+// features, rank 1 their up rows) and the leader issues M256 x N256 x K16 MMAs over both CTAs' shared memory, so that a byte
+// brought to an SM is used for twice the products of a single CTA's tile.  Persistent: one CTA per SM, two accumulators in tensor
+// memory, so that the epilogue of a tile runs under the MMAs of the next.
+//   k-block : 64; a stage is 16 KiB of A and 16 KiB of B per CTA, six stages
+//   order   : bands of kBand row tiles, column tile by column tile, so that the 74 tiles at work at one time share few operand rows in L2
+//   epilogue: eight warps, a lane holds a row: 32 contiguous bytes of the result (and of each saved value 64) per lane and step
+//
+// Adapters as in dense_gemm.cu: behind the k-blocks of a tile come those of the adapters that its rows have, with the lanes
+// of other rows disabled.
+//
+// No TMA multicast is used: every CTA fetches its own tiles (cp.async.bulk.tensor ... cta_group::2 only routes the completion to
+// the leader's mbarrier).  Barriers: full[s] lives in the leader and collects the bytes of both CTAs; empty[s] and acc_full[b] exist
+// in both CTAs and are signalled by tcgen05.commit with a CTA mask; acc_empty[b] lives in the leader and is arrived on by the
+// epilogue warps of both CTAs.
+#include <type_traits>
+
+#include "dense_gemm.cuh"
+
+namespace atenia {
+namespace {
+using namespace tc;
+
+constexpr int kPairM = 256, kPairN = 256;
+constexpr int kPairStages = 6;
+constexpr int kOperandBytes = BM * BK * 2;  // 16 KiB of A, and of B
+constexpr int kPairStageBytes = 2 * kOperandBytes;
+constexpr int kEpiWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;
+constexpr int kPairTmemCols = 512;
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024;
+constexpr int kBand = 8;
+
+struct __align__(8) PairBars {
+  uint64_t full[kPairStages];
+  uint64_t empty[kPairStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+struct PairArgs {
+  int problems, tiles, b_early, a_early;
+  int tile_end[kMaxDenseProblems];
+  DeviceError* err;
+};
+struct NoAdapters {};
+template <int NP>
+struct Problems {
+  DenseProblem p[NP];
+};
+
+constexpr uint32_t kPairIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairM >> 4) << 24);
+
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The following run in a converged warp; one lane (always the same) issues the instruction.
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// The four MMAs of one k-block; `a_step`, `b_step`: descriptor distance of K = 16.
+template <uint64_t A_STEP, uint64_t B_STEP>
+__device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p, t;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+      "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+      "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
+      : "memory");
+}
+__device__ __forceinline__ void mma_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, const uint32_t (&off)[8]) {
+  asm volatile(
+      "{\n\t.reg .pred e, t;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, t;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
+        "r"(off[5]), "r"(off[6]), "r"(off[7])
+      : "memory");
+}
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+  const uint16_t mask = 3;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+      ::"r"(bar), "h"(mask)
+      : "memory");
+}
+
+struct Tile {
+  int which, m0, n0;
+};
+template <int EPI, int NP>
+__device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& pa, int t) {
+  Tile o;
+  o.which = 0;
+  if constexpr (NP > 1) {
+    while (o.which + 1 < pa.problems && t >= pa.tile_end[o.which]) ++o.which;
+    if (o.which > 0) t -= pa.tile_end[o.which - 1];
+  }
+  constexpr int N_OUT = EPI == kDenseSwiGLU ? kPairN / 2 : kPairN;
+  const int m_tiles = (ps.p[o.which].M + kPairM - 1) / kPairM, n_tiles = (ps.p[o.which].N + N_OUT - 1) / N_OUT;
+  const int band = t / (kBand * n_tiles), in_band = t - band * kBand * n_tiles;
+  const int height = min(kBand, m_tiles - band * kBand);
+  const int nt = in_band / height;
+  o.m0 = (band * kBand + in_band - nt * height) * kPairM;
+  o.n0 = nt * N_OUT;
+  return o;
+}
+
+template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ PairArgs pa,
+                  const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PairBars bars;
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int warp = uniform_warp();
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  constexpr int N_OUT = EPI == kDenseSwiGLU ? kPairN / 2 : kPairN;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(smem_u32(&bars.full[s]), 1);
+      mbar_init(smem_u32(&bars.empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&bars.acc_full[b]), 1);
+      mbar_init(smem_u32(&bars.acc_empty[b]), 2 * kEpiWarps);
+    }
+    bars.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
+                 "r"(kPairTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();  // barriers of both CTAs are initialised before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem_base;
+
+  if (warp == 0) {
+    // ================= TMA producer (both CTAs) =================
+    int stage = 0;
+    uint32_t phase = 0, armed = 0;
+    bool ok = true;
+    auto load_b = [&](const DenseProblem& p, const Tile& t, int kb, uint32_t dst, uint32_t bar) {
+      const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
+      const int k = (kb - (seg ? p.kb0 : 0)) * BK;
+      if constexpr (EPI == kDenseSwiGLU) {
+        load_2d(dst, &p.b[rank], bar, k, t.n0);
+        load_2d(dst + 8192, &p.b[rank], bar, k, t.n0 + 64);
+      } else {
+        const int n = t.n0 + (int)rank * 128;
+        load_2d(dst, &p.b[seg], bar, B_MN ? n : k, B_MN ? k : n);
+        load_2d(dst + 8192, &p.b[seg], bar, B_MN ? n + 64 : k, B_MN ? k : n + 64);
+      }
+    };
+    auto load_a = [&](const DenseProblem& p, const Tile& t, int kb, uint32_t dst, uint32_t bar) {
+      const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
+      const int k = (kb - (seg ? p.kb0 : 0)) * BK;
+      const int m = t.m0 + (int)rank * BM;
+      load_2d(dst, &p.a[seg], bar, A_MN ? m : k, A_MN ? k : m);
+      if constexpr (A_MN) load_2d(dst + 8192, &p.a[seg], bar, m + 64, k);
+    };
+    auto free_stage = [&]() {
+      if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
+        if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 2700 + stage);
+        *abort_flag = 1;
+        ok = false;
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    auto next_stage = [&]() {
+      armed |= 1u << stage;
+      if (++stage == kPairStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    };
+    int ahead = 0;
+    if (pa.b_early && pair < pa.tiles) {
+      const Tile t = tile_of<EPI, NP>(ps, pa, pair);
+      const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
+      ahead = min(p.kb, kPairStages);
+      for (int i = 0; i < ahead; ++i) {
+        const uint32_t bar = at_rank(smem_u32(&bars.full[i]), 0), dst = ring + i * kPairStageBytes;
+        if (leader) mbar_expect_tx_one(smem_u32(&bars.full[i]), 2 * kPairStageBytes);
+        load_b(p, t, i, dst + kOperandBytes, bar);
+        if (pa.a_early) load_a(p, t, i, dst, bar);
+      }
+    }
+    if (!(AD && pa.a_early)) chain_wait();
+    for (int i = pair; ok && i < pa.tiles; i += num_pairs) {
+      const Tile t = tile_of<EPI, NP>(ps, pa, i);
+      const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
+      for (int kb = 0; kb < p.kb; ++kb) {
+        const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, 0), dst = ring + stage * kPairStageBytes;
+        if (ahead > 0) {  // (the first tile's first blocks)
+          --ahead;
+          if (!pa.a_early) load_a(p, t, kb, dst, bar);
+        } else {
+          if (!free_stage()) break;
+          if (leader) mbar_expect_tx_one(full, 2 * kPairStageBytes);
+          load_b(p, t, kb, dst + kOperandBytes, bar);
+          load_a(p, t, kb, dst, bar);
+        }
+        next_stage();
+      }
+      if constexpr (AD) {
+        chain_wait();  // v is the kernel before's
+        int32_t id[8];
+        load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
+        int32_t a = -1;
+        while (ok && (a = next_adapter(id, a)) != kNoAdapter) {
+          for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
+            const int r = ad.seg[seg].rank;
+            for (int r0 = 0; ok && r0 < r; r0 += 64) {
+              if (!free_stage()) break;
+              const int steps = (min(r - r0, 64) + 15) / 16;
+              const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, 0), dst = ring + stage * kPairStageBytes;
+              constexpr int b_rows = N_OUT / 2;  // of each CTA
+              if (leader) mbar_expect_tx_one(full, 2 * steps * (BM * 32 + b_rows * 32));
+              const int n = t.n0 + (int)rank * b_rows;
+              for (int c = 0; c < steps; ++c) {
+                load_2d(dst + c * 4096, &ad.seg[seg].v, bar, r0 + 16 * c, t.m0 + (int)rank * BM);
+                load_3d(dst + kOperandBytes + c * 4096, &ad.seg[seg].b, bar, r0 + 16 * c, n, a);
+                if constexpr (EPI != kDenseSwiGLU) load_3d(dst + kOperandBytes + c * 4096 + 2048, &ad.seg[seg].b, bar, r0 + 16 * c, n + 64, a);
+              }
+              next_stage();
+            }
+          }
+        }
+      }
+    }
+    chain_next();  // (every load is on its way: what follows may be launched)
+    if (*abort_flag && leader && lane == 0) {
+      // let the copies already issued (both CTAs') land before the pair's shared memory is released
+      for (int s = 0; s < kPairStages; ++s) {
+        if (!(armed & (1u << s))) continue;
+        const uint32_t par = s < stage ? phase : phase ^ 1u;
+        for (int i = 0; i < (1 << 16) && !mbar_try_wait(smem_u32(&bars.full[s]), par); ++i) {}
+      }
+    }
+  } else if (warp == 1) {
+    // ================= MMA issuer (leader CTA only) =================
+    if (leader) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      bool ok = true;
+      auto filled = [&]() {
+        if (!mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
+          if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 2800 + stage);
+          *abort_flag = 1;
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) tc_fence_after();
+        return ok;
+      };
+      auto used = [&]() {
+        commit_both(smem_u32(&bars.empty[stage]));
+        if (++stage == kPairStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      };
+      constexpr uint32_t idesc = kPairIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kPairN >> 3) << 17);
+      for (int i = pair; ok && i < pa.tiles; i += num_pairs, ++it) {
+        const Tile t = tile_of<EPI, NP>(ps, pa, i);
+        const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
+        int32_t id[8];
+        if constexpr (AD) load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
+        const int acc = it & 1;
+        if (!mbar_wait(smem_u32(&bars.acc_empty[acc]), ((it >> 1) & 1) ^ 1u, abort_flag)) {
+          if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 2900 + acc);
+          *abort_flag = 1;
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * kPairN;
+        for (int kb = 0; kb < p.kb; ++kb) {
+          if (!filled()) break;
+          const uint32_t sa = ring + stage * kPairStageBytes;
+          mma_kblock<kOperandStep<A_MN>, kOperandStep<B_MN>>(d, operand_desc<A_MN>(sa), operand_desc<B_MN>(sa + kOperandBytes), idesc,
+                                                             kb > 0 ? 1u : 0u);
+          used();
+        }
+        if constexpr (AD) {
+          uint32_t off[8];
+          int32_t a = -1;
+          while (ok && (a = next_adapter(id, a)) != kNoAdapter) {
+            lanes_off(off, id, a);
+            for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
+              const int r = ad.seg[seg].rank;
+              for (int r0 = 0; ok && r0 < r; r0 += 64) {
+                if (!filled()) break;
+                const int steps = (min(r - r0, 64) + 15) / 16;
+                const uint32_t sa = ring + stage * kPairStageBytes;
+                constexpr uint32_t idesc_ad = kPairIdesc | (uint32_t(N_OUT >> 3) << 17);
+                for (int c = 0; c < steps; ++c)
+                  mma_lanes(d + seg * N_OUT, make_smem_desc_k16(sa + c * 4096), make_smem_desc_k16(sa + kOperandBytes + c * 4096), idesc_ad,
+                            off);
+                used();
+              }
+            }
+          }
+        }
+        if (ok) commit_both(smem_u32(&bars.acc_full[acc]));
+      }
+    }
+  } else {
+    // ================= epilogue (warps 2..9 of both CTAs) =================
+    chain_wait();
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int row_in = (int)rank * BM + quarter * 32 + lane;
+    int it = 0;
+    for (int i = pair; i < pa.tiles; i += num_pairs, ++it) {
+      const Tile t = tile_of<EPI, NP>(ps, pa, i);
+      const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
+      const int acc = it & 1;
+      const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full[acc]), (it >> 1) & 1, abort_flag));
+      if (!ready) {
+        if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 3000 + acc);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + acc * kPairN + half * (N_OUT / 2);
+      const int row = t.m0 + row_in;
+      const int n = t.n0 + half * (N_OUT / 2);
+      const int cols = min(N_OUT / 2, p.N - n);
+      const int64_t at = (int64_t)row * p.N + n;
+#pragma unroll 1
+      for (int c = 0; c < cols; c += 16) {
+        uint32_t v[16], v1[16];
+        tc_ld16(taddr + c, v);
+        if constexpr (EPI == kDenseSwiGLU) tc_ld16(taddr + N_OUT + c, v1);
+        tc_ld_wait();
+        float f[16], f1[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          f[j] = __uint_as_float(v[j]);
+          f1[j] = EPI == kDenseSwiGLU ? __uint_as_float(v1[j]) : 0.f;
+        }
+        if (row < p.M) dense_emit16<EPI>(p, at + c, f, f1);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(at_rank(smem_u32(&bars.acc_empty[acc]), 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();  // neither CTA leaves while its peer may still signal or read it
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPairTmemCols) : "memory");
+  }
+}
+
+template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
+int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream_t s) {
+  auto kernel = dense_pair_kernel<EPI, A_MN, B_MN, NP, AD>;
+  static bool attr_set[kMaxDevices] = {};
+  if (first_use_on_current_device(attr_set)) {
+    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+  }
+  Problems<NP> ps;
+  for (int i = 0; i < NP; ++i) ps.p[i] = g.p[i];
+  std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
+  if constexpr (AD) ad = *g.adapters;
+  const int pairs = num_sms / 2 < pa.tiles ? num_sms / 2 : pa.tiles;
+  return launch_chained(g.chained, kernel, dim3(2 * pairs), dim3(kPairThreads), kPairSmem, s, ps, pa, ad);
+}
+
+}  // namespace
+
+int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s) {
+  PairArgs pa{};
+  int rc = dense_error_word(&pa.err);
+  if (rc) return rc;
+  const int n_out = g.epilogue == kDenseSwiGLU ? kPairN / 2 : kPairN;
+  int64_t tiles = 0;
+  for (int i = 0; i < g.problems; ++i) {
+    const DenseProblem& p = g.p[i];
+    tiles += (int64_t)((p.M + kPairM - 1) / kPairM) * ((p.N + n_out - 1) / n_out);
+    if (tiles > (1 << 26)) return ATENIA_ERR_SHAPE;
+    pa.tile_end[i] = (int)tiles;
+  }
+  if (tiles == 0) return ATENIA_OK;
+  if (!g.a_mn && g.a_rows != BM) return ATENIA_ERR_SHAPE;
+  pa.problems = g.problems;
+  pa.tiles = (int)tiles;
+  pa.b_early = g.b_early;
+  pa.a_early = g.a_early && g.b_early;
+  count_launch();
+  count_tcgen05_launch();
+  const bool ad = g.adapters != nullptr;
+  if (g.epilogue == kDenseSwiGLU && !g.a_mn && !g.b_mn && g.problems == 1)
+    return ad ? launch_pairs<kDenseSwiGLU, false, false, 1, true>(g, pa, num_sms, s)
+              : launch_pairs<kDenseSwiGLU, false, false, 1, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDensePlain && !g.a_mn && !g.b_mn && g.problems == 1)
+    return ad ? launch_pairs<kDensePlain, false, false, 1, true>(g, pa, num_sms, s)
+              : launch_pairs<kDensePlain, false, false, 1, false>(g, pa, num_sms, s);
+  if (ad) return ATENIA_ERR_UNSUPPORTED;
+  if (g.epilogue == kDenseGateGrad && !g.a_mn && g.b_mn && g.problems == 1)
+    return launch_pairs<kDenseGateGrad, false, true, 1, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDensePlain && !g.a_mn && g.b_mn && g.problems == 1)
+    return launch_pairs<kDensePlain, false, true, 1, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDensePlain && g.a_mn && g.b_mn && g.problems == 3)
+    return launch_pairs<kDensePlain, true, true, 3, false>(g, pa, num_sms, s);
+  return ATENIA_ERR_UNSUPPORTED;
+}
+
+}  // namespace atenia
