@@ -429,6 +429,7 @@ int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s) {
 }
 
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
+  if (dense_gemv_serves(g)) return launch_dense_gemv(g, num_sms, s);
   // pairs where every pair of SMs has a tile
   const int n_out = g.epilogue == kDenseSwiGLU ? 128 : 256;
   int64_t tiles = 0;

@@ -22,6 +22,9 @@ struct DenseProblem {
   __nv_bfloat16* out;      // [M, N]
   float* gate;             // kDenseSwiGLU: g and u [M, N] to be saved, or null; kDenseGateGrad: the saved ones
   float* up;
+  const __nv_bfloat16* a_ptr;     // the same operands for the kernels that read them plainly (dense_gemv.cu)
+  const __nv_bfloat16* b_ptr[2];
+  int K;
   __nv_bfloat16* out_du;   // kDenseGateGrad: du and h [M, N] (dg is `out`)
   __nv_bfloat16* out_h;
 };
@@ -32,6 +35,8 @@ struct AdapterSegment {
   CUtensorMap v;  // [M, rank] bf16, box {16, rows}, 32-byte swizzle
   CUtensorMap b;  // [n, N, rank] bf16, box {16, 64, 1}, 32-byte swizzle
   int rank;
+  const __nv_bfloat16* v_ptr;
+  const __nv_bfloat16* b_ptr;
 };
 struct DenseAdapters {
   AdapterSegment seg[2];
@@ -54,6 +59,9 @@ struct DenseGemm {
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between the two
 int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_gemm.cu
 int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_pair.cu
+int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_gemv.cu, where it serves the product
+bool dense_gemv_serves(const DenseGemm& g);
+constexpr int kGemvTokens = 4;
 
 // Rows of a K-major A box: all of a small batch, so that a call of few tokens moves few token rows.
 inline int dense_a_rows(int64_t rows) { return rows >= 128 ? 128 : (int)((rows + 7) / 8 * 8); }
@@ -65,14 +73,17 @@ struct AdapterReduce {
     const float* scale;  // [n]
     __nv_bfloat16* v;    // [M, rank]
     int rank;
+    const __nv_bfloat16* a_ptr;
   } p[2];
   int projections;
   CUtensorMap x;  // [M, K], box {64, a_rows}
+  const __nv_bfloat16* x_ptr;
   const int32_t* ids;
-  int M, kb, n, a_rows;
+  int M, K, kb, n, a_rows;
   bool chained;
 };
 int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s);
+int launch_adapter_gemv(const AdapterReduce& r, cudaStream_t s);  // dense_gemv.cu, for few tokens
 constexpr int kAdapterMaxRank = 128;
 
 // Where kernels of these files record a wait that gave up: one word per device, read by atenia_ffn_check.

@@ -46,6 +46,19 @@ int matrix_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
   return encode_tmap_bf16(m, base, {(uint64_t)cols, (uint64_t)rows, 0}, {64, (uint32_t)box_rows, 1}, 128);
 }
 
+// A [M, K] and B [N, K] of a product without transposed operands: their maps and plain pointers
+int set_operands(DenseProblem* p, const void* a, const void* b0, const void* b1, int a_rows) {
+  p->a_ptr = static_cast<const __nv_bfloat16*>(a);
+  p->b_ptr[0] = static_cast<const __nv_bfloat16*>(b0);
+  p->b_ptr[1] = static_cast<const __nv_bfloat16*>(b1);
+  p->kb = p->kb0 = kblocks(p->K);
+  if (p->M <= kGemvTokens) return ATENIA_OK;
+  int rc = matrix_map(&p->a[0], a, p->M, p->K, a_rows);
+  if (!rc) rc = matrix_map(&p->b[0], b0, p->N, p->K, 64);
+  if (!rc && b1) rc = matrix_map(&p->b[1], b1, p->N, p->K, 64);
+  return rc;
+}
+
 bool rank_ok(int r) { return r >= 8 && r <= kAdapterMaxRank && r % 8 == 0; }
 int check_adapter(const AteniaLowRank& a) {
   if (!rank_ok(a.rank)) return ATENIA_ERR_SHAPE;
@@ -59,12 +72,16 @@ uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64
 int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, void* v,
                    AdapterReduce::Projection* red, AdapterSegment* seg) {
   const uint64_t r = (uint64_t)a.rank;
-  int rc = encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
-  if (!rc) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {16, (uint32_t)a_rows, 1}, 32);
-  if (!rc) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {16, 64, 1}, 32);
+  const bool few = T <= kGemvTokens;  // (the kernels for few tokens read through plain pointers)
+  int rc = few ? ATENIA_OK : encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
+  if (!rc && !few) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {16, (uint32_t)a_rows, 1}, 32);
+  if (!rc && !few) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {16, 64, 1}, 32);
   red->scale = a.scale;
   red->v = static_cast<__nv_bfloat16*>(v);
   red->rank = seg->rank = a.rank;
+  red->a_ptr = static_cast<const __nv_bfloat16*>(a.a);
+  seg->v_ptr = red->v;
+  seg->b_ptr = static_cast<const __nv_bfloat16*>(a.b);
   return rc;
 }
 
@@ -79,10 +96,12 @@ int plan_adapters(AdapterPlan* p, const AteniaLowRank* const (&sets)[2], const i
   p->red.ids = p->add.ids = ids;
   p->red.n = p->add.n = n;
   p->red.M = (int)T;
+  p->red.K = (int)in;
   p->red.kb = kblocks(in);
+  p->red.x_ptr = static_cast<const __nv_bfloat16*>(x);
   p->red.a_rows = a_rows;
   p->red.chained = chained;
-  int rc = matrix_map(&p->red.x, x, T, in, a_rows);
+  int rc = T <= kGemvTokens ? ATENIA_OK : matrix_map(&p->red.x, x, T, in, a_rows);
   for (int i = 0; i < 2 && !rc; ++i) {
     if (!sets[i] || sets[i]->rank == 0) continue;
     rc = encode_adapter(*sets[i], T, in, out, n, a_rows, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
@@ -170,17 +189,16 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   DenseGemm g1{};
   g1.problems = 1;
   g1.epilogue = kDenseSwiGLU;
+  g1.chained = true;
   g1.a_rows = dense_a_rows(T);
   DenseProblem& p1 = g1.p[0];
   p1.M = T;
   p1.N = d_ff;
-  p1.kb = p1.kb0 = kblocks(d);
+  p1.K = d_model;
   p1.out = h;
   p1.gate = saved_gate;
   p1.up = saved_up;
-  rc = matrix_map(&p1.a[0], x, T, d, g1.a_rows);
-  if (!rc) rc = matrix_map(&p1.b[0], w_gate, F, d, 64);
-  if (!rc) rc = matrix_map(&p1.b[1], w_up, F, d, 64);
+  rc = set_operands(&p1, x, w_gate, w_up, g1.a_rows);
   DenseGemm g2{};
   g2.problems = 1;
   g2.epilogue = kDensePlain;
@@ -189,16 +207,14 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   DenseProblem& p2 = g2.p[0];
   p2.M = T;
   p2.N = d_model;
-  p2.kb = p2.kb0 = kblocks(F);
+  p2.K = d_ff;
   p2.out = static_cast<__nv_bfloat16*>(y);
-  if (!rc) rc = matrix_map(&p2.a[0], h, T, F, g2.a_rows);
-  if (!rc) rc = matrix_map(&p2.b[0], w_down, d, F, 64);
+  if (!rc) rc = set_operands(&p2, h, w_down, nullptr, g2.a_rows);
   if (!rc && ad1) {
-    rc = plan_adapters(&first, {&adapters->gate, &adapters->up}, adapters->ids, adapters->n, x, T, d, F, &ws, false);
+    rc = plan_adapters(&first, {&adapters->gate, &adapters->up}, adapters->ids, adapters->n, x, T, d, F, &ws, true);
     g1.adapters = &first.add;
-    g1.chained = true;
+    g1.b_early = g1.a_early = true;  // (only the adapters' rows are the kernel before's)
   }
-  g1.b_early = g1.a_early = true;  // (only the adapters' rows come from a kernel of this call)
   if (!rc && ad2) {
     rc = plan_adapters(&second, {&adapters->down, nullptr}, adapters->ids, adapters->n, h, T, F, d, &ws, true);
     g2.adapters = &second.add;
@@ -241,7 +257,7 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   g1.epilogue = kDenseGateGrad;
   g1.b_mn = true;
   g1.a_rows = dense_a_rows(T);
-  g1.b_early = g1.a_early = true;
+  g1.chained = true;
   DenseProblem& p1 = g1.p[0];
   p1.M = T;
   p1.N = d_ff;
@@ -313,7 +329,7 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AdapterPlan plan;
-  rc = plan_adapters(&plan, {adapter, nullptr}, ids, n, x, T, d_in, d_out, &ws, false);
+  rc = plan_adapters(&plan, {adapter, nullptr}, ids, n, x, T, d_in, d_out, &ws, true);
   DenseGemm g{};
   g.problems = 1;
   g.epilogue = kDensePlain;
@@ -323,10 +339,9 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   DenseProblem& p = g.p[0];
   p.M = T;
   p.N = d_out;
-  p.kb = p.kb0 = kblocks(d_in);
+  p.K = d_in;
   p.out = static_cast<__nv_bfloat16*>(y);
-  if (!rc) rc = matrix_map(&p.a[0], x, T, d_in, g.a_rows);
-  if (!rc) rc = matrix_map(&p.b[0], weight, d_out, d_in, 64);
+  if (!rc) rc = set_operands(&p, x, weight, nullptr, g.a_rows);
   if (!rc) rc = launch_adapter_reduce(plan.red, sms, s);
   if (!rc) rc = launch_dense_gemm(g, sms, s);
   return rc;

@@ -6,6 +6,7 @@ calls take their workspace from its allocator, on the current stream) and nothin
 step calls `gated_ffn_backward` itself.
 """
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 import torch
@@ -27,19 +28,21 @@ class LowRankAdapters(NamedTuple):
 
 
 def _operand(t, name, shape, dtype, device):
+    """`t`, contiguous, where it is a tensor of this shape and type on this device; else the refusal.  (One test where all is well: the
+    checks of a call cost as much host time as a launch.)"""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
+        return t if t.is_contiguous() else t.contiguous()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, x on {device}")
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{name} is on {t.device}, x on {device}")
 
 
 def _rows(x, name="x"):
-    if not isinstance(x, torch.Tensor) or x.dtype != BF16:
+    if not isinstance(x, torch.Tensor) or x.dtype is not BF16:
         raise TypeError(f"{name} must be a bf16 tensor")
     if x.dim() != 2:
         raise ValueError(f"{name} must be [tokens, width], got {tuple(x.shape)}")
@@ -50,8 +53,8 @@ def _rows(x, name="x"):
 
 def _output(out, shape, x):
     if out is None:
-        return torch.empty(shape, dtype=BF16, device=x.device)
-    if not isinstance(out, torch.Tensor) or out.dtype != BF16 or tuple(out.shape) != shape or out.device != x.device:
+        return torch.empty_like(x) if shape == x.shape else x.new_empty(shape)
+    if not isinstance(out, torch.Tensor) or out.dtype is not BF16 or out.shape != shape or out.device != x.device:
         raise ValueError(f"out must be a bf16 tensor of shape {shape} on {x.device}")
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
@@ -73,8 +76,20 @@ def _low_rank(set_, name, n_in, n_out, device, keep):
     return _lib.LowRank(a.data_ptr(), b.data_ptr(), scale.data_ptr(), rank, 0), n
 
 
-def _workspace(nbytes, device):
-    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+# Bytes of a call's workspace: functions of the sizes alone.
+@functools.lru_cache(maxsize=256)
+def _ffn_bytes(T, d, F, r_gate, r_up, r_down, backward):
+    ranks = _lib.FfnAdapters(gate=_lib.LowRank(rank=r_gate), up=_lib.LowRank(rank=r_up), down=_lib.LowRank(rank=r_down))
+    return _lib.lib().atenia_gated_ffn_workspace_bytes(T, d, F, C.byref(ranks), backward)
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_bytes(T, rank):
+    return _lib.lib().atenia_adapter_linear_workspace_bytes(T, rank)
+
+
+def _workspace(nbytes, x):
+    return x.new_empty(nbytes // 2 or 1)  # (bf16 elements; the sizes are multiples of 256)
 
 
 def _block(x, gate, up, down):
@@ -115,17 +130,19 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
     elif adapter_ids is not None:
         raise ValueError("adapter_ids without adapters")
     y = _output(out, (T, d), x)
-    saved = torch.empty((2, T, F), dtype=torch.float32, device=x.device) if save else None
+    saved, at_gate, at_up = None, None, None
+    if save:
+        saved = x.new_empty((2, T, F), dtype=torch.float32)
+        at_gate = saved.data_ptr()
+        at_up = at_gate + 4 * T * F
+    nbytes = _ffn_bytes(T, d, F, 0, 0, 0, 0) if ad is None else _ffn_bytes(T, d, F, ad.gate.rank, ad.up.rank, ad.down.rank, 0)
+    ws = _workspace(nbytes, x)
     lib = _lib.lib()
-    pad = C.byref(ad) if ad is not None else None
     with _launching(x.device) as st:
-        nbytes = lib.atenia_gated_ffn_workspace_bytes(T, d, F, pad, 0)
-        ws = _workspace(nbytes, x.device)
-        _lib.check(lib.atenia_gated_ffn_forward(x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), T, d, F, pad,
-                                                y.data_ptr(), saved[0].data_ptr() if save else None,
-                                                saved[1].data_ptr() if save else None, ws.data_ptr(), ws.numel(), st), "gated_ffn")
-        if sync:
-            _lib.check(lib.atenia_ffn_check(st), "gated_ffn")
+        rc = lib.atenia_gated_ffn_forward(x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), T, d, F,
+                                          None if ad is None else C.byref(ad), y.data_ptr(), at_gate, at_up, ws.data_ptr(), nbytes, st)
+        if rc or sync:
+            _lib.check(rc or lib.atenia_ffn_check(st), "gated_ffn")
     return (y, saved) if save else y
 
 
@@ -138,16 +155,16 @@ def gated_ffn_backward(dy, x, gate, up, down, saved, sync=False):
     saved = _operand(saved, "saved", (2, T, F), torch.float32, x.device)
     dx = torch.empty_like(x)
     dgate, dup, ddown = torch.empty_like(gate), torch.empty_like(up), torch.empty_like(down)
+    nbytes = _ffn_bytes(T, d, F, 0, 0, 0, 1)
+    ws = _workspace(nbytes, x)
+    at_gate = saved.data_ptr()
     lib = _lib.lib()
     with _launching(x.device) as st:
-        nbytes = lib.atenia_gated_ffn_workspace_bytes(T, d, F, None, 1)
-        ws = _workspace(nbytes, x.device)
-        _lib.check(lib.atenia_gated_ffn_backward(dy.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(),
-                                                 saved[0].data_ptr(), saved[1].data_ptr(), T, d, F, dx.data_ptr(), dgate.data_ptr(),
-                                                 dup.data_ptr(), ddown.data_ptr(), ws.data_ptr(), ws.numel(), st),
-                   "gated_ffn_backward")
-        if sync:
-            _lib.check(lib.atenia_ffn_check(st), "gated_ffn_backward")
+        rc = lib.atenia_gated_ffn_backward(dy.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), at_gate,
+                                           at_gate + 4 * T * F, T, d, F, dx.data_ptr(), dgate.data_ptr(), dup.data_ptr(),
+                                           ddown.data_ptr(), ws.data_ptr(), nbytes, st)
+        if rc or sync:
+            _lib.check(rc or lib.atenia_ffn_check(st), "gated_ffn_backward")
     return dx, dgate, dup, ddown
 
 
@@ -167,11 +184,12 @@ def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
     keep = []
     low, n = _low_rank(adapters, "adapters", n_in, n_out, x.device, keep)
     y = _output(out, (T, n_out), x)
+    nbytes = _linear_bytes(T, low.rank)
+    ws = _workspace(nbytes, x)
     lib = _lib.lib()
     with _launching(x.device) as st:
-        ws = _workspace(lib.atenia_adapter_linear_workspace_bytes(T, low.rank), x.device)
-        _lib.check(lib.atenia_adapter_linear(x.data_ptr(), weight.data_ptr(), T, n_in, n_out, C.byref(low), ids.data_ptr(), n,
-                                             y.data_ptr(), ws.data_ptr(), ws.numel(), st), "adapter_linear")
-        if sync:
-            _lib.check(lib.atenia_ffn_check(st), "adapter_linear")
+        rc = lib.atenia_adapter_linear(x.data_ptr(), weight.data_ptr(), T, n_in, n_out, C.byref(low), ids.data_ptr(), n, y.data_ptr(),
+                                       ws.data_ptr(), nbytes, st)
+        if rc or sync:
+            _lib.check(rc or lib.atenia_ffn_check(st), "adapter_linear")
     return y
