@@ -22,10 +22,6 @@ constexpr int kRedPitch = kAdapterMaxRank + 4;  // floats (see kPartPitch)
 constexpr int kRedPartBytes = BM * kRedPitch * 4;  // f32 sums [row][rank row]
 static_assert(kRedPartBytes <= kRedRingBytes, "");
 
-// The kernel of dense_gemv.cu reads an adapter once per token: for this many tokens and elements of A, over all of them.
-constexpr int kAdapterGemvTokens = 128;
-constexpr int64_t kAdapterGemvElements = (int64_t)32 << 20;
-
 struct __align__(8) RedBars {
   uint64_t full[kRedStages];
   uint64_t empty[kRedStages];
@@ -229,9 +225,7 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int p
 int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s) {
   const int m_tiles = (r.M + BM - 1) / BM;
   if (m_tiles == 0 || r.projections == 0) return ATENIA_OK;
-  int64_t rank_rows = 0;
-  for (int i = 0; i < r.projections; ++i) rank_rows += r.p[i].rank;
-  if (r.M <= kGemvTokens || (r.M <= kAdapterGemvTokens && r.M * rank_rows * r.K <= kAdapterGemvElements)) return launch_adapter_gemv(r, s);
+  if (r.few) return launch_adapter_gemv(r, s);
   DeviceError* err = nullptr;
   int rc = dense_error_word(&err);
   if (rc) return rc;

@@ -61,7 +61,9 @@ int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s);  // den
 int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_pair.cu
 int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_gemv.cu, where it serves the product
 bool dense_gemv_serves(const DenseGemm& g);
-constexpr int kGemvTokens = 4;
+// Two tokens over a large matrix: the tensor-core kernel (dense_gemv.cu has the times).
+constexpr int64_t kGemvTwoElements = (int64_t)1 << 25;
+inline bool dense_gemv_rows(int64_t M, int64_t N, int64_t K) { return M == 1 || (M == 2 && N * K <= kGemvTwoElements); }
 
 // Rows of a K-major A box: all of a small batch, so that a call of few tokens moves few token rows.
 inline int dense_a_rows(int64_t rows) { return rows >= 128 ? 128 : (int)((rows + 7) / 8 * 8); }
@@ -80,10 +82,13 @@ struct AdapterReduce {
   const __nv_bfloat16* x_ptr;
   const int32_t* ids;
   int M, K, kb, n, a_rows;
+  bool few;  // adapter_gemv_rows of every projection: the maps are not encoded
   bool chained;
 };
 int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s);
 int launch_adapter_gemv(const AdapterReduce& r, cudaStream_t s);  // dense_gemv.cu, for few tokens
+// It reads an adapter once per token: up to this many tokens, and elements of A over all of them.
+inline bool adapter_gemv_rows(int64_t M, int64_t rank, int64_t K) { return M <= 128 && M * rank * K <= (int64_t)16 << 20; }
 constexpr int kAdapterMaxRank = 128;
 
 // Where kernels of these files record a wait that gave up: one word per device, read by atenia_ffn_check.

@@ -52,7 +52,7 @@ int set_operands(DenseProblem* p, const void* a, const void* b0, const void* b1,
   p->b_ptr[0] = static_cast<const __nv_bfloat16*>(b0);
   p->b_ptr[1] = static_cast<const __nv_bfloat16*>(b1);
   p->kb = p->kb0 = kblocks(p->K);
-  if (p->M <= kGemvTokens) return ATENIA_OK;
+  if (dense_gemv_rows(p->M, p->N, p->K)) return ATENIA_OK;
   int rc = matrix_map(&p->a[0], a, p->M, p->K, a_rows);
   if (!rc) rc = matrix_map(&p->b[0], b0, p->N, p->K, 64);
   if (!rc && b1) rc = matrix_map(&p->b[1], b1, p->N, p->K, 64);
@@ -69,11 +69,11 @@ int check_adapter(const AteniaLowRank& a) {
 uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64_t)T * rank * 2) : 0; }
 
 // One projection's adapters: the first half's projection and the second half's segment, with v at `v`.
-int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, void* v,
-                   AdapterReduce::Projection* red, AdapterSegment* seg) {
+int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, bool few_reduce,
+                   void* v, AdapterReduce::Projection* red, AdapterSegment* seg) {
   const uint64_t r = (uint64_t)a.rank;
-  const bool few = T <= kGemvTokens;  // (the kernels for few tokens read through plain pointers)
-  int rc = few ? ATENIA_OK : encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
+  const bool few = dense_gemv_rows(T, out, in);  // (the kernels for one or two tokens read through plain pointers)
+  int rc = few_reduce ? ATENIA_OK : encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
   if (!rc && !few) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {16, (uint32_t)a_rows, 1}, 32);
   if (!rc && !few) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {16, 64, 1}, 32);
   red->scale = a.scale;
@@ -101,10 +101,12 @@ int plan_adapters(AdapterPlan* p, const AteniaLowRank* const (&sets)[2], const i
   p->red.x_ptr = static_cast<const __nv_bfloat16*>(x);
   p->red.a_rows = a_rows;
   p->red.chained = chained;
-  int rc = T <= kGemvTokens ? ATENIA_OK : matrix_map(&p->red.x, x, T, in, a_rows);
+  p->red.few = true;
+  for (const AteniaLowRank* a : sets) p->red.few = p->red.few && (!a || adapter_gemv_rows(T, a->rank, in));
+  int rc = p->red.few ? ATENIA_OK : matrix_map(&p->red.x, x, T, in, a_rows);
   for (int i = 0; i < 2 && !rc; ++i) {
     if (!sets[i] || sets[i]->rank == 0) continue;
-    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
+    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, p->red.few, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
     p->red.projections += 1;
     *ws += reduced_bytes(T, sets[i]->rank);
   }
