@@ -18,27 +18,31 @@ namespace atenia {
 namespace {
 using namespace tc;
 
-constexpr int kTileN = 128;
 constexpr int kTileStages = 8;   // at most
-constexpr int kTileThreads = 192;
-constexpr int kTmemCols = 128;
-constexpr int kBBytes = kTileN * BK * 2;
-constexpr int kMaxSplit = 8;
-constexpr int kRingBytes = 100 * 1024;  // two CTAs per SM
-constexpr int kPartPitch = kTileN + 4;         // floats: eight lanes' 16-byte accesses fall into different banks
-constexpr int kPartBytes = BM * kPartPitch * 4;  // f32 sums of a tile [row][column]
-static_assert(kPartBytes <= kRingBytes, "the sums take the ring's place");
+
+template <int BN>
+struct TileSize {
+  static constexpr int kEpiWarps = BN / 32;  // 128 columns a warp and lane quarter at most... two warps a quarter for 256
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kBBytes = BN * BK * 2;
+  static constexpr int kPitch = BN + 4;      // floats of a row of sums: eight lanes' 16-byte accesses fall into different banks
+  static constexpr int kRing = BN == 128 ? 108 * 1024 : 196 * 1024;  // two CTAs per SM, or one
+};
+constexpr int kTileSmemMax = 225 * 1024;
 
 struct __align__(8) TileBars {
   uint64_t full[kTileStages];
   uint64_t empty[kTileStages];
   uint64_t acc_full;
+  uint64_t listed;  // the tile's adapters are in shared memory
+  uint64_t v_full;  // ... and their reduced rows
   uint32_t tmem_base;
   int abort_flag;
 };
 
 struct TileArgs {
   int problems, a_rows, stages, split, b_early, a_early;
+  int v_bytes;                      // of the reduced rows, ahead of the ring
   int tile_end[kMaxDenseProblems];  // tiles of the problems up to and including this one
   DeviceError* err;
 };
@@ -52,15 +56,15 @@ constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >
 
 // This rank's share of a tile whose sums lie in the shared memory of the S CTAs: four columns a thread, columns fastest, all S loads
 // on their way before the first is added; added in rank order.
-template <int EPI, int S>
+template <int EPI, int BN, int S>
 __device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, int rows, int cols, uint32_t part, int rank) {
-  constexpr int N_OUT = EPI == kDenseSwiGLU ? kTileN / 2 : kTileN;
+  constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
   const int quads = cols / 4, total = rows * quads;
   const int begin = total * rank / S, end = total * (rank + 1) / S;
 #pragma unroll 1
-  for (int i = begin + (int)threadIdx.x; i < end; i += kTileThreads) {
+  for (int i = begin + (int)threadIdx.x; i < end; i += TileSize<BN>::kThreads) {
     const int r = i / quads, c = 4 * (i - r * quads);
-    const uint32_t at = part + (r * kPartPitch + c) * 4;
+    const uint32_t at = part + (r * TileSize<BN>::kPitch + c) * 4;
     float4 v[S], v1[EPI == kDenseSwiGLU ? S : 1];
 #pragma unroll
     for (int q = 0; q < S; ++q) {
@@ -77,13 +81,45 @@ __device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, in
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
-__global__ void __launch_bounds__(kTileThreads)
+// The distinct adapters of a tile's rows in the order of their first rows, by the 128 threads of four warps (thread r: row r).
+struct TileList {
+  int32_t id[BM];     // of the rows, kNoAdapter where a row has none
+  int32_t adapter[BM];
+  int32_t count;
+  int32_t in_warp[4];
+};
+__device__ __forceinline__ void list_adapters(TileList& l, const int32_t* __restrict__ ids, int64_t row0, int rows, int n, int w, int lane) {
+  const int r = 32 * w + lane;
+  const int32_t raw = r < rows ? ids[row0 + r] : -1;
+  const int32_t id = raw >= 0 && raw < n ? raw : kNoAdapter;
+  l.id[r] = id;
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  const uint32_t same = __match_any_sync(0xffffffffu, id);  // (every lane: not behind the test)
+  bool first = id != kNoAdapter && (same & ((1u << lane) - 1)) == 0;
+  for (int q = 0; q < 32 * w; ++q) first = first && l.id[q] != id;
+  const uint32_t b = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) l.in_warp[w] = __popc(b);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  int at = __popc(b & ((1u << lane) - 1)), total = 0;
+  for (int q = 0; q < 4; ++q) {
+    if (q < w) at += l.in_warp[q];
+    total += l.in_warp[q];
+  }
+  if (first) l.adapter[at] = id;
+  if (r == 0) l.count = total;
+}
+
+template <int EPI, bool A_MN, bool B_MN, int NP, bool AD, int BN>
+__global__ void __launch_bounds__(TileSize<BN>::kThreads)
 dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ TileArgs ta,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ TileBars bars;
-  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  __shared__ std::conditional_t<AD, TileList, NoAdapters> list;
+  constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
+  constexpr int kChunk = N_OUT * 32;  // a K = 16 step of one adapter's B rows
+  const uint32_t v_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;  // reduced rows, then the ring
+  const uint32_t ring = v_smem + (AD ? ta.v_bytes : 0);
   float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
   volatile int* abort_flag = &bars.abort_flag;
   const int warp = uniform_warp();
@@ -97,7 +133,6 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if (which > 0) tile -= ta.tile_end[which - 1];
   }
   const DenseProblem& p = ps.p[NP > 1 ? which : 0];
-  constexpr int N_OUT = EPI == kDenseSwiGLU ? kTileN / 2 : kTileN;
   const int m_tiles = (p.M + BM - 1) / BM;
   const int nt = tile / m_tiles;  // tiles of the same B rows are neighbours
   const int m0 = (tile - nt * m_tiles) * BM, n0 = nt * N_OUT;
@@ -105,7 +140,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const int kb_begin = (int)((int64_t)p.kb * rank / split), kb_end = (int)((int64_t)p.kb * (rank + 1) / split);
   const int stages = ta.stages;
   const int a_bytes = A_MN ? BM * BK * 2 : ta.a_rows * BK * 2;
-  const int stage_bytes = a_bytes + kBBytes;
+  const int stage_bytes = a_bytes + TileSize<BN>::kBBytes;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -113,12 +148,14 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       mbar_init(smem_u32(&bars.empty[s]), 1);
     }
     mbar_init(smem_u32(&bars.acc_full), 1);
+    mbar_init(smem_u32(&bars.listed), 4);
+    mbar_init(smem_u32(&bars.v_full), 1);
     bars.abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
-                 "r"(kTmemCols)
+                 "r"(BN)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -126,6 +163,25 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
+
+  // Adapters: this rank takes every split-th of the list; an adapter is `steps` K = 16 steps (of both segments), and a stage holds
+  // `slots` of them.
+  constexpr int kSegments = EPI == kDenseSwiGLU ? 2 : 1;
+  int steps0 = 0, steps = 0;
+  const int slots = stage_bytes / kChunk;
+  if constexpr (AD) {
+    steps0 = (ad.seg[0].rank + 15) / 16;
+    steps = steps0 + (kSegments > 1 ? (ad.seg[1].rank + 15) / 16 : 0);
+  }
+  auto give_up = [&](int site) {
+    if (lane == 0) report_error(ta.err, ATENIA_ERR_DEVICE_TIMEOUT, site);
+    *abort_flag = 1;
+    return false;
+  };
+  auto wait_all = [&](uint64_t* bar, uint32_t parity, int site) {
+    const bool ok = mbar_wait(smem_u32(bar), parity, abort_flag) || give_up(site);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
 
   if (warp == 0) {
     // ================= TMA producer =================
@@ -135,15 +191,10 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     auto load_b = [&](int kb, uint32_t dst, uint32_t bar) {
       const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
       const int k = (kb - (seg ? p.kb0 : 0)) * BK;
-      if constexpr (EPI == kDenseSwiGLU) {
-        tma_load_2d_one(dst, &p.b[0], bar, k, n0);
-        tma_load_2d_one(dst + 8192, &p.b[1], bar, k, n0);
-      } else if constexpr (B_MN) {
-        tma_load_2d_one(dst, &p.b[seg], bar, n0, k);
-        tma_load_2d_one(dst + 8192, &p.b[seg], bar, n0 + 64, k);
-      } else {
-        tma_load_2d_one(dst, &p.b[seg], bar, k, n0);
-        tma_load_2d_one(dst + 8192, &p.b[seg], bar, k, n0 + 64);
+#pragma unroll
+      for (int j = 0; j < BN / 64; ++j) {
+        if constexpr (EPI == kDenseSwiGLU) tma_load_2d_one(dst + 8192 * j, &p.b[j >= BN / 128], bar, k, n0 + 64 * (j % (BN / 128)));
+        else tma_load_2d_one(dst + 8192 * j, &p.b[seg], bar, B_MN ? n0 + 64 * j : k, B_MN ? k : n0 + 64 * j);
       }
     };
     auto load_a = [&](int kb, uint32_t dst, uint32_t bar) {
@@ -155,15 +206,6 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       } else {
         tma_load_2d_one(dst, &p.a[seg], bar, k, m0);
       }
-    };
-    auto free_stage = [&]() {
-      if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
-        if (lane == 0) report_error(ta.err, ATENIA_ERR_DEVICE_TIMEOUT, 2100 + stage);
-        *abort_flag = 1;
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      return ok;
     };
     auto next_stage = [&]() {
       armed |= 1u << stage;
@@ -182,13 +224,13 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (ta.a_early) load_a(kb_begin + i, dst, bar);
       }
     }
-    if (!(AD && ta.a_early)) chain_wait();
+    if (!ta.a_early) chain_wait();
     for (int kb = kb_begin; kb < kb_end; ++kb) {
       const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
       if (kb - kb_begin < ahead) {
         if (!ta.a_early) load_a(kb, dst, bar);
       } else {
-        if (!free_stage()) break;
+        if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2100 + stage))) break;
         mbar_expect_tx_one(bar, stage_bytes);
         load_b(kb, dst + a_bytes, bar);
         load_a(kb, dst, bar);
@@ -196,31 +238,30 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       next_stage();
     }
     if constexpr (AD) {
-      chain_wait();  // v is the kernel before's
-      int32_t id[4];
-      load_ids(id, ad.ids, m0, rows, ad.n, lane);
-      int32_t a = -1;
-      for (int i = 0; ok && (a = next_adapter(id, a)) != kNoAdapter; ++i) {
-        if (i % split != rank) continue;
-        for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
-          const int r = ad.seg[seg].rank;
-          for (int r0 = 0; ok && r0 < r; r0 += 64) {
-            if (!free_stage()) break;
-            const int steps = (min(r - r0, 64) + 15) / 16;
-            const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
-            constexpr int b_step = EPI == kDenseSwiGLU ? 2048 : 4096;
-            mbar_expect_tx_one(bar, steps * (ta.a_rows * 32 + b_step));
-            for (int c = 0; c < steps; ++c) {
-              tma_load_2d_one(dst + c * ta.a_rows * 32, &ad.seg[seg].v, bar, r0 + 16 * c, m0);
-              tma_load_3d_one(dst + a_bytes + c * 4096, &ad.seg[seg].b, bar, r0 + 16 * c, n0, a);
-              if constexpr (EPI != kDenseSwiGLU)
-                tma_load_3d_one(dst + a_bytes + c * 4096 + 2048, &ad.seg[seg].b, bar, r0 + 16 * c, n0 + 64, a);
-            }
-            next_stage();
+      // (B is not written by the kernel before; the reduced rows, which are, come with another warp)
+      ok = ok && wait_all(&bars.listed, 0, 2110);
+      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * steps : 0;
+      for (int i = rank, step = 0; left > 0;) {
+        if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2120 + stage))) break;
+        const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
+        const int here = min(left, slots);
+        mbar_expect_tx_one(bar, here * kChunk);
+        for (int s = 0; s < here; ++s) {
+          const int seg = kSegments > 1 && step >= steps0;
+          const int r0 = 16 * (step - (seg ? steps0 : 0));
+#pragma unroll
+          for (int j = 0; j < N_OUT / 64; ++j)
+            tma_load_3d_one(dst + s * kChunk + j * 2048, &ad.seg[seg].b, bar, r0, n0 + 64 * j, list.adapter[i]);
+          if (++step == steps) {
+            step = 0;
+            i += split;
           }
         }
+        left -= here;
+        next_stage();
       }
     }
+    chain_wait();
     chain_next();  // (every load is on its way: what follows may be launched)
     if (*abort_flag && lane == 0) {
       // let the copies already issued land before the shared memory is released
@@ -236,12 +277,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     uint32_t phase = 0;
     bool ok = true;
     auto filled = [&]() {
-      if (!mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
-        if (lane == 0) report_error(ta.err, ATENIA_ERR_DEVICE_TIMEOUT, 2200 + stage);
-        *abort_flag = 1;
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok);
+      ok = wait_all(&bars.full[stage], phase, 2200 + stage);
       if (ok) tc_fence_after();
       return ok;
     };
@@ -252,7 +288,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         phase ^= 1u;
       }
     };
-    constexpr uint32_t idesc = kIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kTileN >> 3) << 17);
+    constexpr uint32_t idesc = kIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(BN >> 3) << 17);
     for (int kb = kb_begin; kb < kb_end; ++kb) {
       if (!filled()) break;
       const uint32_t sa = ring + stage * stage_bytes;
@@ -263,44 +299,70 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       used();
     }
     if constexpr (AD) {
-      int32_t id[4];
-      uint32_t off[4];
-      load_ids(id, ad.ids, m0, rows, ad.n, lane);
-      int32_t a = -1;
-      for (int i = 0; ok && (a = next_adapter(id, a)) != kNoAdapter; ++i) {
-        if (i % split != rank) continue;
-        lanes_off(off, id, a);
-        for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
-          const int r = ad.seg[seg].rank;
-          for (int r0 = 0; ok && r0 < r; r0 += 64) {
-            if (!filled()) break;
-            const int steps = (min(r - r0, 64) + 15) / 16;
-            const uint32_t sa = ring + stage * stage_bytes;
-            constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
-            for (int c = 0; c < steps; ++c)
-              tc_mma_bf16_lanes_one(tmem + seg * N_OUT, make_smem_desc_k16(sa + c * ta.a_rows * 32),
-                                    make_smem_desc_k16(sa + a_bytes + c * 4096), idesc_ad, off);
-            used();
+      ok = ok && wait_all(&bars.listed, 0, 2210);
+      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * steps : 0;
+      if (left > 0) ok = wait_all(&bars.v_full, 0, 2220);
+      uint32_t off[4] = {};
+      for (int i = rank, step = 0; ok && left > 0;) {
+        if (!filled()) break;
+        const uint32_t sb = ring + stage * stage_bytes;
+        const int here = min(left, slots);
+        for (int s = 0; s < here; ++s) {
+          if (step == 0) {
+            const int32_t a = list.adapter[i];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) off[w] = __ballot_sync(0xffffffffu, list.id[32 * w + lane] != a);
+          }
+          const int seg = kSegments > 1 && step >= steps0;
+          constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
+          tc_mma_bf16_lanes_one(tmem + seg * N_OUT, make_smem_desc_k16(v_smem + step * ta.a_rows * 32), make_smem_desc_k16(sb + s * kChunk),
+                                idesc_ad, off);
+          if (++step == steps) {
+            step = 0;
+            i += split;
           }
         }
+        left -= here;
+        used();
       }
     }
     if (ok) tc_commit_one(smem_u32(&bars.acc_full));
   } else {
-    // ================= epilogue (warps 2..5) =================
+    // ================= epilogue =================
+    if constexpr (AD) {
+      if (warp < 6) {
+        list_adapters(list, ad.ids, m0, rows, ad.n, warp - 2, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.listed));
+      }
+    }
     chain_wait();
+    if constexpr (AD) {
+      if (warp == 2 && wait_all(&bars.listed, 0, 2310) && list.count > rank) {
+        const uint32_t bar = smem_u32(&bars.v_full);
+        mbar_expect_tx_one(bar, steps * ta.a_rows * 32);
+        for (int step = 0; step < steps; ++step) {
+          const int seg = kSegments > 1 && step >= steps0;
+          tma_load_2d_one(v_smem + step * ta.a_rows * 32, &ad.seg[seg].v, bar, 16 * (step - (seg ? steps0 : 0)), m0);
+        }
+        if (*abort_flag)
+          for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, 0); ++i) {}
+      }
+    }
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full), 0, abort_flag));
-    if (!ready) {
-      if (lane == 0) report_error(ta.err, ATENIA_ERR_DEVICE_TIMEOUT, 2300);
-      *abort_flag = 1;
+    if (!wait_all(&bars.acc_full, 0, 2300)) {
+      // (reported)
     } else if (quarter * 32 < rows) {
       tc_fence_after();
       const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
+      constexpr int kShares = BN / 128;  // warps of a quarter: each its share of the columns
+      const int share = (warp - 2) >> 2;
       if (split == 1) {
+        constexpr int kCols = N_OUT / kShares;
+        const int end = min(cols, (share + 1) * kCols);
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 16) {
+        for (int c = share * kCols; c < end; c += 16) {
           uint32_t v[16], v1[16];
           tc_ld16(taddr + c, v);
           if constexpr (EPI == kDenseSwiGLU) tc_ld16(taddr + N_OUT + c, v1);
@@ -315,12 +377,12 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         }
       } else {
 #pragma unroll 2
-        for (int c = 0; c < kTileN; c += 16) {
+        for (int c = share * 128; c < share * 128 + 128; c += 16) {
           uint32_t v[16];
           tc_ld16(taddr + c, v);
           tc_ld_wait();
           if (row < rows) {
-            uint4* dst = reinterpret_cast<uint4*>(part + row * kPartPitch + c);
+            uint4* dst = reinterpret_cast<uint4*>(part + row * TileSize<BN>::kPitch + c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
@@ -335,9 +397,16 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     cluster_barrier();
     if (!*abort_flag) {
       const int64_t at0 = (int64_t)m0 * p.N + n0;
-      if (split == 2) add_parts<EPI, 2>(p, at0, rows, cols, smem_u32(part), rank);
-      else if (split == 4) add_parts<EPI, 4>(p, at0, rows, cols, smem_u32(part), rank);
-      else add_parts<EPI, 8>(p, at0, rows, cols, smem_u32(part), rank);
+      const uint32_t at = smem_u32(part);
+      switch (split) {
+        case 2: add_parts<EPI, BN, 2>(p, at0, rows, cols, at, rank); break;
+        case 3: add_parts<EPI, BN, 3>(p, at0, rows, cols, at, rank); break;
+        case 4: add_parts<EPI, BN, 4>(p, at0, rows, cols, at, rank); break;
+        case 5: add_parts<EPI, BN, 5>(p, at0, rows, cols, at, rank); break;
+        case 6: add_parts<EPI, BN, 6>(p, at0, rows, cols, at, rank); break;
+        case 7: add_parts<EPI, BN, 7>(p, at0, rows, cols, at, rank); break;
+        default: add_parts<EPI, BN, 8>(p, at0, rows, cols, at, rank); break;
+      }
     }
     __syncthreads();
     cluster_barrier();  // no CTA leaves while another reads its sums
@@ -347,17 +416,32 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BN) : "memory");
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
-int launch_tiles(const DenseGemm& g, const TileArgs& ta, int grid, int smem, cudaStream_t s) {
-  auto kernel = dense_tile_kernel<EPI, A_MN, B_MN, NP, AD>;
+template <int EPI, bool A_MN, bool B_MN, int NP, bool AD, int BN>
+int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
+  auto kernel = dense_tile_kernel<EPI, A_MN, B_MN, NP, AD, BN>;
   static bool attr_set[kMaxDevices] = {};
   if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024));
+    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemMax));
   }
+  const int rows = A_MN ? BM : g.a_rows;
+  const int stage_bytes = rows * BK * 2 + TileSize<BN>::kBBytes;
+  std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
+  if constexpr (AD) {
+    ad = *g.adapters;
+    const int steps = (ad.seg[0].rank + 15) / 16 + (EPI == kDenseSwiGLU ? (ad.seg[1].rank + 15) / 16 : 0);
+    ta.v_bytes = (steps * rows * 32 + 1023) / 1024 * 1024;
+  }
+  int ring = TileSize<BN>::kRing - ta.v_bytes;
+  if (ring < 3 * stage_bytes) ring = TileSize<256>::kRing - ta.v_bytes;  // (many reduced rows: one CTA per SM)
+  ta.stages = ring / stage_bytes;
+  if (ta.stages > kTileStages) ta.stages = kTileStages;
+  ring = ta.stages * stage_bytes;
+  const int sums = ta.split > 1 ? rows * TileSize<BN>::kPitch * 4 : 0;
+  if (ring < sums) ring = sums;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ta.split;
@@ -365,77 +449,72 @@ int launch_tiles(const DenseGemm& g, const TileArgs& ta, int grid, int smem, cud
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(tiles * ta.split);
+  cfg.blockDim = dim3(TileSize<BN>::kThreads);
+  cfg.dynamicSmemBytes = 1024 + ta.v_bytes + ring;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = g.chained ? 2 : 1;
   Problems<NP> ps;
   for (int i = 0; i < NP; ++i) ps.p[i] = g.p[i];
-  std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
-  if constexpr (AD) ad = *g.adapters;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ps, ta, ad);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return (int)e;
 }
 
+template <int BN>
+int launch_tiles_of(const DenseGemm& g, const TileArgs& ta, int tiles, cudaStream_t s) {
+  const bool ad = g.adapters != nullptr;
+  if (g.epilogue == kDenseSwiGLU && !g.a_mn && !g.b_mn && g.problems == 1)
+    return ad ? launch_tiles<kDenseSwiGLU, false, false, 1, true, BN>(g, ta, tiles, s)
+              : launch_tiles<kDenseSwiGLU, false, false, 1, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDensePlain && !g.a_mn && !g.b_mn && g.problems == 1)
+    return ad ? launch_tiles<kDensePlain, false, false, 1, true, BN>(g, ta, tiles, s)
+              : launch_tiles<kDensePlain, false, false, 1, false, BN>(g, ta, tiles, s);
+  if (ad) return ATENIA_ERR_UNSUPPORTED;
+  if (g.epilogue == kDenseGateGrad && !g.a_mn && g.b_mn && g.problems == 1)
+    return launch_tiles<kDenseGateGrad, false, true, 1, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDensePlain && !g.a_mn && g.b_mn && g.problems == 1)
+    return launch_tiles<kDensePlain, false, true, 1, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDensePlain && g.a_mn && g.b_mn && g.problems == 3)
+    return launch_tiles<kDensePlain, true, true, 3, false, BN>(g, ta, tiles, s);
+  return ATENIA_ERR_UNSUPPORTED;
+}
+
 }  // namespace
 
-int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s) {
+int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s) {
+  if (split < 1 || split > 8 || (columns != 128 && columns != 256)) return ATENIA_ERR_SHAPE;
   TileArgs ta{};
   int rc = dense_error_word(&ta.err);
   if (rc) return rc;
-  const int n_out = g.epilogue == kDenseSwiGLU ? kTileN / 2 : kTileN;
+  const int n_out = g.epilogue == kDenseSwiGLU ? columns / 2 : columns;
   int64_t tiles = 0;
-  int min_kb = 1 << 30;
   for (int i = 0; i < g.problems; ++i) {
     const DenseProblem& p = g.p[i];
     tiles += (int64_t)((p.M + BM - 1) / BM) * ((p.N + n_out - 1) / n_out);
-    if (tiles > (1 << 26)) return ATENIA_ERR_SHAPE;
+    if (tiles * split > (1 << 28)) return ATENIA_ERR_SHAPE;
+    if (p.kb < split) return ATENIA_ERR_SHAPE;
     ta.tile_end[i] = (int)tiles;
-    if (p.kb < min_kb) min_kb = p.kb;
   }
   if (tiles == 0) return ATENIA_OK;
   ta.problems = g.problems;
   ta.a_rows = g.a_rows;
   ta.b_early = g.b_early;
   ta.a_early = g.a_early && g.b_early;
-  // clusters until every SM has a CTA, each with four k-blocks at least
-  ta.split = 1;
-  while (ta.split < kMaxSplit && tiles * ta.split < num_sms && min_kb >= 8 * ta.split) ta.split *= 2;
-  const int stage_bytes = (g.a_mn ? BM * BK * 2 : g.a_rows * BK * 2) + kBBytes;
-  ta.stages = kRingBytes / stage_bytes;
-  if (ta.stages > kTileStages) ta.stages = kTileStages;
-  const int grid = (int)tiles * ta.split;
-  const int smem = kRingBytes + 1024;
+  ta.split = split;
   count_launch();
   count_tcgen05_launch();
-  const bool ad = g.adapters != nullptr;
-  if (g.epilogue == kDenseSwiGLU && !g.a_mn && !g.b_mn && g.problems == 1)
-    return ad ? launch_tiles<kDenseSwiGLU, false, false, 1, true>(g, ta, grid, smem, s)
-              : launch_tiles<kDenseSwiGLU, false, false, 1, false>(g, ta, grid, smem, s);
-  if (g.epilogue == kDensePlain && !g.a_mn && !g.b_mn && g.problems == 1)
-    return ad ? launch_tiles<kDensePlain, false, false, 1, true>(g, ta, grid, smem, s)
-              : launch_tiles<kDensePlain, false, false, 1, false>(g, ta, grid, smem, s);
-  if (ad) return ATENIA_ERR_UNSUPPORTED;
-  if (g.epilogue == kDenseGateGrad && !g.a_mn && g.b_mn && g.problems == 1)
-    return launch_tiles<kDenseGateGrad, false, true, 1, false>(g, ta, grid, smem, s);
-  if (g.epilogue == kDensePlain && !g.a_mn && g.b_mn && g.problems == 1)
-    return launch_tiles<kDensePlain, false, true, 1, false>(g, ta, grid, smem, s);
-  if (g.epilogue == kDensePlain && g.a_mn && g.b_mn && g.problems == 3)
-    return launch_tiles<kDensePlain, true, true, 3, false>(g, ta, grid, smem, s);
-  return ATENIA_ERR_UNSUPPORTED;
+  return columns == 256 ? launch_tiles_of<256>(g, ta, (int)tiles, s) : launch_tiles_of<128>(g, ta, (int)tiles, s);
 }
 
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   if (dense_gemv_serves(g)) return launch_dense_gemv(g, num_sms, s);
-  // pairs where every pair of SMs has a tile
-  const int n_out = g.epilogue == kDenseSwiGLU ? 128 : 256;
-  int64_t tiles = 0;
-  for (int i = 0; i < g.problems; ++i) tiles += (int64_t)((g.p[i].M + 255) / 256) * ((g.p[i].N + n_out - 1) / n_out);
-  if ((g.a_mn || g.a_rows == BM) && tiles >= num_sms / 2) return launch_dense_pairs(g, num_sms, s);
-  return launch_dense_tiles(g, num_sms, s);
+  DenseSize sizes[kMaxDenseProblems];
+  for (int i = 0; i < g.problems; ++i) sizes[i] = {g.p[i].M, g.p[i].N, g.p[i].kb};
+  const DensePlan plan = dense_plan(sizes, g.problems, g.epilogue == kDenseSwiGLU, g.a_mn || g.a_rows == BM, num_sms);
+  if (plan.pairs) return launch_dense_pairs(g, num_sms, s);
+  return launch_dense_tiles(g, plan.columns, plan.split, s);
 }
 
 }  // namespace atenia

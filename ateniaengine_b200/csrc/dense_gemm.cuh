@@ -6,6 +6,7 @@
 // reads of the backward pass, where the reduction runs over the rows of a row-major matrix).  Both come through TMA into
 // 128-byte-swizzled tiles and the MMA reads either, so nothing is transposed in memory.
 #pragma once
+#include "dense_choice.cuh"
 #include "tc_common.cuh"
 
 namespace atenia {
@@ -57,7 +58,7 @@ struct DenseGemm {
   bool a_early;                  // neither is A: only the adapters' v is waited for
 };
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between the two
-int launch_dense_tiles(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_gemm.cu
+int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s);  // dense_gemm.cu
 int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_pair.cu
 int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_gemv.cu, where it serves the product
 bool dense_gemv_serves(const DenseGemm& g);
