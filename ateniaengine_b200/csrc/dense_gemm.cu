@@ -25,7 +25,6 @@ struct TileSize {
   static constexpr int kEpiWarps = BN / 32;  // 128 columns a warp and lane quarter at most... two warps a quarter for 256
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kBBytes = BN * BK * 2;
-  static constexpr int kPitch = BN + 4;      // floats of a row of sums: eight lanes' 16-byte accesses fall into different banks
   static constexpr int kRing = BN == 128 ? 108 * 1024 : 196 * 1024;  // two CTAs per SM, or one
 };
 constexpr int kTileSmemMax = 225 * 1024;
@@ -53,33 +52,6 @@ struct Problems {
 };
 
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 4) << 24);
-
-// This rank's share of a tile whose sums lie in the shared memory of the S CTAs: four columns a thread, columns fastest, all S loads
-// on their way before the first is added; added in rank order.
-template <int EPI, int BN, int S>
-__device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, int rows, int cols, uint32_t part, int rank) {
-  constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
-  const int quads = cols / 4, total = rows * quads;
-  const int begin = total * rank / S, end = total * (rank + 1) / S;
-#pragma unroll 1
-  for (int i = begin + (int)threadIdx.x; i < end; i += TileSize<BN>::kThreads) {
-    const int r = i / quads, c = 4 * (i - r * quads);
-    const uint32_t at = part + (r * TileSize<BN>::kPitch + c) * 4;
-    float4 v[S], v1[EPI == kDenseSwiGLU ? S : 1];
-#pragma unroll
-    for (int q = 0; q < S; ++q) {
-      v[q] = ld_cluster_f32x4(at, q);
-      if constexpr (EPI == kDenseSwiGLU) v1[q] = ld_cluster_f32x4(at + N_OUT * 4, q);
-    }
-    float acc[4] = {}, acc1[4] = {};
-#pragma unroll
-    for (int q = 0; q < S; ++q) {
-      acc[0] += v[q].x, acc[1] += v[q].y, acc[2] += v[q].z, acc[3] += v[q].w;
-      if constexpr (EPI == kDenseSwiGLU) acc1[0] += v1[q].x, acc1[1] += v1[q].y, acc1[2] += v1[q].z, acc1[3] += v1[q].w;
-    }
-    dense_emit4<EPI>(p, at0 + (int64_t)r * p.N + c, acc, acc1);
-  }
-}
 
 // The distinct adapters of a tile's rows in the order of their first rows, by the 128 threads of four warps (thread r: row r).
 struct TileList {
@@ -382,7 +354,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           tc_ld16(taddr + c, v);
           tc_ld_wait();
           if (row < rows) {
-            uint4* dst = reinterpret_cast<uint4*>(part + row * TileSize<BN>::kPitch + c);
+            uint4* dst = reinterpret_cast<uint4*>(part + row * kSumsPitch<BN> + c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
@@ -399,13 +371,11 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       const int64_t at0 = (int64_t)m0 * p.N + n0;
       const uint32_t at = smem_u32(part);
       switch (split) {
-        case 2: add_parts<EPI, BN, 2>(p, at0, rows, cols, at, rank); break;
-        case 3: add_parts<EPI, BN, 3>(p, at0, rows, cols, at, rank); break;
-        case 4: add_parts<EPI, BN, 4>(p, at0, rows, cols, at, rank); break;
-        case 5: add_parts<EPI, BN, 5>(p, at0, rows, cols, at, rank); break;
-        case 6: add_parts<EPI, BN, 6>(p, at0, rows, cols, at, rank); break;
-        case 7: add_parts<EPI, BN, 7>(p, at0, rows, cols, at, rank); break;
-        default: add_parts<EPI, BN, 8>(p, at0, rows, cols, at, rank); break;
+        case 2: add_parts<EPI, BN, 2, 1>(p, at0, rows, cols, at, rank, 0); break;
+        case 3: add_parts<EPI, BN, 3, 1>(p, at0, rows, cols, at, rank, 0); break;
+        case 4: add_parts<EPI, BN, 4, 1>(p, at0, rows, cols, at, rank, 0); break;
+        case 6: add_parts<EPI, BN, 6, 1>(p, at0, rows, cols, at, rank, 0); break;
+        default: add_parts<EPI, BN, 8, 1>(p, at0, rows, cols, at, rank, 0); break;
       }
     }
     __syncthreads();
@@ -440,7 +410,7 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
   ta.stages = ring / stage_bytes;
   if (ta.stages > kTileStages) ta.stages = kTileStages;
   ring = ta.stages * stage_bytes;
-  const int sums = ta.split > 1 ? rows * TileSize<BN>::kPitch * 4 : 0;
+  const int sums = ta.split > 1 ? rows * kSumsPitch<BN> * 4 : 0;
   if (ring < sums) ring = sums;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -484,7 +454,7 @@ int launch_tiles_of(const DenseGemm& g, const TileArgs& ta, int tiles, cudaStrea
 }  // namespace
 
 int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s) {
-  if (split < 1 || split > 8 || (columns != 128 && columns != 256)) return ATENIA_ERR_SHAPE;
+  if (split < 1 || split > 8 || split == 5 || split == 7 || (columns != 128 && columns != 256)) return ATENIA_ERR_SHAPE;
   TileArgs ta{};
   int rc = dense_error_word(&ta.err);
   if (rc) return rc;
@@ -513,7 +483,7 @@ int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   DenseSize sizes[kMaxDenseProblems];
   for (int i = 0; i < g.problems; ++i) sizes[i] = {g.p[i].M, g.p[i].N, g.p[i].kb};
   const DensePlan plan = dense_plan(sizes, g.problems, g.epilogue == kDenseSwiGLU, g.a_mn || g.a_rows == BM, num_sms);
-  if (plan.pairs) return launch_dense_pairs(g, num_sms, s);
+  if (plan.pairs) return launch_dense_pairs(g, plan.split, num_sms, s);
   return launch_dense_tiles(g, plan.columns, plan.split, s);
 }
 

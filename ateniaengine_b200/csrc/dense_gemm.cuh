@@ -59,7 +59,7 @@ struct DenseGemm {
 };
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between the two
 int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s);  // dense_gemm.cu
-int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s);  // dense_pair.cu
+int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t s);  // dense_pair.cu
 int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_gemv.cu, where it serves the product
 bool dense_gemv_serves(const DenseGemm& g);
 // Two tokens over a large matrix: the tensor-core kernel (dense_gemv.cu has the times).
@@ -285,6 +285,47 @@ __device__ __forceinline__ void dense_emit4(const DenseProblem& p, int64_t at, c
     store(p.out, dg[0], dg[1], dg[2], dg[3]);
     store(p.out_du, du[0], du[1], du[2], du[3]);
     store(p.out_h, h[0], h[1], h[2], h[3]);
+  }
+}
+// Sums of a tile in shared memory, [row][column]: floats of a row, so that eight lanes' 16-byte accesses fall into different banks
+template <int COLUMNS>
+constexpr int kSumsPitch = COLUMNS + 4;
+// Share `share` of S of a tile whose sums lie in the shared memory of S CTAs (ranks first, first + STEP, ...): four columns at a time,
+// columns fastest, added in rank order.  A thread has 16 loads on their way: one after another they cost more than the products of a
+// whole k-block each (1021 x 2048 over 5632, two pairs a tile: 23.5 -> XX us).
+template <int EPI, int BN, int S, int STEP>
+__device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, int rows, int cols, uint32_t part, int share, int first) {
+  constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
+  constexpr int kHalves = EPI == kDenseSwiGLU ? 2 : 1;
+  constexpr int U = 16 / (S * kHalves) > 0 ? 16 / (S * kHalves) : 1;
+  const int quads = cols / 4, total = rows * quads;
+  const int begin = total * share / S, end = total * (share + 1) / S;
+#pragma unroll 1
+  for (int i0 = begin + (int)threadIdx.x; i0 < end; i0 += U * (int)blockDim.x) {
+    float4 v[U][kHalves][S];
+    int at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * (int)blockDim.x, end - 1);
+      const int r = i / quads, c = 4 * (i - r * quads);
+      at[u] = r * p.N + c;
+#pragma unroll
+      for (int q = 0; q < S; ++q)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) v[u][h][q] = ld_cluster_f32x4(part + (r * kSumsPitch<BN> + c + h * N_OUT) * 4, first + STEP * q);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float acc[2][4] = {};
+#pragma unroll
+      for (int q = 0; q < S; ++q)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          acc[h][0] += v[u][h][q].x, acc[h][1] += v[u][h][q].y;
+          acc[h][2] += v[u][h][q].z, acc[h][3] += v[u][h][q].w;
+        }
+      if (i0 + u * (int)blockDim.x < end) dense_emit4<EPI>(p, at0 + at[u], acc[0], acc[1]);
+    }
   }
 }
 }  // namespace tc

@@ -2,10 +2,12 @@
 //
 // Two CTAs on the two SMs of a TPC stage 128 A rows and half of the 256 B rows each (kDenseSwiGLU: rank 0 the gate rows of 128
 // features, rank 1 their up rows) and the leader issues M256 x N256 x K16 MMAs over both CTAs' shared memory, so that a byte
-// brought to an SM is used for twice the products of a single CTA's tile.  Persistent: one CTA per SM, two accumulators in tensor
-// memory, so that the epilogue of a tile runs under the MMAs of the next.
+// brought to an SM is used for twice the products of a single CTA's tile (whose MMAs wait for shared memory: 128 x 256 of one CTA
+// reads and writes 192 bytes a cycle at full rate, a pair 128).  Persistent: one CTA per SM, two accumulators in tensor memory, so that the epilogue of a tile runs under the MMAs of the next.
 //   k-block : 64; a stage is 16 KiB of A and 16 KiB of B per CTA, six stages
 //   order   : bands of kBand row tiles, column tile by column tile, so that the 74 tiles at work at one time share few operand rows in L2
+//   split   : where the tiles are too few, the pairs of a cluster (two, three or four) share a tile: consecutive k ranges, added through
+//             distributed shared memory in rank order
 //   epilogue: eight warps, a lane holds a row: 32 contiguous bytes of the result (and of each saved value 64) per lane and step
 //
 // Adapters as in dense_gemm.cu: behind the k-blocks of a tile come those of the adapters that its rows have, with the lanes
@@ -42,7 +44,7 @@ struct __align__(8) PairBars {
   int abort_flag;
 };
 struct PairArgs {
-  int problems, tiles, b_early, a_early;
+  int problems, tiles, split, b_early, a_early;
   int tile_end[kMaxDenseProblems];
   DeviceError* err;
 };
@@ -108,8 +110,8 @@ __device__ __forceinline__ void mma_lanes(uint32_t d_tmem, uint64_t a_desc, uint
         "r"(off[5]), "r"(off[6]), "r"(off[7])
       : "memory");
 }
-__device__ __forceinline__ void commit_both(uint32_t bar) {
-  const uint16_t mask = 3;
+__device__ __forceinline__ void commit_both(uint32_t bar, uint32_t lead) {
+  const uint16_t mask = (uint16_t)(3u << lead);
   asm volatile(
       "{\n\t.reg .pred e;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
@@ -140,19 +142,28 @@ __device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& 
 }
 
 template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ PairArgs pa,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PairBars bars;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
   volatile int* abort_flag = &bars.abort_flag;
   const int warp = uniform_warp();
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  const uint32_t in_cluster = cluster_rank();
+  const uint32_t rank = in_cluster & 1, lead = in_cluster & ~1u;  // of the pair
   const bool leader = rank == 0;
-  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  // split 1: a pair walks the tiles; else the `split` pairs of a cluster share one tile's reduction
+  const int split = pa.split;
+  const int pair = split > 1 ? (int)(blockIdx.x >> 1) / split : (int)(blockIdx.x >> 1);
+  const int num_pairs = split > 1 ? pa.tiles : (int)(gridDim.x >> 1);
+  const int piece = split > 1 ? (int)(in_cluster >> 1) : 0;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? kPairN / 2 : kPairN;
+
+  auto kb_begin = [&](const DenseProblem& p) { return (int)((int64_t)p.kb * piece / split); };
+  auto kb_end = [&](const DenseProblem& p) { return (int)((int64_t)p.kb * (piece + 1) / split); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
@@ -222,20 +233,21 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if (pa.b_early && pair < pa.tiles) {
       const Tile t = tile_of<EPI, NP>(ps, pa, pair);
       const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
-      ahead = min(p.kb, kPairStages);
+      const int kb0 = kb_begin(p);
+      ahead = min(kb_end(p) - kb0, kPairStages);
       for (int i = 0; i < ahead; ++i) {
-        const uint32_t bar = at_rank(smem_u32(&bars.full[i]), 0), dst = ring + i * kPairStageBytes;
+        const uint32_t bar = at_rank(smem_u32(&bars.full[i]), lead), dst = ring + i * kPairStageBytes;
         if (leader) mbar_expect_tx_one(smem_u32(&bars.full[i]), 2 * kPairStageBytes);
-        load_b(p, t, i, dst + kOperandBytes, bar);
-        if (pa.a_early) load_a(p, t, i, dst, bar);
+        load_b(p, t, kb0 + i, dst + kOperandBytes, bar);
+        if (pa.a_early) load_a(p, t, kb0 + i, dst, bar);
       }
     }
     if (!(AD && pa.a_early)) chain_wait();
     for (int i = pair; ok && i < pa.tiles; i += num_pairs) {
       const Tile t = tile_of<EPI, NP>(ps, pa, i);
       const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
-      for (int kb = 0; kb < p.kb; ++kb) {
-        const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, 0), dst = ring + stage * kPairStageBytes;
+      for (int kb = kb_begin(p), end = kb_end(p); kb < end; ++kb) {
+        const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
         if (ahead > 0) {  // (the first tile's first blocks)
           --ahead;
           if (!pa.a_early) load_a(p, t, kb, dst, bar);
@@ -252,13 +264,14 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         int32_t id[8];
         load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
         int32_t a = -1;
-        while (ok && (a = next_adapter(id, a)) != kNoAdapter) {
+        for (int i_ad = 0; ok && (a = next_adapter(id, a)) != kNoAdapter; ++i_ad) {
+          if (i_ad % split != piece) continue;
           for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
             const int r = ad.seg[seg].rank;
             for (int r0 = 0; ok && r0 < r; r0 += 64) {
               if (!free_stage()) break;
               const int steps = (min(r - r0, 64) + 15) / 16;
-              const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, 0), dst = ring + stage * kPairStageBytes;
+              const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
               constexpr int b_rows = N_OUT / 2;  // of each CTA
               if (leader) mbar_expect_tx_one(full, 2 * steps * (BM * 32 + b_rows * 32));
               const int n = t.n0 + (int)rank * b_rows;
@@ -300,7 +313,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         return ok;
       };
       auto used = [&]() {
-        commit_both(smem_u32(&bars.empty[stage]));
+        commit_both(smem_u32(&bars.empty[stage]), lead);
         if (++stage == kPairStages) {
           stage = 0;
           phase ^= 1u;
@@ -322,17 +335,19 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * kPairN;
-        for (int kb = 0; kb < p.kb; ++kb) {
+        const int begin = kb_begin(p), end = kb_end(p);
+        for (int kb = begin; kb < end; ++kb) {
           if (!filled()) break;
           const uint32_t sa = ring + stage * kPairStageBytes;
           mma_kblock<kOperandStep<A_MN>, kOperandStep<B_MN>>(d, operand_desc<A_MN>(sa), operand_desc<B_MN>(sa + kOperandBytes), idesc,
-                                                             kb > 0 ? 1u : 0u);
+                                                             kb > begin ? 1u : 0u);
           used();
         }
         if constexpr (AD) {
           uint32_t off[8];
           int32_t a = -1;
-          while (ok && (a = next_adapter(id, a)) != kNoAdapter) {
+          for (int i_ad = 0; ok && (a = next_adapter(id, a)) != kNoAdapter; ++i_ad) {
+            if (i_ad % split != piece) continue;
             lanes_off(off, id, a);
             for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
               const int r = ad.seg[seg].rank;
@@ -349,7 +364,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
             }
           }
         }
-        if (ok) commit_both(smem_u32(&bars.acc_full[acc]));
+        if (ok) commit_both(smem_u32(&bars.acc_full[acc]), lead);
       }
     }
   } else {
@@ -374,6 +389,20 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       const int n = t.n0 + half * (N_OUT / 2);
       const int cols = min(N_OUT / 2, p.N - n);
       const int64_t at = (int64_t)row * p.N + n;
+      if (split > 1) {  // (one tile: the sums go to the ring, which nothing uses any more)
+        float* mine = part + (quarter * 32 + lane) * kSumsPitch<kPairN> + half * 128;
+        const uint32_t from = tmem + (uint32_t(quarter * 32) << 16) + half * 128;
+#pragma unroll 2
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t v[16];
+          tc_ld16(from + c, v);
+          tc_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            reinterpret_cast<uint4*>(mine + c)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+        break;
+      }
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {
         uint32_t v[16], v1[16];
@@ -390,13 +419,27 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_remote(at_rank(smem_u32(&bars.acc_empty[acc]), 0));
+      if (lane == 0) arrive_remote(at_rank(smem_u32(&bars.acc_empty[acc]), lead));
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  cluster_barrier();  // neither CTA leaves while its peer may still signal or read it
+  if (split > 1) {
+    cluster_barrier();
+    if (!*abort_flag) {
+      const Tile t = tile_of<EPI, NP>(ps, pa, pair);
+      const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
+      const int m0 = t.m0 + (int)rank * BM;
+      const int rows = max(0, min(BM, p.M - m0)), cols = min(N_OUT, p.N - t.n0);
+      const int64_t at0 = (int64_t)m0 * p.N + t.n0;
+      if (split == 2) add_parts<EPI, kPairN, 2, 2>(p, at0, rows, cols, smem_u32(part), piece, rank);
+      else if (split == 3) add_parts<EPI, kPairN, 3, 2>(p, at0, rows, cols, smem_u32(part), piece, rank);
+      else add_parts<EPI, kPairN, 4, 2>(p, at0, rows, cols, smem_u32(part), piece, rank);
+    }
+    __syncthreads();
+  }
+  cluster_barrier();  // no CTA leaves while its peers may still signal or read it
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -415,13 +458,29 @@ int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream
   for (int i = 0; i < NP; ++i) ps.p[i] = g.p[i];
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
   if constexpr (AD) ad = *g.adapters;
-  const int pairs = num_sms / 2 < pa.tiles ? num_sms / 2 : pa.tiles;
-  return launch_chained(g.chained, kernel, dim3(2 * pairs), dim3(kPairThreads), kPairSmem, s, ps, pa, ad);
+  const int pairs = pa.split > 1 ? pa.tiles * pa.split : num_sms / 2 < pa.tiles ? num_sms / 2 : pa.tiles;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2 * pa.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = g.chained ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ps, pa, ad);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return (int)e;
 }
 
 }  // namespace
 
-int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s) {
+int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t s) {
+  if (split < 1 || split > 4) return ATENIA_ERR_SHAPE;
   PairArgs pa{};
   int rc = dense_error_word(&pa.err);
   if (rc) return rc;
@@ -430,13 +489,14 @@ int launch_dense_pairs(const DenseGemm& g, int num_sms, cudaStream_t s) {
   for (int i = 0; i < g.problems; ++i) {
     const DenseProblem& p = g.p[i];
     tiles += (int64_t)((p.M + kPairM - 1) / kPairM) * ((p.N + n_out - 1) / n_out);
-    if (tiles > (1 << 26)) return ATENIA_ERR_SHAPE;
+    if (tiles > (1 << 26) || p.kb < split) return ATENIA_ERR_SHAPE;
     pa.tile_end[i] = (int)tiles;
   }
   if (tiles == 0) return ATENIA_OK;
   if (!g.a_mn && g.a_rows != BM) return ATENIA_ERR_SHAPE;
   pa.problems = g.problems;
   pa.tiles = (int)tiles;
+  pa.split = split;
   pa.b_early = g.b_early;
   pa.a_early = g.a_early && g.b_early;
   count_launch();
