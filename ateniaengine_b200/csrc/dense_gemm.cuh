@@ -174,6 +174,12 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank)
   return v;
 }
 
+__device__ __forceinline__ float4 ld_shared_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
 constexpr int kNoAdapter = 0x7fffffff;
 // The ids of 32 * W token rows from `row0` on, W per lane; kNoAdapter where a row is past the end or has none.
 template <int W>
@@ -208,32 +214,36 @@ __device__ __forceinline__ void gate_grad(float dh, float g, float u, float& dg,
   du = dh * (g * s);
   h = silu_mul(g, u);
 }
-// 16 values of one row to consecutive bf16 (32 bytes; 16-byte aligned)
+// 32 bytes of one row: lanes hold rows, so each 32-byte access of a warp is a line of its own and two of 16 bytes cost twice as much
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// 16 values of one row to consecutive bf16
 __device__ __forceinline__ void store16_bf16(__nv_bfloat16* dst, const float (&v)[16]) {
-  uint4 a, b;
-  a.x = pack_bf16x2(v[0], v[1]);
-  a.y = pack_bf16x2(v[2], v[3]);
-  a.z = pack_bf16x2(v[4], v[5]);
-  a.w = pack_bf16x2(v[6], v[7]);
-  b.x = pack_bf16x2(v[8], v[9]);
-  b.y = pack_bf16x2(v[10], v[11]);
-  b.z = pack_bf16x2(v[12], v[13]);
-  b.w = pack_bf16x2(v[14], v[15]);
-  reinterpret_cast<uint4*>(dst)[0] = a;
-  reinterpret_cast<uint4*>(dst)[1] = b;
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  store32(dst, w);
 }
 __device__ __forceinline__ void store16_f32(float* dst, const float (&v)[16]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * i + j]);
+    store32(dst + 8 * i, w);
+  }
 }
 __device__ __forceinline__ void load16_f32(const float* src, float (&v)[16]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 q = reinterpret_cast<const float4*>(src)[i];
-    v[4 * i] = q.x;
-    v[4 * i + 1] = q.y;
-    v[4 * i + 2] = q.z;
-    v[4 * i + 3] = q.w;
+  for (int i = 0; i < 2; ++i) {
+    float* w = v + 8 * i;
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7])
+                 : "l"(src + 8 * i)
+                 : "memory");
   }
 }
 // What becomes of 16 neighbouring columns of one row (acc1: the up columns of kDenseSwiGLU)
@@ -312,7 +322,10 @@ __device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, in
 #pragma unroll
       for (int q = 0; q < S; ++q)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) v[u][h][q] = ld_cluster_f32x4(part + (r * kSumsPitch<BN> + c + h * N_OUT) * 4, first + STEP * q);
+        for (int h = 0; h < kHalves; ++h) {
+          const uint32_t from = part + (r * kSumsPitch<BN> + c + h * N_OUT) * 4;
+          v[u][h][q] = q == share ? ld_shared_f32x4(from) : ld_cluster_f32x4(from, first + STEP * q);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
