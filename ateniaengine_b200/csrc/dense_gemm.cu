@@ -81,7 +81,7 @@ __device__ __forceinline__ void list_adapters(TileList& l, const int32_t* __rest
   if (r == 0) l.count = total;
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NP, bool AD, int BN>
+template <int EPI, int NP, bool AD, int BN>
 __global__ void __launch_bounds__(TileSize<BN>::kThreads)
 dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ TileArgs ta,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
@@ -111,30 +111,38 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const int rows = min(BM, p.M - m0), cols = min(N_OUT, p.N - n0);
   const int kb_begin = (int)((int64_t)p.kb * rank / split), kb_end = (int)((int64_t)p.kb * (rank + 1) / split);
   const int stages = ta.stages;
-  const int a_bytes = A_MN ? BM * BK * 2 : ta.a_rows * BK * 2;
+  const bool a_mn = p.a_mn, b_mn = p.b_mn;
+  const int a_bytes = ta.a_rows * BK * 2;
   const int stage_bytes = a_bytes + TileSize<BN>::kBBytes;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
-      mbar_init(smem_u32(&bars.full[s]), 1);
-      mbar_init(smem_u32(&bars.empty[s]), 1);
+  // Warp 0 initialises the barriers and goes on to its first loads; the other warps meet it (it only arrives) behind the
+  // allocation of tensor memory.
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < stages; ++s) {
+        mbar_init(smem_u32(&bars.full[s]), 1);
+        mbar_init(smem_u32(&bars.empty[s]), 1);
+      }
+      mbar_init(smem_u32(&bars.acc_full), 1);
+      mbar_init(smem_u32(&bars.listed), 4);
+      mbar_init(smem_u32(&bars.v_full), 1);
+      bars.abort_flag = 0;
+      fence_barrier_init();
     }
-    mbar_init(smem_u32(&bars.acc_full), 1);
-    mbar_init(smem_u32(&bars.listed), 4);
-    mbar_init(smem_u32(&bars.v_full), 1);
-    bars.abort_flag = 0;
-    fence_barrier_init();
+    __syncwarp();
+    asm volatile("barrier.cta.arrive 2, %0;" ::"n"(TileSize<BN>::kThreads) : "memory");
+  } else {
+    if (warp == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
+                   "r"(BN)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    asm volatile("barrier.cta.sync 2, %0;" ::"n"(TileSize<BN>::kThreads) : "memory");
+    tc_fence_after();
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
-                 "r"(BN)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars.tmem_base;
+  const uint32_t tmem = warp == 0 ? 0 : *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
 
   // Adapters: this rank takes every split-th of the list; an adapter is `steps` K = 16 steps (of both segments), and a stage holds
   // `slots` of them.
@@ -157,6 +165,12 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 
   if (warp == 0) {
     // ================= TMA producer =================
+    if (lane == 0) {
+      prefetch_map(&p.a[0]);
+      prefetch_map(&p.b[0]);
+      if constexpr (EPI == kDenseSwiGLU) prefetch_map(&p.b[1]);
+    }
+    __syncwarp();
     int stage = 0;
     uint32_t phase = 0, armed = 0;
     bool ok = true;
@@ -166,13 +180,13 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 #pragma unroll
       for (int j = 0; j < BN / 64; ++j) {
         if constexpr (EPI == kDenseSwiGLU) tma_load_2d_one(dst + 8192 * j, &p.b[j >= BN / 128], bar, k, n0 + 64 * (j % (BN / 128)));
-        else tma_load_2d_one(dst + 8192 * j, &p.b[seg], bar, B_MN ? n0 + 64 * j : k, B_MN ? k : n0 + 64 * j);
+        else tma_load_2d_one(dst + 8192 * j, &p.b[seg], bar, b_mn ? n0 + 64 * j : k, b_mn ? k : n0 + 64 * j);
       }
     };
     auto load_a = [&](int kb, uint32_t dst, uint32_t bar) {
       const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
       const int k = (kb - (seg ? p.kb0 : 0)) * BK;
-      if constexpr (A_MN) {
+      if (a_mn) {
         tma_load_2d_one(dst, &p.a[seg], bar, m0, k);
         tma_load_2d_one(dst + 8192, &p.a[seg], bar, m0 + 64, k);
       } else {
@@ -260,14 +274,15 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         phase ^= 1u;
       }
     };
-    constexpr uint32_t idesc = kIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(BN >> 3) << 17);
+    const uint32_t idesc = kIdesc | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(BN >> 3) << 17);
+    const uint64_t a_step = operand_step(a_mn), b_step = operand_step(b_mn);
     for (int kb = kb_begin; kb < kb_end; ++kb) {
       if (!filled()) break;
       const uint32_t sa = ring + stage * stage_bytes;
-      const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sa + a_bytes);
+      const uint64_t da = operand_desc(sa, a_mn), db = operand_desc(sa + a_bytes, b_mn);
 #pragma unroll
       for (int k = 0; k < BK / UMMA_K; ++k)
-        tc_mma_bf16_one(tmem, da + k * kOperandStep<A_MN>, db + k * kOperandStep<B_MN>, idesc, kb > kb_begin || k > 0);
+        tc_mma_bf16_one(tmem, da + k * a_step, db + k * b_step, idesc, kb > kb_begin || k > 0);
       used();
     }
     if constexpr (AD) {
@@ -345,7 +360,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
             f[j] = __uint_as_float(v[j]);
             f1[j] = EPI == kDenseSwiGLU ? __uint_as_float(v1[j]) : 0.f;
           }
-          if (row < rows) dense_emit16<EPI>(p, (int64_t)(m0 + row) * p.N + n0 + c, f, f1);
+          if (row < rows) dense_emit<EPI, 16>(p, m0 + row, n0 + c, f, f1);
         }
       } else {
 #pragma unroll 2
@@ -368,14 +383,13 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     __syncthreads();
     cluster_barrier();
     if (!*abort_flag) {
-      const int64_t at0 = (int64_t)m0 * p.N + n0;
       const uint32_t at = smem_u32(part);
       switch (split) {
-        case 2: add_parts<EPI, BN, 2, 1>(p, at0, rows, cols, at, rank, 0); break;
-        case 3: add_parts<EPI, BN, 3, 1>(p, at0, rows, cols, at, rank, 0); break;
-        case 4: add_parts<EPI, BN, 4, 1>(p, at0, rows, cols, at, rank, 0); break;
-        case 6: add_parts<EPI, BN, 6, 1>(p, at0, rows, cols, at, rank, 0); break;
-        default: add_parts<EPI, BN, 8, 1>(p, at0, rows, cols, at, rank, 0); break;
+        case 2: add_parts<EPI, BN, 2, 1>(p, m0, n0, rows, cols, at, rank, 0); break;
+        case 3: add_parts<EPI, BN, 3, 1>(p, m0, n0, rows, cols, at, rank, 0); break;
+        case 4: add_parts<EPI, BN, 4, 1>(p, m0, n0, rows, cols, at, rank, 0); break;
+        case 6: add_parts<EPI, BN, 6, 1>(p, m0, n0, rows, cols, at, rank, 0); break;
+        default: add_parts<EPI, BN, 8, 1>(p, m0, n0, rows, cols, at, rank, 0); break;
       }
     }
     __syncthreads();
@@ -390,14 +404,14 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NP, bool AD, int BN>
+template <int EPI, int NP, bool AD, int BN>
 int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
-  auto kernel = dense_tile_kernel<EPI, A_MN, B_MN, NP, AD, BN>;
+  auto kernel = dense_tile_kernel<EPI, NP, AD, BN>;
   static bool attr_set[kMaxDevices] = {};
   if (first_use_on_current_device(attr_set)) {
     ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemMax));
   }
-  const int rows = A_MN ? BM : g.a_rows;
+  const int rows = g.a_rows;
   const int stage_bytes = rows * BK * 2 + TileSize<BN>::kBBytes;
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
   if constexpr (AD) {
@@ -435,19 +449,13 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
 template <int BN>
 int launch_tiles_of(const DenseGemm& g, const TileArgs& ta, int tiles, cudaStream_t s) {
   const bool ad = g.adapters != nullptr;
-  if (g.epilogue == kDenseSwiGLU && !g.a_mn && !g.b_mn && g.problems == 1)
-    return ad ? launch_tiles<kDenseSwiGLU, false, false, 1, true, BN>(g, ta, tiles, s)
-              : launch_tiles<kDenseSwiGLU, false, false, 1, false, BN>(g, ta, tiles, s);
-  if (g.epilogue == kDensePlain && !g.a_mn && !g.b_mn && g.problems == 1)
-    return ad ? launch_tiles<kDensePlain, false, false, 1, true, BN>(g, ta, tiles, s)
-              : launch_tiles<kDensePlain, false, false, 1, false, BN>(g, ta, tiles, s);
-  if (ad) return ATENIA_ERR_UNSUPPORTED;
-  if (g.epilogue == kDenseGateGrad && !g.a_mn && g.b_mn && g.problems == 1)
-    return launch_tiles<kDenseGateGrad, false, true, 1, false, BN>(g, ta, tiles, s);
-  if (g.epilogue == kDensePlain && !g.a_mn && g.b_mn && g.problems == 1)
-    return launch_tiles<kDensePlain, false, true, 1, false, BN>(g, ta, tiles, s);
-  if (g.epilogue == kDensePlain && g.a_mn && g.b_mn && g.problems == 3)
-    return launch_tiles<kDensePlain, true, true, 3, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDensePlain && g.problems > 1 && !ad) return launch_tiles<kDensePlain, kMaxDenseProblems, false, BN>(g, ta, tiles, s);
+  if (g.problems != 1) return ATENIA_ERR_UNSUPPORTED;
+  if (g.epilogue == kDenseSwiGLU)
+    return ad ? launch_tiles<kDenseSwiGLU, 1, true, BN>(g, ta, tiles, s) : launch_tiles<kDenseSwiGLU, 1, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDensePlain)
+    return ad ? launch_tiles<kDensePlain, 1, true, BN>(g, ta, tiles, s) : launch_tiles<kDensePlain, 1, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDenseGateGrad && !ad) return launch_tiles<kDenseGateGrad, 1, false, BN>(g, ta, tiles, s);
   return ATENIA_ERR_UNSUPPORTED;
 }
 
@@ -482,7 +490,7 @@ int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   if (dense_gemv_serves(g)) return launch_dense_gemv(g, num_sms, s);
   DenseSize sizes[kMaxDenseProblems];
   for (int i = 0; i < g.problems; ++i) sizes[i] = {g.p[i].M, g.p[i].N, g.p[i].kb};
-  const DensePlan plan = dense_plan(sizes, g.problems, g.epilogue == kDenseSwiGLU, g.a_mn || g.a_rows == BM, num_sms);
+  const DensePlan plan = dense_plan(sizes, g.problems, g.epilogue == kDenseSwiGLU, g.a_rows == BM, num_sms);
   if (plan.pairs) return launch_dense_pairs(g, plan.split, num_sms, s);
   return launch_dense_tiles(g, plan.columns, plan.split, s);
 }

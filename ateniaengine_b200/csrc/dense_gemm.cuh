@@ -11,17 +11,21 @@
 
 namespace atenia {
 
+// What the forward pass keeps for the backward one (g and u, f32) is laid out in quads, [N / 4][M][4]: a lane of tensor memory holds a
+// row of D, so a warp that takes four features of 32 tokens reads or writes 512 bytes in a row, where the rows of a plain [M, N]
+// would be 32 lines an access.
 enum DenseEpilogue {
   kDensePlain = 0,     // out[m, n] = D
-  kDenseSwiGLU = 1,    // B = gate and up rows of the same features: out[m, f] = silu(g) u, optionally g and u in f32
+  kDenseSwiGLU = 1,    // B = gate and up rows of the same features: out[m, f] = silu(g) u, optionally g and u in quads
   kDenseGateGrad = 2,  // D = dh: dg, du and h from the saved g and u
 };
 
 struct DenseProblem {
   CUtensorMap a[2], b[2];  // kDenseSwiGLU: b[0] gate, b[1] up.  Else the k-blocks from kb0 on come through a[1] and b[1]
   int M, N, kb, kb0;       // N: columns of `out`; kb: k-blocks of 64 in all
+  bool a_mn, b_mn;         // MN-major operands
   __nv_bfloat16* out;      // [M, N]
-  float* gate;             // kDenseSwiGLU: g and u [M, N] to be saved, or null; kDenseGateGrad: the saved ones
+  float* gate;             // kDenseSwiGLU: g and u to be saved, or null; kDenseGateGrad: the saved ones
   float* up;
   const __nv_bfloat16* a_ptr;     // the same operands for the kernels that read them plainly (dense_gemv.cu)
   const __nv_bfloat16* b_ptr[2];
@@ -50,9 +54,8 @@ struct DenseGemm {
   DenseProblem p[kMaxDenseProblems];
   int problems;
   int epilogue;
-  bool a_mn, b_mn;               // MN-major operands
   const DenseAdapters* adapters;  // or null (host pointer, copied at the launch)
-  int a_rows;                    // K-major A: rows of its box (dense_a_rows)
+  int a_rows;                    // rows of A a stage holds: of a K-major A's box (dense_a_rows), else 128
   bool chained;                  // see launch_chained
   bool b_early;                  // B is not written by the kernel before: its first tiles are requested before the wait
   bool a_early;                  // neither is A: only the adapters' v is waited for
@@ -120,13 +123,14 @@ __device__ __forceinline__ uint64_t make_smem_desc_k16(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(6) << 61;
   return d;
 }
-template <bool MN>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
-  return MN ? make_smem_desc_mn(smem_addr) : make_smem_desc(smem_addr);
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr, bool mn) {
+  return mn ? make_smem_desc_mn(smem_addr) : make_smem_desc(smem_addr);
 }
 // K = 16 further inside the tile: 32 bytes of the swizzle row, or 16 rows of 128 bytes
-template <bool MN>
-constexpr uint64_t kOperandStep = MN ? (2048 >> 4) : (32 >> 4);
+__device__ __forceinline__ uint64_t operand_step(bool mn) { return mn ? 2048 >> 4 : 32 >> 4; }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
 
 __device__ __forceinline__ void tma_load_3d_one(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
@@ -214,118 +218,103 @@ __device__ __forceinline__ void gate_grad(float dh, float g, float u, float& dg,
   du = dh * (g * s);
   h = silu_mul(g, u);
 }
-// 32 bytes of one row: lanes hold rows, so each 32-byte access of a warp is a line of its own and two of 16 bytes cost twice as much
-__device__ __forceinline__ void store32(void* dst, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+// Four features of a token in the quads of the saved projections
+__device__ __forceinline__ float4* quad(float* base, const DenseProblem& p, int row, int col) {
+  return reinterpret_cast<float4*>(base) + (int64_t)(col >> 2) * p.M + row;
 }
-// 16 values of one row to consecutive bf16
-__device__ __forceinline__ void store16_bf16(__nv_bfloat16* dst, const float (&v)[16]) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-  store32(dst, w);
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
-__device__ __forceinline__ void store16_f32(float* dst, const float (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * i + j]);
-    store32(dst + 8 * i, w);
-  }
-}
-__device__ __forceinline__ void load16_f32(const float* src, float (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float* w = v + 8 * i;
-    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7])
-                 : "l"(src + 8 * i)
-                 : "memory");
-  }
-}
-// What becomes of 16 neighbouring columns of one row (acc1: the up columns of kDenseSwiGLU)
-template <int EPI>
-__device__ __forceinline__ void dense_emit16(const DenseProblem& p, int64_t at, const float (&acc)[16], const float (&acc1)[16]) {
-  float o[16];
+// The values that N neighbouring columns of one row become (acc1: the up columns of kDenseSwiGLU): o, and du and h of kDenseGateGrad.
+// `in`: the row exists, the saved projections may be read or written.
+template <int EPI, int N>
+__device__ __forceinline__ void dense_values(const DenseProblem& p, int row, int col, bool in, const float (&acc)[N], const float (&acc1)[N],
+                                             float (&o)[N], float (&du)[N], float (&h)[N]) {
   if constexpr (EPI == kDensePlain) {
-    store16_bf16(p.out + at, acc);
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = acc[j];
   } else if constexpr (EPI == kDenseSwiGLU) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = silu_mul(acc[j], acc1[j]);
-    store16_bf16(p.out + at, o);
-    if (p.gate) {
-      store16_f32(p.gate + at, acc);
-      store16_f32(p.up + at, acc1);
+    for (int j = 0; j < N; ++j) o[j] = silu_mul(acc[j], acc1[j]);
+    if (p.gate && in) {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        *quad(p.gate, p, row, col + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        *quad(p.up, p, row, col + j) = make_float4(acc1[j], acc1[j + 1], acc1[j + 2], acc1[j + 3]);
+      }
     }
   } else {
-    float g[16], u[16], du[16], h[16];
-    load16_f32(p.gate + at, g);
-    load16_f32(p.up + at, u);
+    float4 g[N / 4], u[N / 4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) gate_grad(acc[j], g[j], u[j], o[j], du[j], h[j]);
-    store16_bf16(p.out + at, o);
-    store16_bf16(p.out_du + at, du);
-    store16_bf16(p.out_h + at, h);
+    for (int j = 0; j < N / 4; ++j) {
+      g[j] = in ? *quad(p.gate, p, row, col + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      u[j] = in ? *quad(p.up, p, row, col + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      gate_grad(acc[4 * j], g[j].x, u[j].x, o[4 * j], du[4 * j], h[4 * j]);
+      gate_grad(acc[4 * j + 1], g[j].y, u[j].y, o[4 * j + 1], du[4 * j + 1], h[4 * j + 1]);
+      gate_grad(acc[4 * j + 2], g[j].z, u[j].z, o[4 * j + 2], du[4 * j + 2], h[4 * j + 2]);
+      gate_grad(acc[4 * j + 3], g[j].w, u[j].w, o[4 * j + 3], du[4 * j + 3], h[4 * j + 3]);
+    }
   }
 }
-// ... of four
-template <int EPI>
-__device__ __forceinline__ void dense_emit4(const DenseProblem& p, int64_t at, const float (&acc)[4], const float (&acc1)[4]) {
-  auto store = [&](__nv_bfloat16* dst, float a, float b, float c, float d) {
-    *reinterpret_cast<uint2*>(dst + at) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+// ... stored from the lane that holds the row; N = 16 or 4
+template <int EPI, int N>
+__device__ __forceinline__ void dense_emit(const DenseProblem& p, int row, int col, const float (&acc)[N], const float (&acc1)[N]) {
+  float o[N], du[N], h[N];
+  dense_values<EPI, N>(p, row, col, true, acc, acc1, o, du, h);
+  auto store = [&](__nv_bfloat16* base, const float (&v)[N]) {
+    __nv_bfloat16* dst = base + (int64_t)row * p.N + col;
+    if constexpr (N == 16) {
+      reinterpret_cast<uint4*>(dst)[0] = pack8(v);
+      reinterpret_cast<uint4*>(dst)[1] = pack8(v + 8);
+    } else {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
   };
-  if constexpr (EPI == kDensePlain) {
-    store(p.out, acc[0], acc[1], acc[2], acc[3]);
-  } else if constexpr (EPI == kDenseSwiGLU) {
-    store(p.out, silu_mul(acc[0], acc1[0]), silu_mul(acc[1], acc1[1]), silu_mul(acc[2], acc1[2]), silu_mul(acc[3], acc1[3]));
-    if (p.gate) {
-      *reinterpret_cast<float4*>(p.gate + at) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      *reinterpret_cast<float4*>(p.up + at) = make_float4(acc1[0], acc1[1], acc1[2], acc1[3]);
-    }
-  } else {
-    const float4 g = *reinterpret_cast<const float4*>(p.gate + at), u = *reinterpret_cast<const float4*>(p.up + at);
-    float dg[4], du[4], h[4];
-    gate_grad(acc[0], g.x, u.x, dg[0], du[0], h[0]);
-    gate_grad(acc[1], g.y, u.y, dg[1], du[1], h[1]);
-    gate_grad(acc[2], g.z, u.z, dg[2], du[2], h[2]);
-    gate_grad(acc[3], g.w, u.w, dg[3], du[3], h[3]);
-    store(p.out, dg[0], dg[1], dg[2], dg[3]);
-    store(p.out_du, du[0], du[1], du[2], du[3]);
-    store(p.out_h, h[0], h[1], h[2], h[3]);
+  store(p.out, o);
+  if constexpr (EPI == kDenseGateGrad) {
+    store(p.out_du, du);
+    store(p.out_h, h);
   }
 }
 // Sums of a tile in shared memory, [row][column]: floats of a row, so that eight lanes' 16-byte accesses fall into different banks
 template <int COLUMNS>
 constexpr int kSumsPitch = COLUMNS + 4;
-// Share `share` of S of a tile whose sums lie in the shared memory of S CTAs (ranks first, first + STEP, ...): four columns at a time,
-// columns fastest, added in rank order.  A thread has 16 loads on their way: one after another they cost more than the products of a
-// whole k-block each (1021 x 2048 over 5632, two pairs a tile: 23.5 -> XX us).
+// Share `share` of S of a tile whose sums lie in the shared memory of S CTAs (ranks first, first + STEP, ...): four columns of a row
+// at a time, added in rank order.  A warp covers one row, or eight rows of four quads where the saved projections are written too.
 template <int EPI, int BN, int S, int STEP>
-__device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, int rows, int cols, uint32_t part, int share, int first) {
+__device__ __forceinline__ void add_parts(const DenseProblem& p, int m0, int n0, int rows, int cols, uint32_t part, int share, int first) {
   constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
   constexpr int kHalves = EPI == kDenseSwiGLU ? 2 : 1;
-  constexpr int U = 16 / (S * kHalves) > 0 ? 16 / (S * kHalves) : 1;
-  const int quads = cols / 4, total = rows * quads;
+  constexpr int U = 16 / (S * kHalves) > 0 ? 16 / (S * kHalves) : 1;  // 16 loads of a thread on their way
+  const bool by_quads = EPI == kDenseGateGrad || (EPI == kDenseSwiGLU && p.gate != nullptr);
+  const int quads = cols / 4;
+  const int row_groups = (rows + 7) / 8;
+  const int total = by_quads ? row_groups * ((quads + 3) / 4) * 32 : rows * quads;
   const int begin = total * share / S, end = total * (share + 1) / S;
 #pragma unroll 1
   for (int i0 = begin + (int)threadIdx.x; i0 < end; i0 += U * (int)blockDim.x) {
     float4 v[U][kHalves][S];
-    int at[U];
+    int row[U], col[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = min(i0 + u * (int)blockDim.x, end - 1);
-      const int r = i / quads, c = 4 * (i - r * quads);
-      at[u] = r * p.N + c;
+      if (by_quads) {
+        const int w = i >> 5, l = i & 31, g = w / row_groups;
+        row[u] = (w - g * row_groups) * 8 + (l & 7);
+        col[u] = 4 * (4 * g + (l >> 3));
+      } else {
+        row[u] = i / quads;
+        col[u] = 4 * (i - row[u] * quads);
+      }
+      const uint32_t from = part + (min(row[u], rows - 1) * kSumsPitch<BN> + min(col[u], cols - 4)) * 4;
 #pragma unroll
       for (int q = 0; q < S; ++q)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const uint32_t from = part + (r * kSumsPitch<BN> + c + h * N_OUT) * 4;
-          v[u][h][q] = q == share ? ld_shared_f32x4(from) : ld_cluster_f32x4(from, first + STEP * q);
-        }
+        for (int h = 0; h < kHalves; ++h)
+          v[u][h][q] = q == share ? ld_shared_f32x4(from + h * N_OUT * 4) : ld_cluster_f32x4(from + h * N_OUT * 4, first + STEP * q);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -337,7 +326,7 @@ __device__ __forceinline__ void add_parts(const DenseProblem& p, int64_t at0, in
           acc[h][0] += v[u][h][q].x, acc[h][1] += v[u][h][q].y;
           acc[h][2] += v[u][h][q].z, acc[h][3] += v[u][h][q].w;
         }
-      if (i0 + u * (int)blockDim.x < end) dense_emit4<EPI>(p, at0 + at[u], acc[0], acc[1]);
+      if (i0 + u * (int)blockDim.x < end && row[u] < rows && col[u] < cols) dense_emit<EPI, 4>(p, m0 + row[u], n0 + col[u], acc[0], acc[1]);
     }
   }
 }

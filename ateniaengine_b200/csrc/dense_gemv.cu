@@ -161,8 +161,9 @@ dense_gemv_kernel(const __grid_constant__ VecArgs va, const __grid_constant__ st
       if constexpr (EPI == kDenseSwiGLU) {
         va.out[at] = __float2bfloat16(silu_mul(acc[0][t], acc[1][t]));
         if (va.gate) {
-          va.gate[at] = acc[0][t];
-          va.up[at] = acc[1][t];
+          const int64_t kept = (row / 4 * NT + t) * 4 + row % 4;  // (in quads: [N / 4][T][4])
+          va.gate[kept] = acc[0][t];
+          va.up[kept] = acc[1][t];
         }
       } else {
         *reinterpret_cast<uint32_t*>(va.out + at) = pack_bf16x2(acc[0][t], acc[1][t]);
@@ -245,7 +246,7 @@ int launch_vec_tokens(const DenseGemm& g, const VecArgs& va, int blocks, cudaStr
 
 bool dense_gemv_serves(const DenseGemm& g) {
   const DenseProblem& p = g.p[0];
-  return g.problems == 1 && !g.a_mn && !g.b_mn && g.epilogue != kDenseGateGrad && dense_gemv_rows(p.M, p.N, p.K);
+  return g.problems == 1 && !p.a_mn && !p.b_mn && (g.epilogue == kDensePlain || g.epilogue == kDenseSwiGLU) && dense_gemv_rows(p.M, p.N, p.K);
 }
 
 int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s) {

@@ -8,7 +8,8 @@
 //   order   : bands of kBand row tiles, column tile by column tile, so that the 74 tiles at work at one time share few operand rows in L2
 //   split   : where the tiles are too few, the pairs of a cluster (two, three or four) share a tile: consecutive k ranges, added through
 //             distributed shared memory in rank order
-//   epilogue: eight warps, a lane holds a row: 32 contiguous bytes of the result (and of each saved value 64) per lane and step
+//   epilogue: eight warps; a lane holds a row, so the results go through shared memory to TMA, which writes whole lines (32 bytes a
+//             lane were 32 lines an access, and a tile's 5400 cycles of them hid only behind a reduction of 700 and more)
 //
 // Adapters as in dense_gemm.cu: behind the k-blocks of a tile come those of the adapters that its rows have, with the lanes
 // of other rows disabled.
@@ -26,13 +27,23 @@ namespace {
 using namespace tc;
 
 constexpr int kPairM = 256, kPairN = 256;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 6;  // at most
 constexpr int kOperandBytes = BM * BK * 2;  // 16 KiB of A, and of B
 constexpr int kPairStageBytes = 2 * kOperandBytes;
 constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 constexpr int kPairTmemCols = 512;
-constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024;
+// Behind the ring each epilogue warp has a piece of shared memory for what it hands to TMA: 32 rows of 64 columns, or of 32 of each of
+// the three results of kDenseGateGrad (whose ring is a stage shorter for it).
+template <int EPI>
+struct PairSize {
+  static constexpr int kResults = EPI == kDenseGateGrad ? 3 : 1;
+  static constexpr int kCols = EPI == kDenseGateGrad ? 32 : 64;
+  static constexpr int kWarpBytes = kResults * kCols * 2 * 32;
+  static constexpr int kStages = EPI == kDenseGateGrad ? 5 : 6;
+  static constexpr int kSmem = kStages * kPairStageBytes + kEpiWarps * kWarpBytes + 1024;
+  static_assert(kSmem <= 226 * 1024 && BM * (kPairN + 4) * 4 <= kStages * kPairStageBytes, "");
+};
 constexpr int kBand = 8;
 
 struct __align__(8) PairBars {
@@ -52,6 +63,9 @@ struct NoAdapters {};
 template <int NP>
 struct Problems {
   DenseProblem p[NP];
+};
+struct PairResults {
+  CUtensorMap out[3];  // of the problems, or dg, du, h
 };
 
 constexpr uint32_t kPairIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairM >> 4) << 24);
@@ -82,8 +96,8 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, ui
       : "memory");
 }
 // The four MMAs of one k-block; `a_step`, `b_step`: descriptor distance of K = 16.
-template <uint64_t A_STEP, uint64_t B_STEP>
-__device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint64_t a_step, uint64_t b_step,
+                                           uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred e, p, t;\n\t"
       ".reg .b64 a, b;\n\t"
@@ -97,7 +111,7 @@ __device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uin
       "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
       "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
       "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "l"(a_step), "l"(b_step)
       : "memory");
 }
 __device__ __forceinline__ void mma_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, const uint32_t (&off)[8]) {
@@ -118,6 +132,21 @@ __device__ __forceinline__ void commit_both(uint32_t bar, uint32_t lead) {
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
       ::"r"(bar), "h"(mask)
       : "memory");
+}
+
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// 16 bytes of row `row` at 16-byte piece `c` of a box of rows of ROW_BYTES (64 or 128) under the swizzle of that width
+template <int ROW_BYTES>
+__device__ __forceinline__ void stage16(uint32_t box, int row, int c, const uint4& v) {
+  const uint32_t at = box + row * ROW_BYTES + ((c ^ (ROW_BYTES == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 struct Tile {
@@ -141,9 +170,9 @@ __device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& 
   return o;
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
+template <int EPI, int NP, bool AD>
 __global__ void __launch_bounds__(kPairThreads, 1)
-dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ PairArgs pa,
+dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ PairArgs pa, const __grid_constant__ PairResults res,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PairBars bars;
@@ -161,12 +190,15 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const int num_pairs = split > 1 ? pa.tiles : (int)(gridDim.x >> 1);
   const int piece = split > 1 ? (int)(in_cluster >> 1) : 0;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? kPairN / 2 : kPairN;
+  constexpr int kStages = PairSize<EPI>::kStages;
 
   auto kb_begin = [&](const DenseProblem& p) { return (int)((int64_t)p.kb * piece / split); };
   auto kb_end = [&](const DenseProblem& p) { return (int)((int64_t)p.kb * (piece + 1) / split); };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    prefetch_map(&ps.p[0].a[0]);
+    prefetch_map(&ps.p[0].b[EPI == kDenseSwiGLU ? rank : 0]);
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&bars.full[s]), 1);
       mbar_init(smem_u32(&bars.empty[s]), 1);
     }
@@ -202,16 +234,16 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         load_2d(dst + 8192, &p.b[rank], bar, k, t.n0 + 64);
       } else {
         const int n = t.n0 + (int)rank * 128;
-        load_2d(dst, &p.b[seg], bar, B_MN ? n : k, B_MN ? k : n);
-        load_2d(dst + 8192, &p.b[seg], bar, B_MN ? n + 64 : k, B_MN ? k : n + 64);
+        load_2d(dst, &p.b[seg], bar, p.b_mn ? n : k, p.b_mn ? k : n);
+        load_2d(dst + 8192, &p.b[seg], bar, p.b_mn ? n + 64 : k, p.b_mn ? k : n + 64);
       }
     };
     auto load_a = [&](const DenseProblem& p, const Tile& t, int kb, uint32_t dst, uint32_t bar) {
       const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
       const int k = (kb - (seg ? p.kb0 : 0)) * BK;
       const int m = t.m0 + (int)rank * BM;
-      load_2d(dst, &p.a[seg], bar, A_MN ? m : k, A_MN ? k : m);
-      if constexpr (A_MN) load_2d(dst + 8192, &p.a[seg], bar, m + 64, k);
+      load_2d(dst, &p.a[seg], bar, p.a_mn ? m : k, p.a_mn ? k : m);
+      if (p.a_mn) load_2d(dst + 8192, &p.a[seg], bar, m + 64, k);
     };
     auto free_stage = [&]() {
       if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
@@ -224,7 +256,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     };
     auto next_stage = [&]() {
       armed |= 1u << stage;
-      if (++stage == kPairStages) {
+      if (++stage == kStages) {
         stage = 0;
         phase ^= 1u;
       }
@@ -234,7 +266,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       const Tile t = tile_of<EPI, NP>(ps, pa, pair);
       const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
       const int kb0 = kb_begin(p);
-      ahead = min(kb_end(p) - kb0, kPairStages);
+      ahead = min(kb_end(p) - kb0, kStages);
       for (int i = 0; i < ahead; ++i) {
         const uint32_t bar = at_rank(smem_u32(&bars.full[i]), lead), dst = ring + i * kPairStageBytes;
         if (leader) mbar_expect_tx_one(smem_u32(&bars.full[i]), 2 * kPairStageBytes);
@@ -289,7 +321,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     chain_next();  // (every load is on its way: what follows may be launched)
     if (*abort_flag && leader && lane == 0) {
       // let the copies already issued (both CTAs') land before the pair's shared memory is released
-      for (int s = 0; s < kPairStages; ++s) {
+      for (int s = 0; s < kStages; ++s) {
         if (!(armed & (1u << s))) continue;
         const uint32_t par = s < stage ? phase : phase ^ 1u;
         for (int i = 0; i < (1 << 16) && !mbar_try_wait(smem_u32(&bars.full[s]), par); ++i) {}
@@ -314,12 +346,11 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       };
       auto used = [&]() {
         commit_both(smem_u32(&bars.empty[stage]), lead);
-        if (++stage == kPairStages) {
+        if (++stage == kStages) {
           stage = 0;
           phase ^= 1u;
         }
       };
-      constexpr uint32_t idesc = kPairIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kPairN >> 3) << 17);
       for (int i = pair; ok && i < pa.tiles; i += num_pairs, ++it) {
         const Tile t = tile_of<EPI, NP>(ps, pa, i);
         const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
@@ -335,12 +366,14 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * kPairN;
+        const bool a_mn = p.a_mn, b_mn = p.b_mn;
+        const uint32_t idesc = kPairIdesc | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(kPairN >> 3) << 17);
+        const uint64_t a_step = operand_step(a_mn), b_step = operand_step(b_mn);
         const int begin = kb_begin(p), end = kb_end(p);
         for (int kb = begin; kb < end; ++kb) {
           if (!filled()) break;
           const uint32_t sa = ring + stage * kPairStageBytes;
-          mma_kblock<kOperandStep<A_MN>, kOperandStep<B_MN>>(d, operand_desc<A_MN>(sa), operand_desc<B_MN>(sa + kOperandBytes), idesc,
-                                                             kb > begin ? 1u : 0u);
+          mma_kblock(d, operand_desc(sa, a_mn), operand_desc(sa + kOperandBytes, b_mn), a_step, b_step, idesc, kb > begin ? 1u : 0u);
           used();
         }
         if constexpr (AD) {
@@ -372,6 +405,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     chain_wait();
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int row_in = (int)rank * BM + quarter * 32 + lane;
+    const uint32_t box = ring + kStages * kPairStageBytes + (warp - 2) * PairSize<EPI>::kWarpBytes;
     int it = 0;
     for (int i = pair; i < pa.tiles; i += num_pairs, ++it) {
       const Tile t = tile_of<EPI, NP>(ps, pa, i);
@@ -388,7 +422,6 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       const int row = t.m0 + row_in;
       const int n = t.n0 + half * (N_OUT / 2);
       const int cols = min(N_OUT / 2, p.N - n);
-      const int64_t at = (int64_t)row * p.N + n;
       if (split > 1) {  // (one tile: the sums go to the ring, which nothing uses any more)
         float* mine = part + (quarter * 32 + lane) * kSumsPitch<kPairN> + half * 128;
         const uint32_t from = tmem + (uint32_t(quarter * 32) << 16) + half * 128;
@@ -403,24 +436,49 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         }
         break;
       }
+      constexpr int kCols = PairSize<EPI>::kCols, kResults = PairSize<EPI>::kResults;
+      const bool any = t.m0 + (int)rank * BM + quarter * 32 < p.M;
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 16) {
-        uint32_t v[16], v1[16];
-        tc_ld16(taddr + c, v);
-        if constexpr (EPI == kDenseSwiGLU) tc_ld16(taddr + N_OUT + c, v1);
-        tc_ld_wait();
-        float f[16], f1[16];
+      for (int c0 = 0; c0 < cols; c0 += kCols) {
+        if (lane == 0) store_wait_read();  // (the piece's last store)
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          f[j] = __uint_as_float(v[j]);
-          f1[j] = EPI == kDenseSwiGLU ? __uint_as_float(v1[j]) : 0.f;
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t v[16], v1[16];
+          tc_ld16(taddr + c0 + c, v);
+          if constexpr (EPI == kDenseSwiGLU) tc_ld16(taddr + N_OUT + c0 + c, v1);
+          tc_ld_wait();
+          float f[16], f1[16], o[16], du[16], h[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            f[j] = __uint_as_float(v[j]);
+            f1[j] = EPI == kDenseSwiGLU ? __uint_as_float(v1[j]) : 0.f;
+          }
+          dense_values<EPI, 16>(p, row, n + c0 + c, row < p.M && c0 + c < cols, f, f1, o, du, h);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            stage16<kCols * 2>(box, lane, c / 8 + q, pack8(o + 8 * q));
+            if constexpr (EPI == kDenseGateGrad) {
+              stage16<kCols * 2>(box + kCols * 64, lane, c / 8 + q, pack8(du + 8 * q));
+              stage16<kCols * 2>(box + 2 * kCols * 64, lane, c / 8 + q, pack8(h + 8 * q));
+            }
+          }
         }
-        if (row < p.M) dense_emit16<EPI>(p, at + c, f, f1);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && any) {
+#pragma unroll
+          for (int r = 0; r < kResults; ++r)
+            store_2d(&res.out[kResults > 1 ? r : t.which], box + r * kCols * 64, n + c0, row - lane);
+          store_commit();
+        }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_remote(at_rank(smem_u32(&bars.acc_empty[acc]), lead));
     }
+    if (lane == 0) store_wait();
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -432,10 +490,9 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
       const int m0 = t.m0 + (int)rank * BM;
       const int rows = max(0, min(BM, p.M - m0)), cols = min(N_OUT, p.N - t.n0);
-      const int64_t at0 = (int64_t)m0 * p.N + t.n0;
-      if (split == 2) add_parts<EPI, kPairN, 2, 2>(p, at0, rows, cols, smem_u32(part), piece, rank);
-      else if (split == 3) add_parts<EPI, kPairN, 3, 2>(p, at0, rows, cols, smem_u32(part), piece, rank);
-      else add_parts<EPI, kPairN, 4, 2>(p, at0, rows, cols, smem_u32(part), piece, rank);
+      if (split == 2) add_parts<EPI, kPairN, 2, 2>(p, m0, t.n0, rows, cols, smem_u32(part), piece, rank);
+      else if (split == 3) add_parts<EPI, kPairN, 3, 2>(p, m0, t.n0, rows, cols, smem_u32(part), piece, rank);
+      else add_parts<EPI, kPairN, 4, 2>(p, m0, t.n0, rows, cols, smem_u32(part), piece, rank);
     }
     __syncthreads();
   }
@@ -447,12 +504,12 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NP, bool AD>
+template <int EPI, int NP, bool AD>
 int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream_t s) {
-  auto kernel = dense_pair_kernel<EPI, A_MN, B_MN, NP, AD>;
+  auto kernel = dense_pair_kernel<EPI, NP, AD>;
   static bool attr_set[kMaxDevices] = {};
   if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairSize<EPI>::kSmem));
   }
   Problems<NP> ps;
   for (int i = 0; i < NP; ++i) ps.p[i] = g.p[i];
@@ -468,11 +525,21 @@ int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * pairs);
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = PairSize<EPI>::kSmem;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = g.chained ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ps, pa, ad);
+  PairResults res{};
+  auto map = [](CUtensorMap* m, const __nv_bfloat16* out, const DenseProblem& p) {
+    constexpr uint32_t cols = PairSize<EPI>::kCols;
+    return encode_tmap_bf16(m, out, {(uint64_t)p.N, (uint64_t)p.M, 0}, {cols, 32, 1}, 2 * cols);
+  };
+  int rc = ATENIA_OK;
+  for (int i = 0; i < NP && !rc; ++i) rc = map(&res.out[i], g.p[i].out, g.p[i]);
+  if (EPI == kDenseGateGrad && !rc) rc = map(&res.out[1], g.p[0].out_du, g.p[0]);
+  if (EPI == kDenseGateGrad && !rc) rc = map(&res.out[2], g.p[0].out_h, g.p[0]);
+  if (rc) return rc;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ps, pa, res, ad);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return (int)e;
 }
@@ -493,7 +560,7 @@ int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t 
     pa.tile_end[i] = (int)tiles;
   }
   if (tiles == 0) return ATENIA_OK;
-  if (!g.a_mn && g.a_rows != BM) return ATENIA_ERR_SHAPE;
+  if (g.a_rows != BM) return ATENIA_ERR_SHAPE;
   pa.problems = g.problems;
   pa.tiles = (int)tiles;
   pa.split = split;
@@ -502,19 +569,13 @@ int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t 
   count_launch();
   count_tcgen05_launch();
   const bool ad = g.adapters != nullptr;
-  if (g.epilogue == kDenseSwiGLU && !g.a_mn && !g.b_mn && g.problems == 1)
-    return ad ? launch_pairs<kDenseSwiGLU, false, false, 1, true>(g, pa, num_sms, s)
-              : launch_pairs<kDenseSwiGLU, false, false, 1, false>(g, pa, num_sms, s);
-  if (g.epilogue == kDensePlain && !g.a_mn && !g.b_mn && g.problems == 1)
-    return ad ? launch_pairs<kDensePlain, false, false, 1, true>(g, pa, num_sms, s)
-              : launch_pairs<kDensePlain, false, false, 1, false>(g, pa, num_sms, s);
-  if (ad) return ATENIA_ERR_UNSUPPORTED;
-  if (g.epilogue == kDenseGateGrad && !g.a_mn && g.b_mn && g.problems == 1)
-    return launch_pairs<kDenseGateGrad, false, true, 1, false>(g, pa, num_sms, s);
-  if (g.epilogue == kDensePlain && !g.a_mn && g.b_mn && g.problems == 1)
-    return launch_pairs<kDensePlain, false, true, 1, false>(g, pa, num_sms, s);
-  if (g.epilogue == kDensePlain && g.a_mn && g.b_mn && g.problems == 3)
-    return launch_pairs<kDensePlain, true, true, 3, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDensePlain && g.problems > 1 && !ad) return launch_pairs<kDensePlain, kMaxDenseProblems, false>(g, pa, num_sms, s);
+  if (g.problems != 1) return ATENIA_ERR_UNSUPPORTED;
+  if (g.epilogue == kDenseSwiGLU)
+    return ad ? launch_pairs<kDenseSwiGLU, 1, true>(g, pa, num_sms, s) : launch_pairs<kDenseSwiGLU, 1, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDensePlain)
+    return ad ? launch_pairs<kDensePlain, 1, true>(g, pa, num_sms, s) : launch_pairs<kDensePlain, 1, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDenseGateGrad && !ad) return launch_pairs<kDenseGateGrad, 1, false>(g, pa, num_sms, s);
   return ATENIA_ERR_UNSUPPORTED;
 }
 

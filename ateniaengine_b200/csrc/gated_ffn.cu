@@ -257,12 +257,12 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   DenseGemm g1{};  // dh = dy Wd: the reduction runs over the rows of Wd [d, F]
   g1.problems = 1;
   g1.epilogue = kDenseGateGrad;
-  g1.b_mn = true;
   g1.a_rows = dense_a_rows(T);
   g1.chained = true;
   DenseProblem& p1 = g1.p[0];
   p1.M = T;
   p1.N = d_ff;
+  p1.b_mn = true;
   p1.kb = p1.kb0 = kblocks(d);
   p1.out = dg;
   p1.out_du = du;
@@ -275,12 +275,12 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   DenseGemm g2{};  // dx = dg Wg + du Wu
   g2.problems = 1;
   g2.epilogue = kDensePlain;
-  g2.b_mn = true;
   g2.a_rows = g1.a_rows;
   g2.chained = g2.b_early = true;
   DenseProblem& p2 = g2.p[0];
   p2.M = T;
   p2.N = d_model;
+  p2.b_mn = true;
   p2.kb0 = kblocks(F);
   p2.kb = 2 * p2.kb0;
   p2.out = static_cast<__nv_bfloat16*>(dx);
@@ -292,7 +292,7 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   DenseGemm g3{};  // the weights' gradients: reductions over the tokens
   g3.problems = 3;
   g3.epilogue = kDensePlain;
-  g3.a_mn = g3.b_mn = true;
+  g3.a_rows = tc::BM;
   g3.chained = true;
   const void* lhs[3] = {dg, du, dy};
   const void* rhs[3] = {x, x, h};
@@ -301,6 +301,7 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
     DenseProblem& p = g3.p[i];
     p.M = i < 2 ? d_ff : d_model;
     p.N = i < 2 ? d_model : d_ff;
+    p.a_mn = p.b_mn = true;
     p.kb = p.kb0 = kblocks(T);
     p.out = static_cast<__nv_bfloat16*>(out[i]);
     if (!rc) rc = matrix_map(&p.a[0], lhs[i], T, p.M, 64);

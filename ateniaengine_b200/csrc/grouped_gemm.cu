@@ -520,7 +520,9 @@ int encode_tmap_bf16(CUtensorMap* out, const void* base, const uint64_t (&dims)[
   cuuint32_t boxes[3] = {box[0], box[1], box[2]};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), size, strides, boxes, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
+                                                 : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                       : CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
 }

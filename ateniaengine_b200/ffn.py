@@ -108,7 +108,7 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
 
     `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
     the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
-    [2, T, F], the two projections before the activation.  `sync=True` waits and raises what the kernels recorded."""
+    [2, F / 4, T, 4], the two projections before the activation.  `sync=True` waits and raises what the kernels recorded."""
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     keep, ad = [], None
@@ -132,7 +132,7 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
     y = _output(out, (T, d), x)
     saved, at_gate, at_up = None, None, None
     if save:
-        saved = x.new_empty((2, T, F), dtype=torch.float32)
+        saved = x.new_empty((2, F // 4, T, 4), dtype=torch.float32)
         at_gate = saved.data_ptr()
         at_up = at_gate + 4 * T * F
     nbytes = _ffn_bytes(T, d, F, 0, 0, 0, 0) if ad is None else _ffn_bytes(T, d, F, ad.gate.rank, ad.up.rank, ad.down.rank, 0)
@@ -152,7 +152,7 @@ def gated_ffn_backward(dy, x, gate, up, down, saved, sync=False):
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     dy = _operand(dy, "dy", (T, d), BF16, x.device)
-    saved = _operand(saved, "saved", (2, T, F), torch.float32, x.device)
+    saved = _operand(saved, "saved", (2, F // 4, T, 4), torch.float32, x.device)
     dx = torch.empty_like(x)
     dgate, dup, ddown = torch.empty_like(gate), torch.empty_like(up), torch.empty_like(down)
     nbytes = _ffn_bytes(T, d, F, 0, 0, 0, 1)

@@ -433,7 +433,8 @@ ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
  * ATENIA_ERR_CAPACITY); its content need not be kept between calls, and calls that may run at the same time, captured ones
  * included, need one each.  Asynchronous on `stream`; the calls allocate nothing and can be captured in a graph (make the first call
  * per device outside of a capture).
- * saved_gate, saved_up (device, f32 [T, d_ff], both or neither): g = x Wg^T and u = x Wu^T are stored for the backward pass.
+ * saved_gate, saved_up (device, f32 [d_ff / 4][T][4], both or neither): g = x Wg^T and u = x Wu^T are stored for the backward pass,
+ * four features of a token side by side.
  *
  * Adapters: token t adds scale[a] * B_a (A_a x_t) to a projection W x_t, where a = ids[t]; an id outside [0, n) means none.
  * A is [n, rank, in], B [n, out, rank] (device, bf16, 16-byte aligned), scale [n] and ids [T] device.  A rank is a multiple of 8

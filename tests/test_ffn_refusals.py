@@ -146,13 +146,13 @@ def test_python_entries_refuse_shapes_types_and_devices():
                  lambda: adapter_linear(x, g, LowRankAdapters(low.a[:, :4], low.b[:, :, :4], low.scale), ids),
                  lambda: adapter_linear(x, g, low._replace(scale=low.scale[:1]), ids),
                  lambda: adapter_linear(x, g, low._replace(b=low.b[:1]), ids),
-                 lambda: gated_ffn_backward(x[:3], x, g, u, d, z(2, 4, 96, dtype=torch.float32)),
-                 lambda: gated_ffn_backward(x, x, g, u, d, z(2, 3, 96, dtype=torch.float32))):
+                 lambda: gated_ffn_backward(x[:3], x, g, u, d, z(2, 24, 4, 4, dtype=torch.float32)),
+                 lambda: gated_ffn_backward(x, x, g, u, d, z(2, 24, 3, 4, dtype=torch.float32))):
         with pytest.raises(ValueError):
             call()
     for call in (lambda: gated_ffn(x, g.float(), u, d), lambda: gated_ffn(x, g, u, d, adapters={"gate": low}),
                  lambda: adapter_linear(x, g, low, ids.long()), lambda: adapter_linear(x, g, low._replace(scale=low.scale.double()), ids),
-                 lambda: gated_ffn_backward(x, x, g, u, d, z(2, 4, 96))):
+                 lambda: gated_ffn_backward(x, x, g, u, d, z(2, 24, 4, 4))):
         with pytest.raises(TypeError):
             call()
     from ateniaengine_b200._lib import AteniaError
