@@ -81,7 +81,7 @@ __device__ __forceinline__ void list_adapters(TileList& l, const int32_t* __rest
   if (r == 0) l.count = total;
 }
 
-template <int EPI, int NP, bool AD, int BN>
+template <int EPI, bool B_MN, int NP, bool AD, int BN>
 __global__ void __launch_bounds__(TileSize<BN>::kThreads)
 dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ TileArgs ta,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
@@ -111,38 +111,31 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const int rows = min(BM, p.M - m0), cols = min(N_OUT, p.N - n0);
   const int kb_begin = (int)((int64_t)p.kb * rank / split), kb_end = (int)((int64_t)p.kb * (rank + 1) / split);
   const int stages = ta.stages;
-  const bool a_mn = p.a_mn, b_mn = p.b_mn;
+  constexpr bool A_MN = NP > 1;
   const int a_bytes = ta.a_rows * BK * 2;
   const int stage_bytes = a_bytes + TileSize<BN>::kBBytes;
 
-  // Warp 0 initialises the barriers and goes on to its first loads; the other warps meet it (it only arrives) behind the
-  // allocation of tensor memory.
-  if (warp == 0) {
-    if (lane == 0) {
-      for (int s = 0; s < stages; ++s) {
-        mbar_init(smem_u32(&bars.full[s]), 1);
-        mbar_init(smem_u32(&bars.empty[s]), 1);
-      }
-      mbar_init(smem_u32(&bars.acc_full), 1);
-      mbar_init(smem_u32(&bars.listed), 4);
-      mbar_init(smem_u32(&bars.v_full), 1);
-      bars.abort_flag = 0;
-      fence_barrier_init();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(smem_u32(&bars.full[s]), 1);
+      mbar_init(smem_u32(&bars.empty[s]), 1);
     }
-    __syncwarp();
-    asm volatile("barrier.cta.arrive 2, %0;" ::"n"(TileSize<BN>::kThreads) : "memory");
-  } else {
-    if (warp == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
-                   "r"(BN)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    asm volatile("barrier.cta.sync 2, %0;" ::"n"(TileSize<BN>::kThreads) : "memory");
-    tc_fence_after();
+    mbar_init(smem_u32(&bars.acc_full), 1);
+    mbar_init(smem_u32(&bars.listed), 4);
+    mbar_init(smem_u32(&bars.v_full), 1);
+    bars.abort_flag = 0;
+    fence_barrier_init();
   }
-  const uint32_t tmem = warp == 0 ? 0 : *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
+                 "r"(BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem_base;
 
   // Adapters: this rank takes every split-th of the list; an adapter is `steps` K = 16 steps (of both segments), and a stage holds
   // `slots` of them.
@@ -165,12 +158,6 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 
   if (warp == 0) {
     // ================= TMA producer =================
-    if (lane == 0) {
-      prefetch_map(&p.a[0]);
-      prefetch_map(&p.b[0]);
-      if constexpr (EPI == kDenseSwiGLU) prefetch_map(&p.b[1]);
-    }
-    __syncwarp();
     int stage = 0;
     uint32_t phase = 0, armed = 0;
     bool ok = true;
@@ -180,13 +167,13 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 #pragma unroll
       for (int j = 0; j < BN / 64; ++j) {
         if constexpr (EPI == kDenseSwiGLU) tma_load_2d_one(dst + 8192 * j, &p.b[j >= BN / 128], bar, k, n0 + 64 * (j % (BN / 128)));
-        else tma_load_2d_one(dst + 8192 * j, &p.b[seg], bar, b_mn ? n0 + 64 * j : k, b_mn ? k : n0 + 64 * j);
+        else tma_load_2d_one(dst + 8192 * j, &p.b[seg], bar, B_MN ? n0 + 64 * j : k, B_MN ? k : n0 + 64 * j);
       }
     };
     auto load_a = [&](int kb, uint32_t dst, uint32_t bar) {
       const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
       const int k = (kb - (seg ? p.kb0 : 0)) * BK;
-      if (a_mn) {
+      if constexpr (A_MN) {
         tma_load_2d_one(dst, &p.a[seg], bar, m0, k);
         tma_load_2d_one(dst + 8192, &p.a[seg], bar, m0 + 64, k);
       } else {
@@ -274,15 +261,14 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         phase ^= 1u;
       }
     };
-    const uint32_t idesc = kIdesc | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(BN >> 3) << 17);
-    const uint64_t a_step = operand_step(a_mn), b_step = operand_step(b_mn);
+    constexpr uint32_t idesc = kIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(BN >> 3) << 17);
     for (int kb = kb_begin; kb < kb_end; ++kb) {
       if (!filled()) break;
       const uint32_t sa = ring + stage * stage_bytes;
-      const uint64_t da = operand_desc(sa, a_mn), db = operand_desc(sa + a_bytes, b_mn);
+      const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sa + a_bytes);
 #pragma unroll
       for (int k = 0; k < BK / UMMA_K; ++k)
-        tc_mma_bf16_one(tmem, da + k * a_step, db + k * b_step, idesc, kb > kb_begin || k > 0);
+        tc_mma_bf16_one(tmem, da + k * kOperandStep<A_MN>, db + k * kOperandStep<B_MN>, idesc, kb > kb_begin || k > 0);
       used();
     }
     if constexpr (AD) {
@@ -404,9 +390,9 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   }
 }
 
-template <int EPI, int NP, bool AD, int BN>
+template <int EPI, bool B_MN, int NP, bool AD, int BN>
 int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
-  auto kernel = dense_tile_kernel<EPI, NP, AD, BN>;
+  auto kernel = dense_tile_kernel<EPI, B_MN, NP, AD, BN>;
   static bool attr_set[kMaxDevices] = {};
   if (first_use_on_current_device(attr_set)) {
     ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemMax));
@@ -449,13 +435,17 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
 template <int BN>
 int launch_tiles_of(const DenseGemm& g, const TileArgs& ta, int tiles, cudaStream_t s) {
   const bool ad = g.adapters != nullptr;
-  if (g.epilogue == kDensePlain && g.problems > 1 && !ad) return launch_tiles<kDensePlain, kMaxDenseProblems, false, BN>(g, ta, tiles, s);
-  if (g.problems != 1) return ATENIA_ERR_UNSUPPORTED;
-  if (g.epilogue == kDenseSwiGLU)
-    return ad ? launch_tiles<kDenseSwiGLU, 1, true, BN>(g, ta, tiles, s) : launch_tiles<kDenseSwiGLU, 1, false, BN>(g, ta, tiles, s);
+  const bool b_mn = g.p[0].b_mn;
+  if (g.problems > 1)
+    return g.epilogue == kDensePlain && b_mn && !ad ? launch_tiles<kDensePlain, true, kMaxDenseProblems, false, BN>(g, ta, tiles, s) : ATENIA_ERR_UNSUPPORTED;
+  if (ad && b_mn) return ATENIA_ERR_UNSUPPORTED;
+  if (g.epilogue == kDenseSwiGLU && !b_mn)
+    return ad ? launch_tiles<kDenseSwiGLU, false, 1, true, BN>(g, ta, tiles, s) : launch_tiles<kDenseSwiGLU, false, 1, false, BN>(g, ta, tiles, s);
   if (g.epilogue == kDensePlain)
-    return ad ? launch_tiles<kDensePlain, 1, true, BN>(g, ta, tiles, s) : launch_tiles<kDensePlain, 1, false, BN>(g, ta, tiles, s);
-  if (g.epilogue == kDenseGateGrad && !ad) return launch_tiles<kDenseGateGrad, 1, false, BN>(g, ta, tiles, s);
+    return ad     ? launch_tiles<kDensePlain, false, 1, true, BN>(g, ta, tiles, s)
+           : b_mn ? launch_tiles<kDensePlain, true, 1, false, BN>(g, ta, tiles, s)
+                  : launch_tiles<kDensePlain, false, 1, false, BN>(g, ta, tiles, s);
+  if (g.epilogue == kDenseGateGrad && b_mn && !ad) return launch_tiles<kDenseGateGrad, true, 1, false, BN>(g, ta, tiles, s);
   return ATENIA_ERR_UNSUPPORTED;
 }
 

@@ -23,7 +23,7 @@ enum DenseEpilogue {
 struct DenseProblem {
   CUtensorMap a[2], b[2];  // kDenseSwiGLU: b[0] gate, b[1] up.  Else the k-blocks from kb0 on come through a[1] and b[1]
   int M, N, kb, kb0;       // N: columns of `out`; kb: k-blocks of 64 in all
-  bool a_mn, b_mn;         // MN-major operands
+  bool b_mn;               // MN-major operands: B, or (several problems in a launch) A and B
   __nv_bfloat16* out;      // [M, N]
   float* gate;             // kDenseSwiGLU: g and u to be saved, or null; kDenseGateGrad: the saved ones
   float* up;
@@ -123,14 +123,13 @@ __device__ __forceinline__ uint64_t make_smem_desc_k16(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(6) << 61;
   return d;
 }
-__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr, bool mn) {
-  return mn ? make_smem_desc_mn(smem_addr) : make_smem_desc(smem_addr);
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
+  return MN ? make_smem_desc_mn(smem_addr) : make_smem_desc(smem_addr);
 }
 // K = 16 further inside the tile: 32 bytes of the swizzle row, or 16 rows of 128 bytes
-__device__ __forceinline__ uint64_t operand_step(bool mn) { return mn ? 2048 >> 4 : 32 >> 4; }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-}
+template <bool MN>
+constexpr uint64_t kOperandStep = MN ? (2048 >> 4) : (32 >> 4);
 
 __device__ __forceinline__ void tma_load_3d_one(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
@@ -284,50 +283,45 @@ template <int COLUMNS>
 constexpr int kSumsPitch = COLUMNS + 4;
 // Share `share` of S of a tile whose sums lie in the shared memory of S CTAs (ranks first, first + STEP, ...): four columns of a row
 // at a time, added in rank order.  A warp covers one row, or eight rows of four quads where the saved projections are written too.
+// (All S loads of an element are on their way at once; more elements a thread cost the registers that the second CTA of an SM needs:
+// four of them 2048 x 2816, 128 tokens 23.2 -> 29.5 us.)
 template <int EPI, int BN, int S, int STEP>
 __device__ __forceinline__ void add_parts(const DenseProblem& p, int m0, int n0, int rows, int cols, uint32_t part, int share, int first) {
   constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
   constexpr int kHalves = EPI == kDenseSwiGLU ? 2 : 1;
-  constexpr int U = 16 / (S * kHalves) > 0 ? 16 / (S * kHalves) : 1;  // 16 loads of a thread on their way
   const bool by_quads = EPI == kDenseGateGrad || (EPI == kDenseSwiGLU && p.gate != nullptr);
   const int quads = cols / 4;
   const int row_groups = (rows + 7) / 8;
   const int total = by_quads ? row_groups * ((quads + 3) / 4) * 32 : rows * quads;
   const int begin = total * share / S, end = total * (share + 1) / S;
 #pragma unroll 1
-  for (int i0 = begin + (int)threadIdx.x; i0 < end; i0 += U * (int)blockDim.x) {
-    float4 v[U][kHalves][S];
-    int row[U], col[U];
+  for (int i = begin + (int)threadIdx.x; i < end; i += (int)blockDim.x) {
+    int row, col;
+    if (by_quads) {
+      const int w = i >> 5, l = i & 31, g = w / row_groups;
+      row = (w - g * row_groups) * 8 + (l & 7);
+      col = 4 * (4 * g + (l >> 3));
+      if (row >= rows || col >= cols) continue;
+    } else {
+      row = i / quads;
+      col = 4 * (i - row * quads);
+    }
+    const uint32_t from = part + (row * kSumsPitch<BN> + col) * 4;
+    float4 v[kHalves][S];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = min(i0 + u * (int)blockDim.x, end - 1);
-      if (by_quads) {
-        const int w = i >> 5, l = i & 31, g = w / row_groups;
-        row[u] = (w - g * row_groups) * 8 + (l & 7);
-        col[u] = 4 * (4 * g + (l >> 3));
-      } else {
-        row[u] = i / quads;
-        col[u] = 4 * (i - row[u] * quads);
+    for (int q = 0; q < S; ++q)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        v[h][q] = q == share ? ld_shared_f32x4(from + h * N_OUT * 4) : ld_cluster_f32x4(from + h * N_OUT * 4, first + STEP * q);
+    float acc[2][4] = {};
+#pragma unroll
+    for (int q = 0; q < S; ++q)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        acc[h][0] += v[h][q].x, acc[h][1] += v[h][q].y;
+        acc[h][2] += v[h][q].z, acc[h][3] += v[h][q].w;
       }
-      const uint32_t from = part + (min(row[u], rows - 1) * kSumsPitch<BN> + min(col[u], cols - 4)) * 4;
-#pragma unroll
-      for (int q = 0; q < S; ++q)
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-          v[u][h][q] = q == share ? ld_shared_f32x4(from + h * N_OUT * 4) : ld_cluster_f32x4(from + h * N_OUT * 4, first + STEP * q);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float acc[2][4] = {};
-#pragma unroll
-      for (int q = 0; q < S; ++q)
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          acc[h][0] += v[u][h][q].x, acc[h][1] += v[u][h][q].y;
-          acc[h][2] += v[u][h][q].z, acc[h][3] += v[u][h][q].w;
-        }
-      if (i0 + u * (int)blockDim.x < end && row[u] < rows && col[u] < cols) dense_emit<EPI, 4>(p, m0 + row[u], n0 + col[u], acc[0], acc[1]);
-    }
+    dense_emit<EPI, 4>(p, m0 + row, n0 + col, acc[0], acc[1]);
   }
 }
 }  // namespace tc

@@ -246,7 +246,7 @@ int launch_vec_tokens(const DenseGemm& g, const VecArgs& va, int blocks, cudaStr
 
 bool dense_gemv_serves(const DenseGemm& g) {
   const DenseProblem& p = g.p[0];
-  return g.problems == 1 && !p.a_mn && !p.b_mn && (g.epilogue == kDensePlain || g.epilogue == kDenseSwiGLU) && dense_gemv_rows(p.M, p.N, p.K);
+  return g.problems == 1 && !p.b_mn && (g.epilogue == kDensePlain || g.epilogue == kDenseSwiGLU) && dense_gemv_rows(p.M, p.N, p.K);
 }
 
 int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s) {

@@ -96,8 +96,8 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, ui
       : "memory");
 }
 // The four MMAs of one k-block; `a_step`, `b_step`: descriptor distance of K = 16.
-__device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint64_t a_step, uint64_t b_step,
-                                           uint32_t idesc, uint32_t accumulate) {
+template <uint64_t A_STEP, uint64_t B_STEP>
+__device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred e, p, t;\n\t"
       ".reg .b64 a, b;\n\t"
@@ -111,7 +111,7 @@ __device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uin
       "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
       "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
       "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "l"(a_step), "l"(b_step)
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
       : "memory");
 }
 __device__ __forceinline__ void mma_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, const uint32_t (&off)[8]) {
@@ -170,7 +170,7 @@ __device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& 
   return o;
 }
 
-template <int EPI, int NP, bool AD>
+template <int EPI, bool B_MN, int NP, bool AD>
 __global__ void __launch_bounds__(kPairThreads, 1)
 dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ PairArgs pa, const __grid_constant__ PairResults res,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
@@ -191,13 +191,12 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const int piece = split > 1 ? (int)(in_cluster >> 1) : 0;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? kPairN / 2 : kPairN;
   constexpr int kStages = PairSize<EPI>::kStages;
+  constexpr bool A_MN = NP > 1;
 
   auto kb_begin = [&](const DenseProblem& p) { return (int)((int64_t)p.kb * piece / split); };
   auto kb_end = [&](const DenseProblem& p) { return (int)((int64_t)p.kb * (piece + 1) / split); };
 
   if (threadIdx.x == 0) {
-    prefetch_map(&ps.p[0].a[0]);
-    prefetch_map(&ps.p[0].b[EPI == kDenseSwiGLU ? rank : 0]);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&bars.full[s]), 1);
       mbar_init(smem_u32(&bars.empty[s]), 1);
@@ -234,16 +233,16 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         load_2d(dst + 8192, &p.b[rank], bar, k, t.n0 + 64);
       } else {
         const int n = t.n0 + (int)rank * 128;
-        load_2d(dst, &p.b[seg], bar, p.b_mn ? n : k, p.b_mn ? k : n);
-        load_2d(dst + 8192, &p.b[seg], bar, p.b_mn ? n + 64 : k, p.b_mn ? k : n + 64);
+        load_2d(dst, &p.b[seg], bar, B_MN ? n : k, B_MN ? k : n);
+        load_2d(dst + 8192, &p.b[seg], bar, B_MN ? n + 64 : k, B_MN ? k : n + 64);
       }
     };
     auto load_a = [&](const DenseProblem& p, const Tile& t, int kb, uint32_t dst, uint32_t bar) {
       const int seg = EPI != kDenseSwiGLU && kb >= p.kb0;
       const int k = (kb - (seg ? p.kb0 : 0)) * BK;
       const int m = t.m0 + (int)rank * BM;
-      load_2d(dst, &p.a[seg], bar, p.a_mn ? m : k, p.a_mn ? k : m);
-      if (p.a_mn) load_2d(dst + 8192, &p.a[seg], bar, m + 64, k);
+      load_2d(dst, &p.a[seg], bar, A_MN ? m : k, A_MN ? k : m);
+      if constexpr (A_MN) load_2d(dst + 8192, &p.a[seg], bar, m + 64, k);
     };
     auto free_stage = [&]() {
       if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
@@ -351,6 +350,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           phase ^= 1u;
         }
       };
+      constexpr uint32_t idesc = kPairIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kPairN >> 3) << 17);
       for (int i = pair; ok && i < pa.tiles; i += num_pairs, ++it) {
         const Tile t = tile_of<EPI, NP>(ps, pa, i);
         const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
@@ -366,14 +366,12 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * kPairN;
-        const bool a_mn = p.a_mn, b_mn = p.b_mn;
-        const uint32_t idesc = kPairIdesc | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(kPairN >> 3) << 17);
-        const uint64_t a_step = operand_step(a_mn), b_step = operand_step(b_mn);
         const int begin = kb_begin(p), end = kb_end(p);
         for (int kb = begin; kb < end; ++kb) {
           if (!filled()) break;
           const uint32_t sa = ring + stage * kPairStageBytes;
-          mma_kblock(d, operand_desc(sa, a_mn), operand_desc(sa + kOperandBytes, b_mn), a_step, b_step, idesc, kb > begin ? 1u : 0u);
+          mma_kblock<kOperandStep<A_MN>, kOperandStep<B_MN>>(d, operand_desc<A_MN>(sa), operand_desc<B_MN>(sa + kOperandBytes), idesc,
+                                                             kb > begin ? 1u : 0u);
           used();
         }
         if constexpr (AD) {
@@ -504,9 +502,9 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   }
 }
 
-template <int EPI, int NP, bool AD>
+template <int EPI, bool B_MN, int NP, bool AD>
 int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream_t s) {
-  auto kernel = dense_pair_kernel<EPI, NP, AD>;
+  auto kernel = dense_pair_kernel<EPI, B_MN, NP, AD>;
   static bool attr_set[kMaxDevices] = {};
   if (first_use_on_current_device(attr_set)) {
     ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairSize<EPI>::kSmem));
@@ -569,13 +567,17 @@ int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t 
   count_launch();
   count_tcgen05_launch();
   const bool ad = g.adapters != nullptr;
-  if (g.epilogue == kDensePlain && g.problems > 1 && !ad) return launch_pairs<kDensePlain, kMaxDenseProblems, false>(g, pa, num_sms, s);
-  if (g.problems != 1) return ATENIA_ERR_UNSUPPORTED;
-  if (g.epilogue == kDenseSwiGLU)
-    return ad ? launch_pairs<kDenseSwiGLU, 1, true>(g, pa, num_sms, s) : launch_pairs<kDenseSwiGLU, 1, false>(g, pa, num_sms, s);
+  const bool b_mn = g.p[0].b_mn;
+  if (g.problems > 1)
+    return g.epilogue == kDensePlain && b_mn && !ad ? launch_pairs<kDensePlain, true, kMaxDenseProblems, false>(g, pa, num_sms, s) : ATENIA_ERR_UNSUPPORTED;
+  if (ad && b_mn) return ATENIA_ERR_UNSUPPORTED;
+  if (g.epilogue == kDenseSwiGLU && !b_mn)
+    return ad ? launch_pairs<kDenseSwiGLU, false, 1, true>(g, pa, num_sms, s) : launch_pairs<kDenseSwiGLU, false, 1, false>(g, pa, num_sms, s);
   if (g.epilogue == kDensePlain)
-    return ad ? launch_pairs<kDensePlain, 1, true>(g, pa, num_sms, s) : launch_pairs<kDensePlain, 1, false>(g, pa, num_sms, s);
-  if (g.epilogue == kDenseGateGrad && !ad) return launch_pairs<kDenseGateGrad, 1, false>(g, pa, num_sms, s);
+    return ad     ? launch_pairs<kDensePlain, false, 1, true>(g, pa, num_sms, s)
+           : b_mn ? launch_pairs<kDensePlain, true, 1, false>(g, pa, num_sms, s)
+                  : launch_pairs<kDensePlain, false, 1, false>(g, pa, num_sms, s);
+  if (g.epilogue == kDenseGateGrad && b_mn && !ad) return launch_pairs<kDenseGateGrad, true, 1, false>(g, pa, num_sms, s);
   return ATENIA_ERR_UNSUPPORTED;
 }
 

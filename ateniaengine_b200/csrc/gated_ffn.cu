@@ -301,7 +301,7 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
     DenseProblem& p = g3.p[i];
     p.M = i < 2 ? d_ff : d_model;
     p.N = i < 2 ? d_model : d_ff;
-    p.a_mn = p.b_mn = true;
+    p.b_mn = true;
     p.kb = p.kb0 = kblocks(T);
     p.out = static_cast<__nv_bfloat16*>(out[i]);
     if (!rc) rc = matrix_map(&p.a[0], lhs[i], T, p.M, 64);
