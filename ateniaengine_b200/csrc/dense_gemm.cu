@@ -324,18 +324,21 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     }
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
+    constexpr int kShares = BN / 128;  // warps of a quarter: each its share of the columns
+    constexpr int kCols = N_OUT / kShares;
+    const int share = (warp - 2) >> 2;
+    const int end = min(cols, (share + 1) * kCols);
+    Saved<EPI, 16> kept, next;
+    if (split == 1) kept.load(p, m0 + row, n0 + share * kCols, row < rows && share * kCols < end);
     if (!wait_all(&bars.acc_full, 0, 2300)) {
       // (reported)
     } else if (quarter * 32 < rows) {
       tc_fence_after();
       const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
-      constexpr int kShares = BN / 128;  // warps of a quarter: each its share of the columns
-      const int share = (warp - 2) >> 2;
       if (split == 1) {
-        constexpr int kCols = N_OUT / kShares;
-        const int end = min(cols, (share + 1) * kCols);
-#pragma unroll 1
+#pragma unroll 2
         for (int c = share * kCols; c < end; c += 16) {
+          next.load(p, m0 + row, n0 + c + 16, row < rows && c + 16 < end);
           uint32_t v[16], v1[16];
           tc_ld16(taddr + c, v);
           if constexpr (EPI == kDenseSwiGLU) tc_ld16(taddr + N_OUT + c, v1);
@@ -346,7 +349,8 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
             f[j] = __uint_as_float(v[j]);
             f1[j] = EPI == kDenseSwiGLU ? __uint_as_float(v1[j]) : 0.f;
           }
-          if (row < rows) dense_emit<EPI, 16>(p, m0 + row, n0 + c, f, f1);
+          if (row < rows) dense_emit<EPI, 16>(p, m0 + row, n0 + c, f, f1, kept);
+          kept = next;
         }
       } else {
 #pragma unroll 2

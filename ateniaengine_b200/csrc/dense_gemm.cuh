@@ -224,11 +224,25 @@ __device__ __forceinline__ float4* quad(float* base, const DenseProblem& p, int 
 __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
+// The saved projections of N columns of a row (kDenseGateGrad): asked for before the sums are there, or the epilogue waits for each.
+template <int EPI, int N>
+struct Saved {
+  float4 g[EPI == kDenseGateGrad ? N / 4 : 1], u[EPI == kDenseGateGrad ? N / 4 : 1];
+  __device__ __forceinline__ void load(const DenseProblem& p, int row, int col, bool in) {
+    if constexpr (EPI == kDenseGateGrad) {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) {
+        g[j] = in ? *quad(p.gate, p, row, col + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        u[j] = in ? *quad(p.up, p, row, col + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+};
 // The values that N neighbouring columns of one row become (acc1: the up columns of kDenseSwiGLU): o, and du and h of kDenseGateGrad.
-// `in`: the row exists, the saved projections may be read or written.
+// `in`: the row exists, the saved projections may be written.
 template <int EPI, int N>
 __device__ __forceinline__ void dense_values(const DenseProblem& p, int row, int col, bool in, const float (&acc)[N], const float (&acc1)[N],
-                                             float (&o)[N], float (&du)[N], float (&h)[N]) {
+                                             const Saved<EPI, N>& kept, float (&o)[N], float (&du)[N], float (&h)[N]) {
   if constexpr (EPI == kDensePlain) {
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = acc[j];
@@ -243,26 +257,21 @@ __device__ __forceinline__ void dense_values(const DenseProblem& p, int row, int
       }
     }
   } else {
-    float4 g[N / 4], u[N / 4];
 #pragma unroll
     for (int j = 0; j < N / 4; ++j) {
-      g[j] = in ? *quad(p.gate, p, row, col + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-      u[j] = in ? *quad(p.up, p, row, col + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j) {
-      gate_grad(acc[4 * j], g[j].x, u[j].x, o[4 * j], du[4 * j], h[4 * j]);
-      gate_grad(acc[4 * j + 1], g[j].y, u[j].y, o[4 * j + 1], du[4 * j + 1], h[4 * j + 1]);
-      gate_grad(acc[4 * j + 2], g[j].z, u[j].z, o[4 * j + 2], du[4 * j + 2], h[4 * j + 2]);
-      gate_grad(acc[4 * j + 3], g[j].w, u[j].w, o[4 * j + 3], du[4 * j + 3], h[4 * j + 3]);
+      gate_grad(acc[4 * j], kept.g[j].x, kept.u[j].x, o[4 * j], du[4 * j], h[4 * j]);
+      gate_grad(acc[4 * j + 1], kept.g[j].y, kept.u[j].y, o[4 * j + 1], du[4 * j + 1], h[4 * j + 1]);
+      gate_grad(acc[4 * j + 2], kept.g[j].z, kept.u[j].z, o[4 * j + 2], du[4 * j + 2], h[4 * j + 2]);
+      gate_grad(acc[4 * j + 3], kept.g[j].w, kept.u[j].w, o[4 * j + 3], du[4 * j + 3], h[4 * j + 3]);
     }
   }
 }
 // ... stored from the lane that holds the row; N = 16 or 4
 template <int EPI, int N>
-__device__ __forceinline__ void dense_emit(const DenseProblem& p, int row, int col, const float (&acc)[N], const float (&acc1)[N]) {
+__device__ __forceinline__ void dense_emit(const DenseProblem& p, int row, int col, const float (&acc)[N], const float (&acc1)[N],
+                                           const Saved<EPI, N>& kept) {
   float o[N], du[N], h[N];
-  dense_values<EPI, N>(p, row, col, true, acc, acc1, o, du, h);
+  dense_values<EPI, N>(p, row, col, true, acc, acc1, kept, o, du, h);
   auto store = [&](__nv_bfloat16* base, const float (&v)[N]) {
     __nv_bfloat16* dst = base + (int64_t)row * p.N + col;
     if constexpr (N == 16) {
@@ -307,6 +316,8 @@ __device__ __forceinline__ void add_parts(const DenseProblem& p, int m0, int n0,
       col = 4 * (i - row * quads);
     }
     const uint32_t from = part + (row * kSumsPitch<BN> + col) * 4;
+    Saved<EPI, 4> kept;
+    kept.load(p, m0 + row, n0 + col, true);
     float4 v[kHalves][S];
 #pragma unroll
     for (int q = 0; q < S; ++q)
@@ -321,7 +332,7 @@ __device__ __forceinline__ void add_parts(const DenseProblem& p, int m0, int n0,
         acc[h][0] += v[h][q].x, acc[h][1] += v[h][q].y;
         acc[h][2] += v[h][q].z, acc[h][3] += v[h][q].w;
       }
-    dense_emit<EPI, 4>(p, m0 + row, n0 + col, acc[0], acc[1]);
+    dense_emit<EPI, 4>(p, m0 + row, n0 + col, acc[0], acc[1], kept);
   }
 }
 }  // namespace tc

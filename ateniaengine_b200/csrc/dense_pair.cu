@@ -409,6 +409,11 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       const Tile t = tile_of<EPI, NP>(ps, pa, i);
       const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
       const int acc = it & 1;
+      const int row = t.m0 + row_in;
+      const int n = t.n0 + half * (N_OUT / 2);
+      const int cols = min(N_OUT / 2, p.N - n);
+      Saved<EPI, 16> kept, next;
+      if (split == 1) kept.load(p, row, n, row < p.M && cols > 0);
       const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full[acc]), (it >> 1) & 1, abort_flag));
       if (!ready) {
         if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 3000 + acc);
@@ -417,9 +422,6 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + acc * kPairN + half * (N_OUT / 2);
-      const int row = t.m0 + row_in;
-      const int n = t.n0 + half * (N_OUT / 2);
-      const int cols = min(N_OUT / 2, p.N - n);
       if (split > 1) {  // (one tile: the sums go to the ring, which nothing uses any more)
         float* mine = part + (quarter * 32 + lane) * kSumsPitch<kPairN> + half * 128;
         const uint32_t from = tmem + (uint32_t(quarter * 32) << 16) + half * 128;
@@ -442,6 +444,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
+          next.load(p, row, n + c0 + c + 16, row < p.M && c0 + c + 16 < cols);
           uint32_t v[16], v1[16];
           tc_ld16(taddr + c0 + c, v);
           if constexpr (EPI == kDenseSwiGLU) tc_ld16(taddr + N_OUT + c0 + c, v1);
@@ -452,7 +455,8 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
             f[j] = __uint_as_float(v[j]);
             f1[j] = EPI == kDenseSwiGLU ? __uint_as_float(v1[j]) : 0.f;
           }
-          dense_values<EPI, 16>(p, row, n + c0 + c, row < p.M && c0 + c < cols, f, f1, o, du, h);
+          dense_values<EPI, 16>(p, row, n + c0 + c, row < p.M && c0 + c < cols, f, f1, kept, o, du, h);
+          kept = next;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             stage16<kCols * 2>(box, lane, c / 8 + q, pack8(o + 8 * q));
