@@ -186,14 +186,14 @@ def lib():
         l.atenia_moe_plan_exec_pieces_measured.argtypes = [C.POINTER(MoeConfig), C.c_uint64, C.c_double, C.c_double,
                                                             C.c_double, C.POINTER(C.c_uint64), C.c_int]
         vp = C.c_void_p
-        l.atenia_gated_ffn_workspace_bytes.argtypes = [C.c_int] * 3 + [C.POINTER(FfnAdapters), C.c_int]
+        l.atenia_gated_ffn_workspace_bytes.argtypes = [C.c_int] * 3 + [vp, C.c_int]
         l.atenia_gated_ffn_workspace_bytes.restype = C.c_uint64
-        l.atenia_gated_ffn_forward.argtypes = ([vp] * 4 + [C.c_int] * 3 + [C.POINTER(FfnAdapters)] + [vp] * 4
+        l.atenia_gated_ffn_forward.argtypes = ([vp] * 4 + [C.c_int] * 3 + [vp] + [vp] * 4
                                                + [C.c_uint64, vp])
         l.atenia_gated_ffn_backward.argtypes = [vp] * 7 + [C.c_int] * 3 + [vp] * 5 + [C.c_uint64, vp]
         l.atenia_adapter_linear_workspace_bytes.argtypes = [C.c_int, C.c_int]
         l.atenia_adapter_linear_workspace_bytes.restype = C.c_uint64
-        l.atenia_adapter_linear.argtypes = ([vp, vp] + [C.c_int] * 3 + [C.POINTER(LowRank), vp, C.c_int, vp, vp, C.c_uint64,
+        l.atenia_adapter_linear.argtypes = ([vp, vp] + [C.c_int] * 3 + [vp, vp, C.c_int, vp, vp, C.c_uint64,
                                                                          vp])
         l.atenia_ffn_check.argtypes = [vp]
         _lib = l

@@ -7,6 +7,7 @@ step calls `gated_ffn_backward` itself.
 """
 import ctypes as C
 import functools
+import struct
 from typing import NamedTuple
 
 import torch
@@ -15,6 +16,7 @@ from . import _lib
 from .moe import _launching
 
 BF16 = torch.bfloat16
+_PARTS = {"gate", "up", "down"}
 
 
 class LowRankAdapters(NamedTuple):
@@ -61,26 +63,32 @@ def _output(out, shape, x):
     return out
 
 
-def _low_rank(set_, name, n_in, n_out, device, keep):
-    """The C description of one projection's adapters; what it points to goes into `keep`."""
+# AteniaLowRank and AteniaFfnAdapters as their bytes: a fifth of the time that filling in ctypes structures takes
+_LOW_RANK = struct.Struct("@PPPii")
+_FFN_ADAPTERS = struct.Struct("@" + 3 * "PPPii" + "Pii")
+_NONE = (0, 0, 0, 0, 0)
+assert _LOW_RANK.size == C.sizeof(_lib.LowRank) and _FFN_ADAPTERS.size == C.sizeof(_lib.FfnAdapters)
+
+
+def _low_rank(set_, name, n_in, n_out, device):
+    """The fields of AteniaLowRank of one projection's adapters, how many there are, and the tensors they point to."""
     a, b, scale = set_
     if not isinstance(a, torch.Tensor) or a.dim() != 3:
         raise ValueError(f"{name}.a must be [n, rank, {n_in}]")
-    n, rank = a.shape[0], a.shape[1]
+    n, rank, _ = a.shape
     if n < 1 or rank < 8 or rank > 128 or rank % 8:
         raise ValueError(f"{name}: at least one adapter, of a rank that is a multiple of 8 up to 128, got {tuple(a.shape)}")
     a = _operand(a, name + ".a", (n, rank, n_in), BF16, device)
     b = _operand(b, name + ".b", (n, n_out, rank), BF16, device)
     scale = _operand(scale, name + ".scale", (n,), torch.float32, device)
-    keep += [a, b, scale]
-    return _lib.LowRank(a.data_ptr(), b.data_ptr(), scale.data_ptr(), rank, 0), n
+    return (a.data_ptr(), b.data_ptr(), scale.data_ptr(), rank, 0), n, (a, b, scale)
 
 
 # Bytes of a call's workspace: functions of the sizes alone.
 @functools.lru_cache(maxsize=256)
 def _ffn_bytes(T, d, F, r_gate, r_up, r_down, backward):
-    ranks = _lib.FfnAdapters(gate=_lib.LowRank(rank=r_gate), up=_lib.LowRank(rank=r_up), down=_lib.LowRank(rank=r_down))
-    return _lib.lib().atenia_gated_ffn_workspace_bytes(T, d, F, C.byref(ranks), backward)
+    ranks = _FFN_ADAPTERS.pack(0, 0, 0, r_gate, 0, 0, 0, 0, r_up, 0, 0, 0, 0, r_down, 0, 0, 0, 0)
+    return _lib.lib().atenia_gated_ffn_workspace_bytes(T, d, F, ranks, backward)
 
 
 @functools.lru_cache(maxsize=256)
@@ -103,6 +111,30 @@ def _block(x, gate, up, down):
             _operand(down, "down", (d, F), BF16, x.device))
 
 
+def _block_adapters(adapters, adapter_ids, T, d, F, save, device):
+    """AteniaFfnAdapters, the three ranks, and the tensors it points to."""
+    if save:
+        raise ValueError("the backward pass is that of the block without adapters: save=True takes none")
+    if not adapters.keys() <= _PARTS:
+        raise ValueError(f"adapters of {sorted(set(adapters) - _PARTS)}: the block has gate, up and down")
+    ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, device)
+    fields, n, ranks, keep = (), 0, [], [ids]
+    for name in ("gate", "up", "down"):
+        set_ = adapters.get(name)
+        if set_ is None:
+            fields += _NONE
+            ranks.append(0)
+            continue
+        low, here, tensors = _low_rank(set_, name, F if name == "down" else d, d if name == "down" else F, device)
+        if n not in (0, here):
+            raise ValueError("the projections have different numbers of adapters")
+        n = here
+        fields += low
+        ranks.append(low[3])
+        keep.append(tensors)
+    return _FFN_ADAPTERS.pack(*fields, ids.data_ptr(), n, 0), ranks, keep
+
+
 def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, out=None, sync=False):
     """y = (silu(x gate^T) * (x up^T)) down^T.  x: CUDA bf16 [T, d], any T; gate, up: bf16 [F, d]; down: bf16 [d, F].
 
@@ -111,22 +143,9 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
     [2, F / 4, T, 4], the two projections before the activation.  `sync=True` waits and raises what the kernels recorded."""
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
-    keep, ad = [], None
+    ad, ranks = None, (0, 0, 0)
     if adapters:
-        if save:
-            raise ValueError("the backward pass is that of the block without adapters: save=True takes none")
-        if set(adapters) - {"gate", "up", "down"}:
-            raise ValueError(f"adapters of {sorted(set(adapters) - {'gate', 'up', 'down'})}: the block has gate, up and down")
-        ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, x.device)
-        ad = _lib.FfnAdapters(ids=ids.data_ptr())
-        for name, set_ in adapters.items():
-            n_in, n_out = (F, d) if name == "down" else (d, F)
-            low, n = _low_rank(set_, name, n_in, n_out, x.device, keep)
-            if ad.n not in (0, n):
-                raise ValueError("the projections have different numbers of adapters")
-            ad.n = n
-            setattr(ad, name, low)
-        keep.append(ids)
+        ad, ranks, keep = _block_adapters(adapters, adapter_ids, T, d, F, save, x.device)
     elif adapter_ids is not None:
         raise ValueError("adapter_ids without adapters")
     y = _output(out, (T, d), x)
@@ -135,12 +154,12 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
         saved = x.new_empty((2, F // 4, T, 4), dtype=torch.float32)
         at_gate = saved.data_ptr()
         at_up = at_gate + 4 * T * F
-    nbytes = _ffn_bytes(T, d, F, 0, 0, 0, 0) if ad is None else _ffn_bytes(T, d, F, ad.gate.rank, ad.up.rank, ad.down.rank, 0)
+    nbytes = _ffn_bytes(T, d, F, *ranks, 0)
     ws = _workspace(nbytes, x)
     lib = _lib.lib()
     with _launching(x.device) as st:
         rc = lib.atenia_gated_ffn_forward(x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), T, d, F,
-                                          None if ad is None else C.byref(ad), y.data_ptr(), at_gate, at_up, ws.data_ptr(), nbytes, st)
+                                          ad, y.data_ptr(), at_gate, at_up, ws.data_ptr(), nbytes, st)
         if rc or sync:
             _lib.check(rc or lib.atenia_ffn_check(st), "gated_ffn")
     return (y, saved) if save else y
@@ -181,14 +200,13 @@ def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
         raise ValueError(f"the projection's sizes must be multiples of 16, got {n_out} x {n_in}")
     weight = _operand(weight, "weight", (n_out, n_in), BF16, x.device)
     ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, x.device)
-    keep = []
-    low, n = _low_rank(adapters, "adapters", n_in, n_out, x.device, keep)
+    low, n, keep = _low_rank(adapters, "adapters", n_in, n_out, x.device)
     y = _output(out, (T, n_out), x)
-    nbytes = _linear_bytes(T, low.rank)
+    nbytes = _linear_bytes(T, low[3])
     ws = _workspace(nbytes, x)
     lib = _lib.lib()
     with _launching(x.device) as st:
-        rc = lib.atenia_adapter_linear(x.data_ptr(), weight.data_ptr(), T, n_in, n_out, C.byref(low), ids.data_ptr(), n, y.data_ptr(),
+        rc = lib.atenia_adapter_linear(x.data_ptr(), weight.data_ptr(), T, n_in, n_out, _LOW_RANK.pack(*low), ids.data_ptr(), n, y.data_ptr(),
                                        ws.data_ptr(), nbytes, st)
         if rc or sync:
             _lib.check(rc or lib.atenia_ffn_check(st), "adapter_linear")
