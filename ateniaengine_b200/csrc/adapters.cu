@@ -1,8 +1,8 @@
 // First half of the low-rank adapters: v[t, :] = scale[a] * (A_a x[t, :]) with a = ids[t], rounded to bf16 (the second product's
 // operand; the sums, over CTAs too, are f32).
 //
-// A tile is 128 token rows; its distinct adapters, in ascending order of their ids, are taken up to 128 rank rows at a time as the
-// N side of one MMA, and a row keeps the columns of its own adapter.  Rows of other adapters are computed and dropped: a
+// A tile is 128 token rows; its distinct adapters, in the order of their first rows, are taken up to 128 rank rows at a time (of gate
+// and up together where they fit) as the N side of one MMA, and a row keeps the columns of its own adapter.  Rows of other adapters are computed and dropped: a
 // decode batch in which every row has its own adapter reads each A once, which is what bounds it, and a tensor core has the
 // products to spare (64 rows, rank 16: 1 GFLOP instead of 8 MFLOP per 4096 inputs).  A cluster of up to 8 CTAs cuts the reduction
 // and adds in rank order.
@@ -13,7 +13,6 @@ namespace {
 using namespace tc;
 
 constexpr int kRankRows = 128;      // rank rows of a tile at most
-constexpr int kMaxList = kRankRows / 8;
 constexpr int kRedStages = 6;       // at most
 constexpr int kRedThreads = 192;
 constexpr int kRedTmemCols = 128;
@@ -30,34 +29,40 @@ struct __align__(8) RedBars {
   int abort_flag;
 };
 
+// What a CTA works on: the rank rows of one projection, or those of both side by side
+struct RedPart {
+  int first, count, rank0, cols;  // projections first .. first + count - 1; rank rows of the first and of all
+};
+
 // This rank's share of the tile's sums, four rank rows a thread, added in rank order.
 template <int S>
-__device__ __forceinline__ void add_rows(const AdapterReduce& ar, int proj, int m0, int rows, uint32_t part, const int32_t* row_id,
-                                         int rank) {
-  const int r = ar.p[proj].rank, quads = r / 4, total = rows * quads;
+__device__ __forceinline__ void add_rows(const AdapterReduce& ar, const RedPart& rp, int m0, int rows, uint32_t part, const TileList& list,
+                                         const int16_t* slot, int begin_slot, int end_slot, int rank) {
+  const int quads = rp.cols / 4, total = rows * quads;
   const int begin = total * rank / S, end = total * (rank + 1) / S;
   for (int i = begin + (int)threadIdx.x; i < end; i += kRedThreads) {
     const int t = i / quads, j = 4 * (i - t * quads);
-    const int32_t a = row_id[t];
-    if (a == kNoAdapter) continue;
-    const float scale = ar.p[proj].scale[a];
+    if (slot[t] < begin_slot || slot[t] >= end_slot) continue;
+    const AdapterReduce::Projection& p = ar.p[rp.first + (j >= rp.rank0)];
+    const int at = j >= rp.rank0 ? j - rp.rank0 : j;
+    const float scale = p.scale[list.id[t]];
     float4 v[S];
 #pragma unroll
     for (int q = 0; q < S; ++q) v[q] = ld_cluster_f32x4(part + (t * kRedPitch + j) * 4, q);
     float4 sum = v[0];
 #pragma unroll
     for (int q = 1; q < S; ++q) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
-    *reinterpret_cast<uint2*>(ar.p[proj].v + (int64_t)(m0 + t) * r + j) =
+    *reinterpret_cast<uint2*>(p.v + (int64_t)(m0 + t) * p.rank + at) =
         make_uint2(pack_bf16x2(sum.x * scale, sum.y * scale), pack_bf16x2(sum.z * scale, sum.w * scale));
   }
 }
 
 __global__ void __launch_bounds__(kRedThreads)
-adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int passes, int stages, DeviceError* err) {
+adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int lanes, int together, int stages, DeviceError* err) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ RedBars bars;
-  __shared__ int32_t list[kMaxList];
-  __shared__ int32_t row_id[BM];  // the row's adapter where this pass has it, else kNoAdapter
+  __shared__ TileList list;
+  __shared__ int16_t slot[BM];  // of a row's adapter in the list, -1 where it has none
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
   volatile int* abort_flag = &bars.abort_flag;
@@ -66,31 +71,16 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int p
   const int rank = split > 1 ? (int)cluster_rank() : 0;
   const int m_tiles = (ar.M + BM - 1) / BM;
   int unit = blockIdx.x / split;
-  const int pass = unit % passes;
-  unit /= passes;
+  const int first_pass = unit % lanes;
+  unit /= lanes;
   const int m0 = (unit % m_tiles) * BM;
-  const int proj = unit / m_tiles;
-  const int r = ar.p[proj].rank;
   const int rows = min(BM, ar.M - m0);
-  const int per_pass = kRankRows / r;
-
-  // (the ids are the caller's)
-  chain_wait();
-  chain_next();  // what follows reads nothing of this kernel's before its own wait
-  int32_t id[4];
-  load_ids(id, ar.ids, m0, rows, ar.n, lane);
-  int count = 0, first = kNoAdapter, last = kNoAdapter;
-  {
-    int32_t a = -1;
-    for (int i = 0; i < (pass + 1) * per_pass && (a = next_adapter(id, a)) != kNoAdapter; ++i) {
-      if (i < pass * per_pass) continue;
-      if (count == 0) first = a;
-      last = a;
-      if (threadIdx.x == 0) list[count] = a;
-      ++count;
-    }
-  }
-  if (count == 0) return;  // (the whole cluster: it shares tile and pass)
+  RedPart rp;
+  rp.first = together ? 0 : unit / m_tiles;
+  rp.count = together ? ar.projections : 1;
+  rp.rank0 = ar.p[rp.first].rank;
+  rp.cols = rp.count > 1 ? rp.rank0 + ar.p[1].rank : rp.rank0;
+  const int per_pass = kRankRows / rp.cols;
 
   const int kb_begin = (int)((int64_t)ar.kb * rank / split), kb_end = (int)((int64_t)ar.kb * (rank + 1) / split);
   const int a_bytes = ar.a_rows * BK * 2;
@@ -110,109 +100,126 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int p
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  chain_wait();
+  chain_next();  // what follows reads nothing of this kernel's before its own wait
+  if (warp >= 2) {
+    const int w = warp - 2, r = 32 * w + lane;
+    list_adapters(list, ar.ids, m0, rows, ar.n, w, lane);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    int at = -1;
+    const int32_t mine = list.id[r];
+    if (mine != kNoAdapter)
+      for (int i = 0; i < list.count; ++i) at = list.adapter[i] == mine ? i : at;
+    slot[r] = (int16_t)at;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
+  const int count = list.count;
 
-  if (warp == 0) {
-    int stage = 0;
-    uint32_t phase = 0, armed = 0;
-    bool ok = true;
-    for (int kb = kb_begin; kb < kb_end; ++kb) {
-      if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
-        if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2400 + stage);
-        *abort_flag = 1;
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
-      mbar_expect_tx_one(bar, a_bytes + count * r * BK * 2);
-      tma_load_2d_one(dst, &ar.x, bar, kb * BK, m0);
-      for (int i = 0; i < count; ++i)
-        tma_load_3d_one(dst + a_bytes + i * r * BK * 2, &ar.p[proj].a, bar, kb * BK, 0, list[i]);
-      armed |= 1u << stage;
-      if (++stage == stages) {
-        stage = 0;
-        phase ^= 1u;
-      }
-    }
-    if (*abort_flag && lane == 0) {
-      for (int s = 0; s < stages; ++s) {
-        if (!(armed & (1u << s))) continue;
-        const uint32_t par = s < stage ? phase : phase ^ 1u;
-        for (int i = 0; i < (1 << 16) && !mbar_try_wait(smem_u32(&bars.full[s]), par); ++i) {}
-      }
-    }
-  } else if (warp == 1) {
-    const int n_mma = (count * r + 15) / 16 * 16;
-    const uint32_t idesc =
-        (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 4) << 24) | (uint32_t(n_mma >> 3) << 17);
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int kb = kb_begin; kb < kb_end; ++kb) {
-      if (!mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
-        if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2500 + stage);
-        *abort_flag = 1;
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t sa = ring + stage * stage_bytes;
-      const uint64_t da = make_smem_desc(sa), db = make_smem_desc(sa + a_bytes);
-#pragma unroll
-      for (int k = 0; k < BK / UMMA_K; ++k) tc_mma_bf16_one(tmem, da + 2 * k, db + 2 * k, idesc, kb > kb_begin || k > 0);
-      tc_commit_one(smem_u32(&bars.empty[stage]));
-      if (++stage == stages) {
-        stage = 0;
-        phase ^= 1u;
-      }
-    }
-    if (ok) tc_commit_one(smem_u32(&bars.acc_full));
-  } else {
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const int32_t all = quarter == 0 ? id[0] : quarter == 1 ? id[1] : quarter == 2 ? id[2] : id[3];
-    const int32_t mine = all >= first && all <= last ? all : kNoAdapter;  // (ascending ids: the pass has all between)
-    row_id[row] = mine;
-    const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full), 0, abort_flag));
-    if (!ready) {
-      if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2600);
-      *abort_flag = 1;
-    } else if (quarter * 32 < rows) {
-      tc_fence_after();
-      const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
-      for (int i = 0; i < count; ++i) {
-        if (!__any_sync(0xffffffffu, mine == list[i])) continue;
-#pragma unroll 1
-        for (int j = 0; j < r; j += 8) {
-          uint32_t v[8];
-          tc_ld8(taddr + i * r + j, v);
-          tc_ld_wait();
-          if (mine == list[i]) {
-            uint4* dst = reinterpret_cast<uint4*>(part + row * kRedPitch + j);
-            dst[0] = make_uint4(v[0], v[1], v[2], v[3]);
-            dst[1] = make_uint4(v[4], v[5], v[6], v[7]);
-          }
+  int stage = 0;
+  uint32_t phase = 0, armed = 0, acc_phase = 0;
+  bool ok = true;
+  for (int pass = first_pass; pass * per_pass < count; pass += lanes) {  // (alike in all CTAs of the cluster)
+    const int begin = pass * per_pass, here = min(per_pass, count - begin);
+    if (warp == 0) {
+      fence_proxy_async();  // (the ring held the last pass's sums)
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
+          if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2400 + stage);
+          *abort_flag = 1;
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
+        mbar_expect_tx_one(bar, a_bytes + here * rp.cols * BK * 2);
+        tma_load_2d_one(dst, &ar.x, bar, kb * BK, m0);
+        for (int i = 0; i < here; ++i) {
+          const uint32_t to = dst + a_bytes + i * rp.cols * BK * 2;
+          tma_load_3d_one(to, &ar.p[rp.first].a, bar, kb * BK, 0, list.adapter[begin + i]);
+          if (rp.count > 1) tma_load_3d_one(to + rp.rank0 * BK * 2, &ar.p[1].a, bar, kb * BK, 0, list.adapter[begin + i]);
+        }
+        armed |= 1u << stage;
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      tc_fence_before();
+      if (*abort_flag && lane == 0) {
+        for (int s = 0; s < stages; ++s) {
+          if (!(armed & (1u << s))) continue;
+          const uint32_t par = s < stage ? phase : phase ^ 1u;
+          for (int i = 0; i < (1 << 16) && !mbar_try_wait(smem_u32(&bars.full[s]), par); ++i) {}
+        }
+      }
+    } else if (warp == 1) {
+      const int n_mma = (here * rp.cols + 15) / 16 * 16;
+      const uint32_t idesc =
+          (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 4) << 24) | (uint32_t(n_mma >> 3) << 17);
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
+          if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2500 + stage);
+          *abort_flag = 1;
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sa = ring + stage * stage_bytes;
+        const uint64_t da = make_smem_desc(sa), db = make_smem_desc(sa + a_bytes);
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k) tc_mma_bf16_one(tmem, da + 2 * k, db + 2 * k, idesc, kb > kb_begin || k > 0);
+        tc_commit_one(smem_u32(&bars.empty[stage]));
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) tc_commit_one(smem_u32(&bars.acc_full));
+    } else {
+      const int quarter = warp & 3;
+      const int row = quarter * 32 + lane;
+      const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full), acc_phase, abort_flag));
+      if (!ready) {
+        if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2600);
+        *abort_flag = 1;
+      } else if (quarter * 32 < rows) {
+        tc_fence_after();
+        const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
+        const int mine = slot[row] - begin;
+        for (int i = 0; i < here; ++i) {
+          if (!__any_sync(0xffffffffu, mine == i)) continue;
+#pragma unroll 1
+          for (int j = 0; j < rp.cols; j += 8) {
+            uint32_t v[8];
+            tc_ld8(taddr + i * rp.cols + j, v);
+            tc_ld_wait();
+            if (mine == i) {
+              uint4* dst = reinterpret_cast<uint4*>(part + row * kRedPitch + j);
+              dst[0] = make_uint4(v[0], v[1], v[2], v[3]);
+              dst[1] = make_uint4(v[4], v[5], v[6], v[7]);
+            }
+          }
+        }
+        tc_fence_before();
+      }
     }
+    acc_phase ^= 1u;
+    __syncthreads();
+    if (split > 1) cluster_barrier();
+    if (!*abort_flag) {
+      const uint32_t sums = smem_u32(part);
+      if (split == 1) add_rows<1>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
+      else if (split == 2) add_rows<2>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
+      else if (split == 4) add_rows<4>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
+      else add_rows<8>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
+    }
+    __syncthreads();
+    if (split > 1) cluster_barrier();  // no CTA goes on, or leaves, while another reads its sums
+    tc_fence_after();
   }
-
-  __syncthreads();
-  if (split > 1) cluster_barrier();
-  if (!*abort_flag) {
-    if (split == 1) add_rows<1>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
-    else if (split == 2) add_rows<2>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
-    else if (split == 4) add_rows<4>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
-    else add_rows<8>(ar, proj, m0, rows, smem_u32(part), row_id, rank);
-  }
-  __syncthreads();
-  if (split > 1) cluster_barrier();  // no CTA leaves while another reads its sums
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -231,16 +238,19 @@ int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s) {
   if (rc) return rc;
   // a tile has no more distinct adapters than rows
   const int most = r.n < BM ? (r.M < r.n ? r.M : r.n) : (r.M < BM ? r.M : BM);
-  int passes = 1;
-  for (int i = 0; i < r.projections; ++i) {
-    const int per_pass = kRankRows / r.p[i].rank;
-    const int need = (most + per_pass - 1) / per_pass;
-    if (need > passes) passes = need;
-  }
-  const int64_t units = (int64_t)m_tiles * passes * r.projections;
-  if (units > (1 << 26)) return ATENIA_ERR_SHAPE;
+  const bool together = r.projections > 1 && r.p[0].rank + r.p[1].rank <= kRankRows;
+  int widest = 0;
+  for (int i = 0; i < r.projections; ++i) widest = together ? widest + r.p[i].rank : (r.p[i].rank > widest ? r.p[i].rank : widest);
+  const int passes = (most + kRankRows / widest - 1) / (kRankRows / widest);
+  const int64_t tiles = (int64_t)m_tiles * (together ? 1 : r.projections);
+  if (tiles > (1 << 24)) return ATENIA_ERR_SHAPE;
+  // the reduction over a cluster until every SM has two CTAs, each with two k-blocks at least; then the passes that a tile can have side by side
+  // (most tiles of a prompt have one, and the CTAs of the others leave at once)
   int split = 1;
-  while (split < 8 && units * split < 2 * num_sms && r.kb >= 4 * split) split *= 2;
+  while (split < 8 && tiles * split < 2 * num_sms && r.kb >= 4 * split) split *= 2;
+  int64_t lanes = 2 * num_sms / (tiles * split);
+  lanes = lanes < 1 ? 1 : lanes > passes ? passes : lanes;
+  const int64_t units = tiles * lanes;
   const int stage_bytes = r.a_rows * BK * 2 + kRankRows * BK * 2;
   int stages = kRedRingBytes / stage_bytes;
   if (stages > kRedStages) stages = kRedStages;
@@ -263,7 +273,7 @@ int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s) {
   cfg.numAttrs = r.chained ? 2 : 1;
   count_launch();
   count_tcgen05_launch();
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_reduce_kernel, r, split, passes, stages, err);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_reduce_kernel, r, split, (int)lanes, (int)together, stages, err);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return (int)e;
 }

@@ -210,6 +210,34 @@ __device__ __forceinline__ void lanes_off(uint32_t (&off)[W], const int32_t (&id
   for (int w = 0; w < W; ++w) off[w] = __ballot_sync(0xffffffffu, id[w] != a);
 }
 
+// The distinct adapters of a tile's rows in the order of their first rows, by the 128 threads of four warps (thread r: row r).
+struct TileList {
+  int32_t id[BM];     // of the rows, kNoAdapter where a row has none
+  int32_t adapter[BM];
+  int32_t count;
+  int32_t in_warp[4];
+};
+__device__ __forceinline__ void list_adapters(TileList& l, const int32_t* __restrict__ ids, int64_t row0, int rows, int n, int w, int lane) {
+  const int r = 32 * w + lane;
+  const int32_t raw = r < rows ? ids[row0 + r] : -1;
+  const int32_t id = raw >= 0 && raw < n ? raw : kNoAdapter;
+  l.id[r] = id;
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  const uint32_t same = __match_any_sync(0xffffffffu, id);  // (every lane: not behind the test)
+  bool first = id != kNoAdapter && (same & ((1u << lane) - 1)) == 0;
+  for (int q = 0; q < 32 * w; ++q) first = first && l.id[q] != id;
+  const uint32_t b = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) l.in_warp[w] = __popc(b);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  int at = __popc(b & ((1u << lane) - 1)), total = 0;
+  for (int q = 0; q < 4; ++q) {
+    if (q < w) at += l.in_warp[q];
+    total += l.in_warp[q];
+  }
+  if (first) l.adapter[at] = id;
+  if (r == 0) l.count = total;
+}
+
 // dg, du and h of one element
 __device__ __forceinline__ void gate_grad(float dh, float g, float u, float& dg, float& du, float& h) {
   const float s = __fdividef(1.0f, 1.0f + __expf(-g));

@@ -11,7 +11,7 @@
 //   epilogue: eight warps; a lane holds a row, so the results go through shared memory to TMA, which writes whole lines (32 bytes a
 //             lane were 32 lines an access, and a tile's 5400 cycles of them hid only behind a reduction of 700 and more)
 //
-// Adapters as in dense_gemm.cu: behind the k-blocks of a tile come those of the adapters that its rows have, with the lanes
+// Adapters as in dense_gemm.cu: behind the k-blocks of a tile come the steps of the adapters that its rows have, with the lanes
 // of other rows disabled.
 //
 // No TMA multicast is used: every CTA fetches its own tiles (cp.async.bulk.tensor ... cta_group::2 only routes the completion to
@@ -170,6 +170,34 @@ __device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& 
   return o;
 }
 
+// The adapters' k-steps of a tile come in rounds: one or two stages with the tile's reduced rows (eight K = 16 steps a stage), then
+// up to four stages of B, as many steps in each as fit.
+template <int EPI>
+struct AdapterRounds {
+  static constexpr int kChunk = EPI == kDenseSwiGLU ? 64 * 32 : 128 * 32;  // a CTA's half of the B rows of a step
+  static constexpr int kSlots = kPairStageBytes / kChunk;
+  int steps0, steps, b_stages, left;
+  __device__ __forceinline__ AdapterRounds(const DenseAdapters& ad, int adapters) {
+    steps0 = (ad.seg[0].rank + 15) / 16;
+    steps = steps0 + (EPI == kDenseSwiGLU ? (ad.seg[1].rank + 15) / 16 : 0);
+    b_stages = kPairStages - (steps + 7) / 8;
+    left = adapters * steps;
+  }
+  __device__ __forceinline__ int seg(int step) const { return EPI == kDenseSwiGLU && step >= steps0 ? 1 : 0; }
+  __device__ __forceinline__ int rank_row(int step) const { return 16 * (seg(step) ? step - steps0 : step); }
+};
+// The adapters that this piece of a split reduction takes: every `split`-th of the ascending ids
+__device__ __forceinline__ int count_adapters(const int32_t (&id)[8], int piece, int split) {
+  int n = 0;
+  for (int32_t a = -1; (a = next_adapter(id, a)) != kNoAdapter;) ++n;
+  return n > piece ? (n - piece + split - 1) / split : 0;
+}
+__device__ __forceinline__ int32_t next_adapter_of(const int32_t (&id)[8], int32_t a, int& index, int piece, int split) {
+  do a = next_adapter(id, a);
+  while (index++ % split != piece);
+  return a;
+}
+
 template <int EPI, bool B_MN, int NP, bool AD>
 __global__ void __launch_bounds__(kPairThreads, 1)
 dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ PairArgs pa, const __grid_constant__ PairResults res,
@@ -294,25 +322,36 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         chain_wait();  // v is the kernel before's
         int32_t id[8];
         load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
+        AdapterRounds<EPI> r(ad, count_adapters(id, piece, split));
         int32_t a = -1;
-        for (int i_ad = 0; ok && (a = next_adapter(id, a)) != kNoAdapter; ++i_ad) {
-          if (i_ad % split != piece) continue;
-          for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
-            const int r = ad.seg[seg].rank;
-            for (int r0 = 0; ok && r0 < r; r0 += 64) {
-              if (!free_stage()) break;
-              const int steps = (min(r - r0, 64) + 15) / 16;
-              const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
-              constexpr int b_rows = N_OUT / 2;  // of each CTA
-              if (leader) mbar_expect_tx_one(full, 2 * steps * (BM * 32 + b_rows * 32));
-              const int n = t.n0 + (int)rank * b_rows;
-              for (int c = 0; c < steps; ++c) {
-                load_2d(dst + c * 4096, &ad.seg[seg].v, bar, r0 + 16 * c, t.m0 + (int)rank * BM);
-                load_3d(dst + kOperandBytes + c * 4096, &ad.seg[seg].b, bar, r0 + 16 * c, n, a);
-                if constexpr (EPI != kDenseSwiGLU) load_3d(dst + kOperandBytes + c * 4096 + 2048, &ad.seg[seg].b, bar, r0 + 16 * c, n + 64, a);
+        int index = 0, step = r.steps;
+        while (ok && r.left > 0) {
+          // the tile's reduced rows, for the stages of B that follow
+          for (int v0 = 0; ok && v0 < r.steps; v0 += 8) {
+            if (!free_stage()) break;
+            const int here = min(8, r.steps - v0);
+            const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
+            if (leader) mbar_expect_tx_one(full, 2 * here * BM * 32);
+            for (int c = 0; c < here; ++c) load_2d(dst + c * 4096, &ad.seg[r.seg(v0 + c)].v, bar, r.rank_row(v0 + c), t.m0 + (int)rank * BM);
+            next_stage();
+          }
+          for (int b = 0; ok && b < r.b_stages && r.left > 0; ++b) {
+            if (!free_stage()) break;
+            const int here = min(r.left, r.kSlots);
+            const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
+            if (leader) mbar_expect_tx_one(full, 2 * here * r.kChunk);
+            const int n = t.n0 + (int)rank * (N_OUT / 2);
+            for (int c = 0; c < here; ++c, ++step) {
+              if (step == r.steps) {
+                step = 0;
+                a = next_adapter_of(id, a, index, piece, split);
               }
-              next_stage();
+              const AdapterSegment& seg = ad.seg[r.seg(step)];
+              load_3d(dst + c * r.kChunk, &seg.b, bar, r.rank_row(step), n, a);
+              if constexpr (EPI != kDenseSwiGLU) load_3d(dst + c * r.kChunk + 2048, &seg.b, bar, r.rank_row(step), n + 64, a);
             }
+            r.left -= here;
+            next_stage();
           }
         }
       }
@@ -343,12 +382,15 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (ok) tc_fence_after();
         return ok;
       };
-      auto used = [&]() {
-        commit_both(smem_u32(&bars.empty[stage]), lead);
+      auto step_stage = [&]() {
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1u;
         }
+      };
+      auto used = [&]() {
+        commit_both(smem_u32(&bars.empty[stage]), lead);
+        step_stage();
       };
       constexpr uint32_t idesc = kPairIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(kPairN >> 3) << 17);
       for (int i = pair; ok && i < pa.tiles; i += num_pairs, ++it) {
@@ -375,23 +417,38 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           used();
         }
         if constexpr (AD) {
-          uint32_t off[8];
+          AdapterRounds<EPI> r(ad, count_adapters(id, piece, split));
+          uint32_t off[8] = {};
           int32_t a = -1;
-          for (int i_ad = 0; ok && (a = next_adapter(id, a)) != kNoAdapter; ++i_ad) {
-            if (i_ad % split != piece) continue;
-            lanes_off(off, id, a);
-            for (int seg = 0; ok && seg < (EPI == kDenseSwiGLU ? 2 : 1); ++seg) {
-              const int r = ad.seg[seg].rank;
-              for (int r0 = 0; ok && r0 < r; r0 += 64) {
-                if (!filled()) break;
-                const int steps = (min(r - r0, 64) + 15) / 16;
-                const uint32_t sa = ring + stage * kPairStageBytes;
+          int index = 0, step = r.steps;
+          while (ok && r.left > 0) {
+            const int v_stage = stage;
+            for (int v0 = 0; ok && v0 < r.steps; v0 += 8) {
+              if (!filled()) break;
+              step_stage();  // (given back behind the MMAs that read it)
+            }
+            for (int b = 0; ok && b < r.b_stages && r.left > 0; ++b) {
+              if (!filled()) break;
+              const int here = min(r.left, r.kSlots);
+              const uint32_t sb = ring + stage * kPairStageBytes;
+              for (int c = 0; c < here; ++c, ++step) {
+                if (step == r.steps) {
+                  step = 0;
+                  a = next_adapter_of(id, a, index, piece, split);
+                  lanes_off(off, id, a);
+                }
+                int v = v_stage + step / 8;
+                v = v >= kStages ? v - kStages : v;
                 constexpr uint32_t idesc_ad = kPairIdesc | (uint32_t(N_OUT >> 3) << 17);
-                for (int c = 0; c < steps; ++c)
-                  mma_lanes(d + seg * N_OUT, make_smem_desc_k16(sa + c * 4096), make_smem_desc_k16(sa + kOperandBytes + c * 4096), idesc_ad,
-                            off);
-                used();
+                mma_lanes(d + r.seg(step) * N_OUT, make_smem_desc_k16(ring + v * kPairStageBytes + (step % 8) * 4096),
+                          make_smem_desc_k16(sb + c * r.kChunk), idesc_ad, off);
               }
+              r.left -= here;
+              used();
+            }
+            for (int v0 = 0, v = v_stage; ok && v0 < r.steps; v0 += 8) {
+              commit_both(smem_u32(&bars.empty[v]), lead);
+              v = v + 1 == kStages ? 0 : v + 1;
             }
           }
         }
