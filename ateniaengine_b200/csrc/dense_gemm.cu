@@ -61,7 +61,6 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   __shared__ TileBars bars;
   __shared__ std::conditional_t<AD, TileList, NoAdapters> list;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
-  constexpr int kChunk = N_OUT * 32;  // a K = 16 step of one adapter's B rows
   const uint32_t v_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;  // reduced rows, then the ring
   const uint32_t ring = v_smem + (AD ? ta.v_bytes : 0);
   float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
@@ -109,14 +108,13 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
 
-  // Adapters: this rank takes every split-th of the list; an adapter is `steps` K = 16 steps (of both segments), and a stage holds
-  // `slots` of them.
-  constexpr int kSegments = EPI == kDenseSwiGLU ? 2 : 1;
-  int steps0 = 0, steps = 0;
-  const int slots = stage_bytes / kChunk;
+  // Adapters: this rank takes every split-th of the list; a stage holds `slots` of their chunks.
+  const std::conditional_t<AD, AdapterChunks<EPI>, NoAdapters> ac(ad);
+  int chunk_bytes = 1, v_bytes = 0, slots = 0;
   if constexpr (AD) {
-    steps0 = (ad.seg[0].rank + 15) / 16;
-    steps = steps0 + (kSegments > 1 ? (ad.seg[1].rank + 15) / 16 : 0);
+    chunk_bytes = N_OUT * ac.width * 2;
+    v_bytes = ta.a_rows * ac.width * 2;
+    slots = stage_bytes / chunk_bytes;
   }
   auto give_up = [&](int site) {
     if (lane == 0) report_error(ta.err, ATENIA_ERR_DEVICE_TIMEOUT, site);
@@ -185,20 +183,22 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if constexpr (AD) {
       // (B is not written by the kernel before; the reduced rows, which are, come with another warp)
       ok = ok && wait_all(&bars.listed, 0, 2110);
-      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * steps : 0;
-      for (int i = rank, step = 0; left > 0;) {
+      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * ac.chunks : 0;
+      for (int i = rank, c = 0; left > 0;) {
         if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2120 + stage))) break;
         const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
         const int here = min(left, slots);
-        mbar_expect_tx_one(bar, here * kChunk);
+        uint32_t bytes = 0;
+        for (int s = 0, at = c; s < here; ++s, at = at + 1 == ac.chunks ? 0 : at + 1) bytes += N_OUT * 2 * ad.seg[ac.seg(at)].width;
+        mbar_expect_tx_one(bar, bytes);
         for (int s = 0; s < here; ++s) {
-          const int seg = kSegments > 1 && step >= steps0;
-          const int r0 = 16 * (step - (seg ? steps0 : 0));
+          const AdapterSegment& seg = ad.seg[ac.seg(c)];
+          const int col = ac.column(ad, c);
 #pragma unroll
           for (int j = 0; j < N_OUT / 64; ++j)
-            tma_load_3d_one(dst + s * kChunk + j * 2048, &ad.seg[seg].b, bar, r0, n0 + 64 * j, list.adapter[i]);
-          if (++step == steps) {
-            step = 0;
+            tma_load_3d_one(dst + s * chunk_bytes + j * 128 * seg.width, &seg.b, bar, col, n0 + 64 * j, list.adapter[i]);
+          if (++c == ac.chunks) {
+            c = 0;
             i += split;
           }
         }
@@ -245,25 +245,25 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     }
     if constexpr (AD) {
       ok = ok && wait_all(&bars.listed, 0, 2210);
-      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * steps : 0;
+      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * ac.chunks : 0;
       if (left > 0) ok = wait_all(&bars.v_full, 0, 2220);
       uint32_t off[4] = {};
-      for (int i = rank, step = 0; ok && left > 0;) {
+      for (int i = rank, c = 0; ok && left > 0;) {
         if (!filled()) break;
         const uint32_t sb = ring + stage * stage_bytes;
         const int here = min(left, slots);
         for (int s = 0; s < here; ++s) {
-          if (step == 0) {
+          if (c == 0) {
             const int32_t a = list.adapter[i];
 #pragma unroll
             for (int w = 0; w < 4; ++w) off[w] = __ballot_sync(0xffffffffu, list.id[32 * w + lane] != a);
           }
-          const int seg = kSegments > 1 && step >= steps0;
           constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
-          tc_mma_bf16_lanes_one(tmem + seg * N_OUT, make_smem_desc_k16(v_smem + step * ta.a_rows * 32), make_smem_desc_k16(sb + s * kChunk),
-                                idesc_ad, off);
-          if (++step == steps) {
-            step = 0;
+          const int seg = ac.seg(c), width = ad.seg[seg].width, steps = ac.steps(ad, c);
+          const uint64_t da = make_smem_desc_width(v_smem + c * v_bytes, width), db = make_smem_desc_width(sb + s * chunk_bytes, width);
+          for (int k = 0; k < steps; ++k) tc_mma_bf16_lanes_one(tmem + seg * N_OUT, da + 2 * k, db + 2 * k, idesc_ad, off);
+          if (++c == ac.chunks) {
+            c = 0;
             i += split;
           }
         }
@@ -285,11 +285,10 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if constexpr (AD) {
       if (warp == 2 && wait_all(&bars.listed, 0, 2310) && list.count > rank) {
         const uint32_t bar = smem_u32(&bars.v_full);
-        mbar_expect_tx_one(bar, steps * ta.a_rows * 32);
-        for (int step = 0; step < steps; ++step) {
-          const int seg = kSegments > 1 && step >= steps0;
-          tma_load_2d_one(v_smem + step * ta.a_rows * 32, &ad.seg[seg].v, bar, 16 * (step - (seg ? steps0 : 0)), m0);
-        }
+        uint32_t bytes = 0;
+        for (int c = 0; c < ac.chunks; ++c) bytes += ta.a_rows * 2 * ad.seg[ac.seg(c)].width;
+        mbar_expect_tx_one(bar, bytes);
+        for (int c = 0; c < ac.chunks; ++c) tma_load_2d_one(v_smem + c * v_bytes, &ad.seg[ac.seg(c)].v, bar, ac.column(ad, c), m0);
         if (*abort_flag)
           for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, 0); ++i) {}
       }
@@ -378,8 +377,14 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
   if constexpr (AD) {
     ad = *g.adapters;
-    const int steps = (ad.seg[0].rank + 15) / 16 + (EPI == kDenseSwiGLU ? (ad.seg[1].rank + 15) / 16 : 0);
-    ta.v_bytes = (steps * rows * 32 + 1023) / 1024 * 1024;
+    int chunks = 0, width = 0;
+    for (int i = 0; i < (EPI == kDenseSwiGLU ? 2 : 1); ++i) {
+      const AdapterSegment& seg = ad.seg[i];
+      if (seg.rank == 0) continue;
+      chunks += (seg.rank + seg.width - 1) / seg.width;
+      width = seg.width > width ? seg.width : width;
+    }
+    ta.v_bytes = (chunks * rows * width * 2 + 1023) / 1024 * 1024;
   }
   int ring = TileSize<BN>::kRing - ta.v_bytes;
   if (ring < 3 * stage_bytes) ring = TileSize<256>::kRing - ta.v_bytes;  // (many reduced rows: one CTA per SM)

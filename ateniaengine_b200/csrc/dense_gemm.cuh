@@ -37,12 +37,15 @@ struct DenseProblem {
 // One projection's adapters beside the product: D[m, :] += B_a v[m, :] for a = ids[m].  (kDenseSwiGLU: segment 0 acts on the
 // gate columns, segment 1 on the up columns; a segment of rank 0 adds nothing.)
 struct AdapterSegment {
-  CUtensorMap v;  // [M, rank] bf16, box {16, rows}, 32-byte swizzle
-  CUtensorMap b;  // [n, N, rank] bf16, box {16, 64, 1}, 32-byte swizzle
-  int rank;
+  CUtensorMap v;  // [M, rank] bf16, box {width, rows}, swizzle of the box's width
+  CUtensorMap b;  // [n, N, rank] bf16, box {width, 64, 1}, likewise
+  int rank, width;  // adapter_width(rank)
   const __nv_bfloat16* v_ptr;
   const __nv_bfloat16* b_ptr;
 };
+// Rank columns of a box.  TMA takes as long for a row of 32 bytes as for one of 128 (about 4 cycles): boxes are as wide as the rank lets
+// them (columns past it are filled with zeros and left out of the MMAs).
+inline int adapter_width(int rank) { return rank > 32 ? 64 : rank > 16 ? 32 : 16; }
 struct DenseAdapters {
   AdapterSegment seg[2];
   const int32_t* ids;  // [M]; an id outside [0, n) means none
@@ -114,15 +117,38 @@ __device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(2) << 61;
   return d;
 }
-// K-major, 32-byte swizzle: rows of 32 bytes (one K = 16 step), eight-row groups 256 bytes apart.
-__device__ __forceinline__ uint64_t make_smem_desc_k16(uint32_t smem_addr) {
+// K-major operand of `width` (16, 32, 64) columns a row under the swizzle of that width; eight-row groups follow one another.
+__device__ __forceinline__ uint64_t make_smem_desc_width(uint32_t smem_addr, int width) {
   uint64_t d = static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
   d |= static_cast<uint64_t>(1) << 16;
-  d |= static_cast<uint64_t>(256 >> 4) << 32;
+  d |= static_cast<uint64_t>(width) << 32;  // 8 rows x 2 width bytes >> 4
   d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(6) << 61;
+  d |= static_cast<uint64_t>(width == 64 ? 2 : width == 32 ? 4 : 6) << 61;
   return d;
 }
+// The chunks (boxes of up to `width` rank columns) that one adapter of a product comes in: segment 0's, then segment 1's.
+template <int EPI>
+struct AdapterChunks {
+  int chunks0, chunks, width;  // width: of the wider segment, which sets the distance of chunks in shared memory
+  __device__ __forceinline__ explicit AdapterChunks(const DenseAdapters& ad) {
+    width = ad.seg[0].rank > 0 ? ad.seg[0].width : 0;
+    chunks0 = ad.seg[0].rank > 0 ? (ad.seg[0].rank + ad.seg[0].width - 1) / ad.seg[0].width : 0;
+    chunks = chunks0;
+    if constexpr (EPI == kDenseSwiGLU) {
+      if (ad.seg[1].rank > 0) {
+        chunks += (ad.seg[1].rank + ad.seg[1].width - 1) / ad.seg[1].width;
+        width = max(width, ad.seg[1].width);
+      }
+    }
+  }
+  __device__ __forceinline__ int seg(int c) const { return EPI == kDenseSwiGLU && c >= chunks0 ? 1 : 0; }
+  __device__ __forceinline__ int column(const DenseAdapters& ad, int c) const { return (seg(c) ? c - chunks0 : c) * ad.seg[seg(c)].width; }
+  // K = 16 steps of chunk c that hold rank columns
+  __device__ __forceinline__ int steps(const DenseAdapters& ad, int c) const {
+    const AdapterSegment& s = ad.seg[seg(c)];
+    return (min(s.width, s.rank - column(ad, c)) + 15) / 16;
+  }
+};
 template <bool MN>
 __device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
   return MN ? make_smem_desc_mn(smem_addr) : make_smem_desc(smem_addr);
@@ -211,7 +237,7 @@ __device__ __forceinline__ void lanes_off(uint32_t (&off)[W], const int32_t (&id
 }
 
 // The distinct adapters of a tile's rows in the order of their first rows, by the 128 threads of four warps (thread r: row r).
-struct TileList {
+struct __align__(16) TileList {
   int32_t id[BM];     // of the rows, kNoAdapter where a row has none
   int32_t adapter[BM];
   int32_t count;
@@ -225,7 +251,15 @@ __device__ __forceinline__ void list_adapters(TileList& l, const int32_t* __rest
   asm volatile("bar.sync 1, 128;" ::: "memory");
   const uint32_t same = __match_any_sync(0xffffffffu, id);  // (every lane: not behind the test)
   bool first = id != kNoAdapter && (same & ((1u << lane) - 1)) == 0;
-  for (int q = 0; q < 32 * w; ++q) first = first && l.id[q] != id;
+  if (w > 0) first = first && l.id[32 * w - 1] != id;
+  if (__any_sync(0xffffffffu, first)) {  // (in a prompt most warps' rows only go on with the last one's adapter)
+    const int4* before = reinterpret_cast<const int4*>(l.id);
+#pragma unroll 4
+    for (int q = 0; q < 8 * w; ++q) {
+      const int4 v = before[q];
+      first = first && v.x != id && v.y != id && v.z != id && v.w != id;
+    }
+  }
   const uint32_t b = __ballot_sync(0xffffffffu, first);
   if (lane == 0) l.in_warp[w] = __popc(b);
   asm volatile("bar.sync 1, 128;" ::: "memory");

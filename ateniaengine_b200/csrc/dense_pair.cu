@@ -170,21 +170,20 @@ __device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& 
   return o;
 }
 
-// The adapters' k-steps of a tile come in rounds: one or two stages with the tile's reduced rows (eight K = 16 steps a stage), then
-// up to four stages of B, as many steps in each as fit.
+// The adapters' chunks of a tile come in rounds: one or two stages with the tile's reduced rows, then stages of B, as many chunks in
+// each as fit, until the ring is full.
 template <int EPI>
-struct AdapterRounds {
-  static constexpr int kChunk = EPI == kDenseSwiGLU ? 64 * 32 : 128 * 32;  // a CTA's half of the B rows of a step
-  static constexpr int kSlots = kPairStageBytes / kChunk;
-  int steps0, steps, b_stages, left;
-  __device__ __forceinline__ AdapterRounds(const DenseAdapters& ad, int adapters) {
-    steps0 = (ad.seg[0].rank + 15) / 16;
-    steps = steps0 + (EPI == kDenseSwiGLU ? (ad.seg[1].rank + 15) / 16 : 0);
-    b_stages = kPairStages - (steps + 7) / 8;
-    left = adapters * steps;
+struct AdapterRounds : AdapterChunks<EPI> {
+  static constexpr int kRows = EPI == kDenseSwiGLU ? 64 : 128;  // a CTA's half of the B rows of a chunk
+  int v_bytes, v_slots, b_bytes, b_slots, b_stages, left;
+  __device__ __forceinline__ AdapterRounds(const DenseAdapters& ad, int adapters) : AdapterChunks<EPI>(ad) {
+    v_bytes = BM * 2 * this->width;
+    v_slots = kPairStageBytes / v_bytes;
+    b_bytes = kRows * 2 * this->width;
+    b_slots = kPairStageBytes / b_bytes;
+    b_stages = kPairStages - (this->chunks + v_slots - 1) / v_slots;
+    left = adapters * this->chunks;
   }
-  __device__ __forceinline__ int seg(int step) const { return EPI == kDenseSwiGLU && step >= steps0 ? 1 : 0; }
-  __device__ __forceinline__ int rank_row(int step) const { return 16 * (seg(step) ? step - steps0 : step); }
 };
 // The adapters that this piece of a split reduction takes: every `split`-th of the ascending ids
 __device__ __forceinline__ int count_adapters(const int32_t (&id)[8], int piece, int split) {
@@ -324,31 +323,40 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
         AdapterRounds<EPI> r(ad, count_adapters(id, piece, split));
         int32_t a = -1;
-        int index = 0, step = r.steps;
+        int index = 0, at = r.chunks;
         while (ok && r.left > 0) {
           // the tile's reduced rows, for the stages of B that follow
-          for (int v0 = 0; ok && v0 < r.steps; v0 += 8) {
+          for (int v0 = 0; ok && v0 < r.chunks; v0 += r.v_slots) {
             if (!free_stage()) break;
-            const int here = min(8, r.steps - v0);
+            const int here = min(r.v_slots, r.chunks - v0);
             const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
-            if (leader) mbar_expect_tx_one(full, 2 * here * BM * 32);
-            for (int c = 0; c < here; ++c) load_2d(dst + c * 4096, &ad.seg[r.seg(v0 + c)].v, bar, r.rank_row(v0 + c), t.m0 + (int)rank * BM);
+            uint32_t bytes = 0;
+            for (int c = 0; c < here; ++c) bytes += BM * 2 * ad.seg[r.seg(v0 + c)].width;
+            if (leader) mbar_expect_tx_one(full, 2 * bytes);
+            for (int c = 0; c < here; ++c)
+              load_2d(dst + c * r.v_bytes, &ad.seg[r.seg(v0 + c)].v, bar, r.column(ad, v0 + c), t.m0 + (int)rank * BM);
             next_stage();
           }
           for (int b = 0; ok && b < r.b_stages && r.left > 0; ++b) {
             if (!free_stage()) break;
-            const int here = min(r.left, r.kSlots);
+            const int here = min(r.left, r.b_slots);
             const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
-            if (leader) mbar_expect_tx_one(full, 2 * here * r.kChunk);
+            uint32_t bytes = 0;
+            for (int c = 0, q = at; c < here; ++c) {
+              q = q == r.chunks ? 0 : q;
+              bytes += r.kRows * 2 * ad.seg[r.seg(q++)].width;
+            }
+            if (leader) mbar_expect_tx_one(full, 2 * bytes);
             const int n = t.n0 + (int)rank * (N_OUT / 2);
-            for (int c = 0; c < here; ++c, ++step) {
-              if (step == r.steps) {
-                step = 0;
+            for (int c = 0; c < here; ++c, ++at) {
+              if (at == r.chunks) {
+                at = 0;
                 a = next_adapter_of(id, a, index, piece, split);
               }
-              const AdapterSegment& seg = ad.seg[r.seg(step)];
-              load_3d(dst + c * r.kChunk, &seg.b, bar, r.rank_row(step), n, a);
-              if constexpr (EPI != kDenseSwiGLU) load_3d(dst + c * r.kChunk + 2048, &seg.b, bar, r.rank_row(step), n + 64, a);
+              const AdapterSegment& seg = ad.seg[r.seg(at)];
+              const int col = r.column(ad, at);
+              load_3d(dst + c * r.b_bytes, &seg.b, bar, col, n, a);
+              if constexpr (EPI != kDenseSwiGLU) load_3d(dst + c * r.b_bytes + 128 * seg.width, &seg.b, bar, col, n + 64, a);
             }
             r.left -= here;
             next_stage();
@@ -420,33 +428,35 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           AdapterRounds<EPI> r(ad, count_adapters(id, piece, split));
           uint32_t off[8] = {};
           int32_t a = -1;
-          int index = 0, step = r.steps;
+          int index = 0, at = r.chunks;
           while (ok && r.left > 0) {
             const int v_stage = stage;
-            for (int v0 = 0; ok && v0 < r.steps; v0 += 8) {
+            for (int v0 = 0; ok && v0 < r.chunks; v0 += r.v_slots) {
               if (!filled()) break;
               step_stage();  // (given back behind the MMAs that read it)
             }
             for (int b = 0; ok && b < r.b_stages && r.left > 0; ++b) {
               if (!filled()) break;
-              const int here = min(r.left, r.kSlots);
+              const int here = min(r.left, r.b_slots);
               const uint32_t sb = ring + stage * kPairStageBytes;
-              for (int c = 0; c < here; ++c, ++step) {
-                if (step == r.steps) {
-                  step = 0;
+              for (int c = 0; c < here; ++c, ++at) {
+                if (at == r.chunks) {
+                  at = 0;
                   a = next_adapter_of(id, a, index, piece, split);
                   lanes_off(off, id, a);
                 }
-                int v = v_stage + step / 8;
+                int v = v_stage + at / r.v_slots;
                 v = v >= kStages ? v - kStages : v;
+                const int seg = r.seg(at), width = ad.seg[seg].width, steps = r.steps(ad, at);
                 constexpr uint32_t idesc_ad = kPairIdesc | (uint32_t(N_OUT >> 3) << 17);
-                mma_lanes(d + r.seg(step) * N_OUT, make_smem_desc_k16(ring + v * kPairStageBytes + (step % 8) * 4096),
-                          make_smem_desc_k16(sb + c * r.kChunk), idesc_ad, off);
+                const uint64_t da = make_smem_desc_width(ring + v * kPairStageBytes + (at % r.v_slots) * r.v_bytes, width);
+                const uint64_t db = make_smem_desc_width(sb + c * r.b_bytes, width);
+                for (int k = 0; k < steps; ++k) mma_lanes(d + seg * N_OUT, da + 2 * k, db + 2 * k, idesc_ad, off);
               }
               r.left -= here;
               used();
             }
-            for (int v0 = 0, v = v_stage; ok && v0 < r.steps; v0 += 8) {
+            for (int v0 = 0, v = v_stage; ok && v0 < r.chunks; v0 += r.v_slots) {
               commit_both(smem_u32(&bars.empty[v]), lead);
               v = v + 1 == kStages ? 0 : v + 1;
             }

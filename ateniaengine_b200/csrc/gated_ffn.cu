@@ -74,8 +74,10 @@ int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, i
   const uint64_t r = (uint64_t)a.rank;
   const bool few = dense_gemv_rows(T, out, in);  // (the kernels for one or two tokens read through plain pointers)
   int rc = few_reduce ? ATENIA_OK : encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
-  if (!rc && !few) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {16, (uint32_t)a_rows, 1}, 32);
-  if (!rc && !few) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {16, 64, 1}, 32);
+  const uint32_t width = (uint32_t)adapter_width(a.rank);
+  seg->width = (int)width;
+  if (!rc && !few) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {width, (uint32_t)a_rows, 1}, 2 * width);
+  if (!rc && !few) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {width, 64, 1}, 2 * width);
   red->scale = a.scale;
   red->v = static_cast<__nv_bfloat16*>(v);
   red->rank = seg->rank = a.rank;
