@@ -108,13 +108,13 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
 
-  // Adapters: this rank takes every split-th of the list; a stage holds `slots` of their chunks.
+  // Adapters: this rank takes every split-th of the list.  A stage holds `group` of them, or (group 0) one chunk of one.
   const std::conditional_t<AD, AdapterChunks<EPI>, NoAdapters> ac(ad);
-  int chunk_bytes = 1, v_bytes = 0, slots = 0;
+  int chunk_bytes = 0, v_bytes = 0, group = 0;
   if constexpr (AD) {
-    chunk_bytes = N_OUT * ac.width * 2;
-    v_bytes = ta.a_rows * ac.width * 2;
-    slots = stage_bytes / chunk_bytes;
+    chunk_bytes = N_OUT * ac.widest * 2;
+    v_bytes = ta.a_rows * ac.widest * 2;
+    group = stage_bytes / (chunk_bytes * ac.chunks);
   }
   auto give_up = [&](int site) {
     if (lane == 0) report_error(ta.err, ATENIA_ERR_DEVICE_TIMEOUT, site);
@@ -183,27 +183,45 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if constexpr (AD) {
       // (B is not written by the kernel before; the reduced rows, which are, come with another warp)
       ok = ok && wait_all(&bars.listed, 0, 2110);
-      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * ac.chunks : 0;
-      for (int i = rank, c = 0; left > 0;) {
-        if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2120 + stage))) break;
-        const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
-        const int here = min(left, slots);
-        uint32_t bytes = 0;
-        for (int s = 0, at = c; s < here; ++s, at = at + 1 == ac.chunks ? 0 : at + 1) bytes += N_OUT * 2 * ad.seg[ac.seg(at)].width;
-        mbar_expect_tx_one(bar, bytes);
-        for (int s = 0; s < here; ++s) {
-          const AdapterSegment& seg = ad.seg[ac.seg(c)];
-          const int col = ac.column(ad, c);
+      const int count = ok ? list.count : 0;
+      int left = count > rank ? (count - rank + split - 1) / split : 0;
+      auto load_chunk = [&](int c, uint32_t dst, uint32_t bar, int adapter) {
+        const CUtensorMap* map = &ad.seg[ac.second[c]].b;
 #pragma unroll
-          for (int j = 0; j < N_OUT / 64; ++j)
-            tma_load_3d_one(dst + s * chunk_bytes + j * 128 * seg.width, &seg.b, bar, col, n0 + 64 * j, list.adapter[i]);
-          if (++c == ac.chunks) {
-            c = 0;
-            i += split;
+        for (int j = 0; j < N_OUT / 64; ++j) tma_load_3d_one(dst + j * 128 * ac.width[c], map, bar, ac.column[c], n0 + 64 * j, adapter);
+      };
+      for (int i = rank; left > 0;) {
+        const int here = group > 0 ? min(left, group) : 1;
+        if (group > 0) {
+          if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2120 + stage))) break;
+          const uint32_t bar = smem_u32(&bars.full[stage]);
+          uint32_t dst = ring + stage * stage_bytes;
+          mbar_expect_tx_one(bar, here * ac.columns * N_OUT * 2);
+          for (int s = 0; s < here; ++s, i += split) {
+            const int adapter = list.adapter[i];
+#pragma unroll
+            for (int c = 0; c < kMaxChunks; ++c) {
+              if (c >= ac.chunks) break;
+              load_chunk(c, dst, bar, adapter);
+              dst += chunk_bytes;
+            }
           }
+          next_stage();
+        } else {
+          const int adapter = list.adapter[i];
+          i += split;
+#pragma unroll
+          for (int c = 0; c < kMaxChunks; ++c) {
+            if (c >= ac.chunks) break;
+            if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2120 + stage))) break;
+            const uint32_t bar = smem_u32(&bars.full[stage]);
+            mbar_expect_tx_one(bar, ac.width[c] * N_OUT * 2);
+            load_chunk(c, ring + stage * stage_bytes, bar, adapter);
+            next_stage();
+          }
+          if (!ok) break;
         }
         left -= here;
-        next_stage();
       }
     }
     chain_wait();
@@ -245,30 +263,43 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     }
     if constexpr (AD) {
       ok = ok && wait_all(&bars.listed, 0, 2210);
-      int left = ok && list.count > rank ? (list.count - rank + split - 1) / split * ac.chunks : 0;
+      const int count = ok ? list.count : 0;
+      int left = count > rank ? (count - rank + split - 1) / split : 0;
       if (left > 0) ok = wait_all(&bars.v_full, 0, 2220);
       uint32_t off[4] = {};
-      for (int i = rank, c = 0; ok && left > 0;) {
-        if (!filled()) break;
-        const uint32_t sb = ring + stage * stage_bytes;
-        const int here = min(left, slots);
-        for (int s = 0; s < here; ++s) {
-          if (c == 0) {
-            const int32_t a = list.adapter[i];
+      uint64_t dv[kMaxChunks];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) off[w] = __ballot_sync(0xffffffffu, list.id[32 * w + lane] != a);
-          }
-          constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
-          const int seg = ac.seg(c), width = ad.seg[seg].width, steps = ac.steps(ad, c);
-          const uint64_t da = make_smem_desc_width(v_smem + c * v_bytes, width), db = make_smem_desc_width(sb + s * chunk_bytes, width);
-          for (int k = 0; k < steps; ++k) tc_mma_bf16_lanes_one(tmem + seg * N_OUT, da + 2 * k, db + 2 * k, idesc_ad, off);
-          if (++c == ac.chunks) {
-            c = 0;
-            i += split;
+      for (int c = 0; c < kMaxChunks; ++c) dv[c] = make_smem_desc_width(v_smem + c * v_bytes, ac.width[c]);
+      int32_t id[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) id[w] = ok ? list.id[32 * w + lane] : kNoAdapter;
+      auto add_chunk = [&](int c, uint32_t at) {
+        constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
+        const uint64_t db = make_smem_desc_width(at, ac.width[c]);
+        const uint32_t d = tmem + (ac.second[c] ? N_OUT : 0);
+#pragma unroll 1
+        for (int k = 0; k < ac.steps[c]; ++k) tc_mma_bf16_lanes_one(d, dv[c] + 2 * k, db + 2 * k, idesc_ad, off);
+      };
+      for (int i = rank; ok && left > 0;) {
+        const int here = group > 0 ? min(left, group) : 1;
+        if (group > 0 && !filled()) break;
+        uint32_t at = ring + stage * stage_bytes;
+        for (int s = 0; s < here; ++s, i += split) {
+          lanes_off(off, id, list.adapter[i]);
+#pragma unroll
+          for (int c = 0; c < kMaxChunks; ++c) {
+            if (c >= ac.chunks) break;
+            if (group == 0) {
+              if (!filled()) break;
+              at = ring + stage * stage_bytes;
+            }
+            add_chunk(c, at);
+            at += chunk_bytes;
+            if (group == 0) used();
           }
         }
+        if (group > 0) used();
         left -= here;
-        used();
       }
     }
     if (ok) tc_commit_one(smem_u32(&bars.acc_full));
@@ -285,10 +316,10 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if constexpr (AD) {
       if (warp == 2 && wait_all(&bars.listed, 0, 2310) && list.count > rank) {
         const uint32_t bar = smem_u32(&bars.v_full);
-        uint32_t bytes = 0;
-        for (int c = 0; c < ac.chunks; ++c) bytes += ta.a_rows * 2 * ad.seg[ac.seg(c)].width;
-        mbar_expect_tx_one(bar, bytes);
-        for (int c = 0; c < ac.chunks; ++c) tma_load_2d_one(v_smem + c * v_bytes, &ad.seg[ac.seg(c)].v, bar, ac.column(ad, c), m0);
+        mbar_expect_tx_one(bar, ta.a_rows * 2 * ac.columns);
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; ++c)
+          if (c < ac.chunks) tma_load_2d_one(v_smem + c * v_bytes, &ad.seg[ac.second[c]].v, bar, ac.column[c], m0);
         if (*abort_flag)
           for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, 0); ++i) {}
       }

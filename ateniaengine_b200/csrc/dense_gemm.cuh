@@ -126,27 +126,30 @@ __device__ __forceinline__ uint64_t make_smem_desc_width(uint32_t smem_addr, int
   d |= static_cast<uint64_t>(width == 64 ? 2 : width == 32 ? 4 : 6) << 61;
   return d;
 }
-// The chunks (boxes of up to `width` rank columns) that one adapter of a product comes in: segment 0's, then segment 1's.
+// The chunks (boxes of up to `width` rank columns) that one adapter of a product comes in: segment 0's, then segment 1's; at most
+// four.  Loops over them are unrolled, so that what they read stays in registers.
+constexpr int kMaxChunks = 4;
 template <int EPI>
 struct AdapterChunks {
-  int chunks0, chunks, width;  // width: of the wider segment, which sets the distance of chunks in shared memory
+  int chunks, widest;  // widest: the wider segment's width, which sets the distance of chunks in shared memory
+  int width[kMaxChunks], column[kMaxChunks], steps[kMaxChunks];  // steps: K = 16 steps that hold rank columns
+  bool second[kMaxChunks];                                       // of segment 1
+  int columns;                                                   // of all chunks
   __device__ __forceinline__ explicit AdapterChunks(const DenseAdapters& ad) {
-    width = ad.seg[0].rank > 0 ? ad.seg[0].width : 0;
-    chunks0 = ad.seg[0].rank > 0 ? (ad.seg[0].rank + ad.seg[0].width - 1) / ad.seg[0].width : 0;
-    chunks = chunks0;
-    if constexpr (EPI == kDenseSwiGLU) {
-      if (ad.seg[1].rank > 0) {
-        chunks += (ad.seg[1].rank + ad.seg[1].width - 1) / ad.seg[1].width;
-        width = max(width, ad.seg[1].width);
-      }
+    const int w0 = ad.seg[0].rank > 0 ? ad.seg[0].width : 0;
+    const int w1 = EPI == kDenseSwiGLU && ad.seg[1].rank > 0 ? ad.seg[1].width : 0;
+    const int n0 = w0 ? (ad.seg[0].rank + w0 - 1) / w0 : 0, n1 = w1 ? (ad.seg[1].rank + w1 - 1) / w1 : 0;
+    chunks = n0 + n1;
+    widest = max(w0, w1);
+    columns = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxChunks; ++c) {
+      second[c] = c >= n0;
+      width[c] = second[c] ? w1 : w0;
+      column[c] = (second[c] ? c - n0 : c) * width[c];
+      steps[c] = c < chunks ? (min(width[c], (second[c] ? ad.seg[1].rank : ad.seg[0].rank) - column[c]) + 15) / 16 : 0;
+      columns += c < chunks ? width[c] : 0;
     }
-  }
-  __device__ __forceinline__ int seg(int c) const { return EPI == kDenseSwiGLU && c >= chunks0 ? 1 : 0; }
-  __device__ __forceinline__ int column(const DenseAdapters& ad, int c) const { return (seg(c) ? c - chunks0 : c) * ad.seg[seg(c)].width; }
-  // K = 16 steps of chunk c that hold rank columns
-  __device__ __forceinline__ int steps(const DenseAdapters& ad, int c) const {
-    const AdapterSegment& s = ad.seg[seg(c)];
-    return (min(s.width, s.rank - column(ad, c)) + 15) / 16;
   }
 };
 template <bool MN>

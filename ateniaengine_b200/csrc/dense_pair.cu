@@ -41,8 +41,8 @@ struct PairSize {
   static constexpr int kCols = EPI == kDenseGateGrad ? 32 : 64;
   static constexpr int kWarpBytes = kResults * kCols * 2 * 32;
   static constexpr int kStages = EPI == kDenseGateGrad ? 5 : 6;
-  static constexpr int kSmem = kStages * kPairStageBytes + kEpiWarps * kWarpBytes + 1024;
-  static_assert(kSmem <= 226 * 1024 && BM * (kPairN + 4) * 4 <= kStages * kPairStageBytes, "");
+  static constexpr int kSmem = kStages * kPairStageBytes + kEpiWarps * kWarpBytes + 1024;  // (and 1.4 KiB of barriers and lists)
+  static_assert(kSmem <= 225 * 1024 && BM * (kPairN + 4) * 4 <= kStages * kPairStageBytes, "");
 };
 constexpr int kBand = 8;
 
@@ -51,6 +51,8 @@ struct __align__(8) PairBars {
   uint64_t empty[kPairStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
+  uint64_t listed[2];    // the lists of a tile's adapters, and the MMA issuer done with them
+  uint64_t unlisted[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -170,32 +172,25 @@ __device__ __forceinline__ Tile tile_of(const Problems<NP>& ps, const PairArgs& 
   return o;
 }
 
-// The adapters' chunks of a tile come in rounds: one or two stages with the tile's reduced rows, then stages of B, as many chunks in
-// each as fit, until the ring is full.
+// The adapters of a tile come in rounds: one or two stages with the tile's reduced rows, then stages of B, as many adapters in each as
+// fit, until the ring is full.
 template <int EPI>
 struct AdapterRounds : AdapterChunks<EPI> {
   static constexpr int kRows = EPI == kDenseSwiGLU ? 64 : 128;  // a CTA's half of the B rows of a chunk
-  int v_bytes, v_slots, b_bytes, b_slots, b_stages, left;
-  __device__ __forceinline__ AdapterRounds(const DenseAdapters& ad, int adapters) : AdapterChunks<EPI>(ad) {
-    v_bytes = BM * 2 * this->width;
+  int v_bytes, v_slots, b_bytes, group, b_stages;
+  __device__ __forceinline__ explicit AdapterRounds(const DenseAdapters& ad) : AdapterChunks<EPI>(ad) {
+    v_bytes = BM * 2 * this->widest;
     v_slots = kPairStageBytes / v_bytes;
-    b_bytes = kRows * 2 * this->width;
-    b_slots = kPairStageBytes / b_bytes;
-    b_stages = kPairStages - (this->chunks + v_slots - 1) / v_slots;
-    left = adapters * this->chunks;
+    b_bytes = kRows * 2 * this->widest;
+    group = kPairStageBytes / (b_bytes * this->chunks);  // (four chunks of 64 columns are a stage)
+    b_stages = kPairStages - (this->chunks > v_slots ? 2 : 1);
   }
 };
-// The adapters that this piece of a split reduction takes: every `split`-th of the ascending ids
-__device__ __forceinline__ int count_adapters(const int32_t (&id)[8], int piece, int split) {
-  int n = 0;
-  for (int32_t a = -1; (a = next_adapter(id, a)) != kNoAdapter;) ++n;
-  return n > piece ? (n - piece + split - 1) / split : 0;
-}
-__device__ __forceinline__ int32_t next_adapter_of(const int32_t (&id)[8], int32_t a, int& index, int piece, int split) {
-  do a = next_adapter(id, a);
-  while (index++ % split != piece);
-  return a;
-}
+// The adapters of two tiles, found by the producer between its loads (in ascending order; of a split reduction every split-th)
+struct PairLists {
+  uint16_t adapter[2][kPairM];
+  int count[2];
+};
 
 template <int EPI, bool B_MN, int NP, bool AD>
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -203,6 +198,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PairBars bars;
+  __shared__ std::conditional_t<AD, PairLists, NoAdapters> lists;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
   volatile int* abort_flag = &bars.abort_flag;
@@ -231,6 +227,8 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&bars.acc_full[b]), 1);
       mbar_init(smem_u32(&bars.acc_empty[b]), 2 * kEpiWarps);
+      mbar_init(smem_u32(&bars.listed[b]), 1);
+      mbar_init(smem_u32(&bars.unlisted[b]), 1);
     }
     bars.abort_flag = 0;
     fence_barrier_init();
@@ -301,9 +299,33 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       }
     }
     if (!(AD && pa.a_early)) chain_wait();
-    for (int i = pair; ok && i < pa.tiles; i += num_pairs) {
+    const std::conditional_t<AD, AdapterRounds<EPI>, NoAdapters> r(ad);
+    int it = 0;
+    for (int i = pair; ok && i < pa.tiles; i += num_pairs, ++it) {
       const Tile t = tile_of<EPI, NP>(ps, pa, i);
       const DenseProblem& p = ps.p[NP > 1 ? t.which : 0];
+      int32_t id[8], last = -1;
+      int found = 0, index = 0;
+      auto find_next = [&]() {
+        if constexpr (AD) {
+          last = next_adapter(id, last);
+          if (last == kNoAdapter) return;
+          if (index++ % split != piece) return;
+          if (lane == 0) lists.adapter[it & 1][found] = (uint16_t)last;
+          ++found;
+        }
+      };
+      if constexpr (AD) {
+        load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
+        // (the leader's issuer is done with the list of the tile before last; the other CTA's list is the producer's own)
+        if (leader && !mbar_wait(smem_u32(&bars.unlisted[it & 1]), ((it >> 1) & 1) ^ 1u, abort_flag)) {
+          if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 2710 + (it & 1));
+          *abort_flag = 1;
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
       for (int kb = kb_begin(p), end = kb_end(p); kb < end; ++kb) {
         const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
         if (ahead > 0) {  // (the first tile's first blocks)
@@ -316,49 +338,53 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           load_a(p, t, kb, dst, bar);
         }
         next_stage();
+        if (AD && last != kNoAdapter && kb > kb_begin(p)) find_next();
       }
       if constexpr (AD) {
+        while (ok && last != kNoAdapter) find_next();
+        __syncwarp();
+        if (leader && lane == 0) {
+          lists.count[it & 1] = found;
+          mbar_arrive(smem_u32(&bars.listed[it & 1]));
+        }
         chain_wait();  // v is the kernel before's
-        int32_t id[8];
-        load_ids(id, ad.ids, t.m0, p.M - t.m0, ad.n, lane);
-        AdapterRounds<EPI> r(ad, count_adapters(id, piece, split));
-        int32_t a = -1;
-        int index = 0, at = r.chunks;
-        while (ok && r.left > 0) {
+        for (int done = 0; ok && done < found;) {
           // the tile's reduced rows, for the stages of B that follow
-          for (int v0 = 0; ok && v0 < r.chunks; v0 += r.v_slots) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (half * r.v_slots >= r.chunks || !ok) break;
             if (!free_stage()) break;
-            const int here = min(r.v_slots, r.chunks - v0);
             const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
-            uint32_t bytes = 0;
-            for (int c = 0; c < here; ++c) bytes += BM * 2 * ad.seg[r.seg(v0 + c)].width;
-            if (leader) mbar_expect_tx_one(full, 2 * bytes);
-            for (int c = 0; c < here; ++c)
-              load_2d(dst + c * r.v_bytes, &ad.seg[r.seg(v0 + c)].v, bar, r.column(ad, v0 + c), t.m0 + (int)rank * BM);
+            int columns = 0;
+#pragma unroll
+            for (int c = 0; c < kMaxChunks; ++c)
+              if (c < r.chunks && c >= half * r.v_slots && c < (half + 1) * r.v_slots) columns += r.width[c];
+            if (leader) mbar_expect_tx_one(full, 2 * columns * BM * 2);
+#pragma unroll
+            for (int c = 0; c < kMaxChunks; ++c)
+              if (c < r.chunks && c >= half * r.v_slots && c < (half + 1) * r.v_slots)
+                load_2d(dst + (c - half * r.v_slots) * r.v_bytes, &ad.seg[r.second[c]].v, bar, r.column[c], t.m0 + (int)rank * BM);
             next_stage();
           }
-          for (int b = 0; ok && b < r.b_stages && r.left > 0; ++b) {
+          for (int b = 0; ok && b < r.b_stages && done < found; ++b) {
             if (!free_stage()) break;
-            const int here = min(r.left, r.b_slots);
-            const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead), dst = ring + stage * kPairStageBytes;
-            uint32_t bytes = 0;
-            for (int c = 0, q = at; c < here; ++c) {
-              q = q == r.chunks ? 0 : q;
-              bytes += r.kRows * 2 * ad.seg[r.seg(q++)].width;
-            }
-            if (leader) mbar_expect_tx_one(full, 2 * bytes);
+            const int here = min(found - done, r.group);
+            const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead);
+            uint32_t dst = ring + stage * kPairStageBytes;
+            if (leader) mbar_expect_tx_one(full, 2 * here * r.columns * r.kRows * 2);
             const int n = t.n0 + (int)rank * (N_OUT / 2);
-            for (int c = 0; c < here; ++c, ++at) {
-              if (at == r.chunks) {
-                at = 0;
-                a = next_adapter_of(id, a, index, piece, split);
+            for (int q = 0; q < here; ++q) {
+              const int a = lists.adapter[it & 1][done + q];
+#pragma unroll
+              for (int c = 0; c < kMaxChunks; ++c) {
+                if (c >= r.chunks) break;
+                const CUtensorMap* map = &ad.seg[r.second[c]].b;
+                load_3d(dst, map, bar, r.column[c], n, a);
+                if constexpr (EPI != kDenseSwiGLU) load_3d(dst + 128 * r.width[c], map, bar, r.column[c], n + 64, a);
+                dst += r.b_bytes;
               }
-              const AdapterSegment& seg = ad.seg[r.seg(at)];
-              const int col = r.column(ad, at);
-              load_3d(dst + c * r.b_bytes, &seg.b, bar, col, n, a);
-              if constexpr (EPI != kDenseSwiGLU) load_3d(dst + c * r.b_bytes + 128 * seg.width, &seg.b, bar, col, n + 64, a);
             }
-            r.left -= here;
+            done += here;
             next_stage();
           }
         }
@@ -380,6 +406,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       uint32_t phase = 0;
       int it = 0;
       bool ok = true;
+      const std::conditional_t<AD, AdapterRounds<EPI>, NoAdapters> r(ad);
       auto filled = [&]() {
         if (!mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
           if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 2800 + stage);
@@ -425,42 +452,54 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           used();
         }
         if constexpr (AD) {
-          AdapterRounds<EPI> r(ad, count_adapters(id, piece, split));
-          uint32_t off[8] = {};
-          int32_t a = -1;
-          int index = 0, at = r.chunks;
-          while (ok && r.left > 0) {
-            const int v_stage = stage;
-            for (int v0 = 0; ok && v0 < r.chunks; v0 += r.v_slots) {
+          if (ok && !mbar_wait(smem_u32(&bars.listed[it & 1]), (it >> 1) & 1, abort_flag)) {
+            if (lane == 0) report_error(pa.err, ATENIA_ERR_DEVICE_TIMEOUT, 2910 + (it & 1));
+            *abort_flag = 1;
+            ok = false;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          const int found = ok ? lists.count[it & 1] : 0;
+          for (int done = 0; ok && done < found;) {
+            const int v_stage = stage, v_next = stage + 1 == kStages ? 0 : stage + 1;
+            const bool two = r.chunks > r.v_slots;
+            if (!filled()) break;
+            step_stage();  // (given back behind the MMAs that read it)
+            if (two) {
               if (!filled()) break;
-              step_stage();  // (given back behind the MMAs that read it)
+              step_stage();
             }
-            for (int b = 0; ok && b < r.b_stages && r.left > 0; ++b) {
+            uint64_t dv[kMaxChunks];
+#pragma unroll
+            for (int c = 0; c < kMaxChunks; ++c) {
+              const bool over = c >= r.v_slots;
+              dv[c] = make_smem_desc_width(ring + (over ? v_next : v_stage) * kPairStageBytes + (over ? c - r.v_slots : c) * r.v_bytes, r.width[c]);
+            }
+            for (int b = 0; ok && b < r.b_stages && done < found; ++b) {
               if (!filled()) break;
-              const int here = min(r.left, r.b_slots);
-              const uint32_t sb = ring + stage * kPairStageBytes;
-              for (int c = 0; c < here; ++c, ++at) {
-                if (at == r.chunks) {
-                  at = 0;
-                  a = next_adapter_of(id, a, index, piece, split);
-                  lanes_off(off, id, a);
+              const int here = min(found - done, r.group);
+              uint32_t at = ring + stage * kPairStageBytes;
+              for (int q = 0; q < here; ++q) {
+                uint32_t off[8];
+                lanes_off(off, id, (int32_t)lists.adapter[it & 1][done + q]);
+#pragma unroll
+                for (int c = 0; c < kMaxChunks; ++c) {
+                  if (c >= r.chunks) break;
+                  constexpr uint32_t idesc_ad = kPairIdesc | (uint32_t(N_OUT >> 3) << 17);
+                  const uint64_t db = make_smem_desc_width(at, r.width[c]);
+#pragma unroll 1
+                  for (int k = 0; k < r.steps[c]; ++k) mma_lanes(d + (r.second[c] ? N_OUT : 0), dv[c] + 2 * k, db + 2 * k, idesc_ad, off);
+                  at += r.b_bytes;
                 }
-                int v = v_stage + at / r.v_slots;
-                v = v >= kStages ? v - kStages : v;
-                const int seg = r.seg(at), width = ad.seg[seg].width, steps = r.steps(ad, at);
-                constexpr uint32_t idesc_ad = kPairIdesc | (uint32_t(N_OUT >> 3) << 17);
-                const uint64_t da = make_smem_desc_width(ring + v * kPairStageBytes + (at % r.v_slots) * r.v_bytes, width);
-                const uint64_t db = make_smem_desc_width(sb + c * r.b_bytes, width);
-                for (int k = 0; k < steps; ++k) mma_lanes(d + seg * N_OUT, da + 2 * k, db + 2 * k, idesc_ad, off);
               }
-              r.left -= here;
+              done += here;
               used();
             }
-            for (int v0 = 0, v = v_stage; ok && v0 < r.chunks; v0 += r.v_slots) {
-              commit_both(smem_u32(&bars.empty[v]), lead);
-              v = v + 1 == kStages ? 0 : v + 1;
-            }
+            if (!ok) break;
+            commit_both(smem_u32(&bars.empty[v_stage]), lead);
+            if (two) commit_both(smem_u32(&bars.empty[v_next]), lead);
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bars.unlisted[it & 1]));
         }
         if (ok) commit_both(smem_u32(&bars.acc_full[acc]), lead);
       }

@@ -32,6 +32,7 @@ int num_sms_of_current_device(int* out) {
 }
 
 constexpr int64_t kMaxRows = 1 << 24, kMaxWidth = 1 << 20;
+constexpr int kMaxAdapters = ATENIA_ADAPTER_MAX_COUNT;
 
 uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -122,7 +123,7 @@ int check_sizes(int64_t T, int64_t d, int64_t f) {
 
 int check_ffn_adapters(const AteniaFfnAdapters* ad) {
   if (!ad->ids) return ATENIA_ERR_NULL;
-  if (ad->n < 1) return ATENIA_ERR_SHAPE;
+  if (ad->n < 1 || ad->n > kMaxAdapters) return ATENIA_ERR_SHAPE;
   const AteniaLowRank* sets[3] = {&ad->gate, &ad->up, &ad->down};
   for (const AteniaLowRank* a : sets) {
     if (a->rank == 0) continue;
@@ -321,7 +322,7 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   int rc = check_sizes(T, d_in, d_out);
   if (rc) return rc;
   if (!weight || !adapter) return ATENIA_ERR_NULL;
-  if (n < 1) return ATENIA_ERR_SHAPE;
+  if (n < 1 || n > kMaxAdapters) return ATENIA_ERR_SHAPE;
   if ((rc = check_adapter(*adapter))) return rc;
   if (T == 0) return ATENIA_OK;
   if (!x || !ids || !y || !workspace) return ATENIA_ERR_NULL;

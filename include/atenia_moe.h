@@ -441,6 +441,7 @@ ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
  * up to ATENIA_ADAPTER_MAX_RANK (zero-pad A's rows and B's columns otherwise); rank 0 = this projection has none.  The reduced
  * rows scale A x are rounded to bf16.  A token reads its own adapter only: infinities and NaN in another one's do not reach it. */
 #define ATENIA_ADAPTER_MAX_RANK 128
+#define ATENIA_ADAPTER_MAX_COUNT 65536 /* n at most */
 typedef struct AteniaLowRank {
   const void* a;      /* device bf16 [n, rank, in] */
   const void* b;      /* device bf16 [n, out, rank] */

@@ -69,7 +69,7 @@ def test_adapters_of_the_block(lib):
     from ateniaengine_b200 import _lib
     def call(**kw):
         return _forward(lib, adapters=C.byref(_lib.FfnAdapters(**{**dict(gate=_low(), up=_low(), down=_low(), ids=P, n=2), **kw})))
-    assert call(ids=None) == -1 and call(n=0) == -2
+    assert call(ids=None) == -1 and call(n=0) == -2 and call(n=65537) == -2
     for part in ("gate", "up", "down"):
         for rank in (-8, 4, 12, 136):
             assert call(**{part: _low(rank)}) == -2
@@ -79,7 +79,7 @@ def test_adapters_of_the_block(lib):
 
 
 def test_linear(lib):
-    for bad in (dict(T=-1), dict(n_in=8), dict(n_in=72), dict(n_out=40), dict(n=0), dict(low=_low(0)), dict(low=_low(7)),
+    for bad in (dict(T=-1), dict(n_in=8), dict(n_in=72), dict(n_out=40), dict(n=0), dict(n=65537), dict(low=_low(0)), dict(low=_low(7)),
                 dict(low=_low(136)), dict(low=_low(b=P + 8)), dict(x=P + 2), dict(y=P + (1 << 20) + 8), dict(ws=P + 4)):
         assert _linear(lib, **bad) == -2, bad
     for bad in (dict(low=None), dict(w=None), dict(x=None), dict(ids=None), dict(y=None), dict(ws=None), dict(low=_low(a=None)),
