@@ -1,10 +1,15 @@
 // Which kernel a dense product takes, from its sizes alone (host arithmetic).
+//
+// Microseconds of each kernel, fitted to 310 products of five shapes (512 x 1408 to 4096 x 14336), 8 to 4096 tokens and each direction,
+// run one after another on a B200 with their weights out of L2, every kernel at every split.  The kernel chosen is within 0.8 % of
+// the fastest on average and 13 % at most; two rules by tile counts alone were 8 % and 2.2 times off.
+//   a wave   : as many CTAs as are resident at once, given how clusters of a size fit the GPU's parts
+//   a k-block: 0.32 us of a pair's 256 x 256 tile, 0.35 of 128 x 256 (its MMAs wait for shared memory), 0.30 of 128 x 128 alone on
+//              its SM and 0.48 beside another
+//   splits   : what adding the sums through distributed shared memory costs
+//   adapters : 0.1 us of each on a tile of 128 columns (a batch of few rows may have one per row; a tile of a prompt has a few)
 #pragma once
 #include <stdint.h>
-#ifdef DENSE_TUNE
-#include <cstdio>
-#include <cstdlib>
-#endif
 
 namespace atenia {
 
@@ -13,36 +18,67 @@ struct DenseSize {
   int kb;        // k-blocks of 64
 };
 struct DensePlan {
-  bool pairs;    // dense_pair.cu; else tiles of 128 x `columns` (dense_gemm.cu), the reduction cut `split` ways
+  bool pairs;    // dense_pair.cu; else tiles of 128 x `columns` (dense_gemm.cu); the reduction cut `split` ways
   int columns;
   int split;
 };
 
-inline DensePlan dense_plan(const DenseSize* sizes, int problems, bool two_columns, bool full_rows, int num_sms) {
-#ifdef DENSE_TUNE
-  if (const char* e = getenv("DENSE_PLAN")) {
-    int a = 0, c = 128, b = 1;
-    const char* q = e;
-    if (getenv("DENSE_PLAN2") && sizes[0].kb >= atoi(getenv("DENSE_KB"))) q = getenv("DENSE_PLAN2");
-    sscanf(q, "%d,%d,%d", &a, &c, &b);
-    for (int i = 0; i < problems; ++i)
-      while (sizes[i].kb < b) b /= 2;
-    return {a && full_rows, c, b};
-  }
-#endif
-  const int n_out = two_columns ? 128 : 256;
-  int64_t pairs = 0, tiles = 0;
-  int min_kb = 1 << 30;
+inline int64_t dense_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// rows: of A a stage holds (128 = all); two_columns: gate and up of a feature (kDenseSwiGLU); grad: kDenseGateGrad; full_rows: the
+// pair kernel can take the call (its A boxes are 128 rows high); adapters: how many there are (0: none in this product)
+inline DensePlan dense_plan(const DenseSize* sizes, int problems, int rows, bool two_columns, bool grad, bool full_rows, int adapters,
+                            int num_sms) {
+  // CTAs of a cluster of 1 .. 8 that are resident at once on 148 SMs, one or two an SM (cudaOccupancyMaxActiveClusters)
+  static const int kAlone[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+  static const int kTwice[9] = {0, 296, 296, 279, 284, 280, 270, 259, 264};
+  const double scale = num_sms / 148.0;
+  const int wide = two_columns ? 128 : 256;  // result columns of a tile of 256 MMA columns
+  int64_t pairs = 0, tiles256 = 0, tiles128 = 0;
+  int kb = 0, least_kb = 1 << 30;
+  double bytes = 0;
   for (int i = 0; i < problems; ++i) {
-    pairs += (sizes[i].M + 255) / 256 * ((sizes[i].N + n_out - 1) / n_out);
-    tiles += (sizes[i].M + 127) / 128 * ((sizes[i].N + n_out / 2 - 1) / (n_out / 2));
-    if (sizes[i].kb < min_kb) min_kb = sizes[i].kb;
+    const DenseSize& s = sizes[i];
+    pairs += dense_ceil(s.M, 256) * dense_ceil(s.N, wide);
+    tiles256 += dense_ceil(s.M, 128) * dense_ceil(s.N, wide);
+    tiles128 += dense_ceil(s.M, 128) * dense_ceil(s.N, wide / 2);
+    kb = s.kb > kb ? s.kb : kb;
+    least_kb = s.kb < least_kb ? s.kb : least_kb;
+    bytes += 128.0 * s.kb * (s.M + (two_columns ? 2 : 1) * s.N) + (grad ? 14.0 : 2.0) * s.M * s.N;
   }
-  if (full_rows && pairs >= num_sms / 2) return {true, 0, 1};
-  // clusters until every SM has a CTA, each with four k-blocks at least
-  int split = 1;
-  while (split < 8 && tiles * split < num_sms && min_kb >= 8 * split) split *= 2;
-  return {false, 128, split};
+  const int most = sizes[0].M > 128 ? 8 : (int)sizes[0].M;
+  const double extra = 0.1 * (adapters < most ? adapters : most);
+  const double floor = 4.5 + bytes / 5.35e6, f = rows / 128.0;
+  DensePlan best{false, 128, 1};
+  double best_us = 1e30;
+  auto offer = [&](bool p, int columns, int split, double us) {
+    us = (us > floor ? us : floor) + (adapters ? 0.5 : 0.05) * us;  // (of two that the bytes bound, the one with less to do)
+    if (us < best_us) {
+      best_us = us;
+      best = {p, columns, split};
+    }
+  };
+  static const int kSplits[6] = {1, 2, 3, 4, 6, 8};
+  for (int s : kSplits) {
+    if (s > least_kb) break;
+    const double kc = (double)dense_ceil(kb, s);
+    const bool cut = s > 1;
+    if (full_rows && s <= 4) {
+      const double w = (double)dense_ceil(pairs * s, (int64_t)(kAlone[2 * s] * scale) / 2);
+      offer(true, 256, s, 3.2 + w * (0.322 * kc + 1.6 + (cut ? 3.9 : 0.0) + (grad ? 5.5 : 0.0) + 2.5 * extra / s));
+    }
+    {
+      const double w = (double)dense_ceil(tiles256 * s, (int64_t)(kAlone[s] * scale));
+      offer(false, 256, s, -0.4 + w * (0.348 * kc * (0.84 + 0.16 * f) + 5.4 + (cut ? 4.9 * f + 0.2 * s : grad ? 12.6 : 0.0) + 2.0 * extra / s));
+    }
+    {
+      const int64_t n = tiles128 * s, room = (int64_t)(kTwice[s] * scale), w = dense_ceil(n, room);
+      const double last = n - (w - 1) * room <= (int64_t)(kAlone[s] * scale) ? 0.30 : 0.477;
+      offer(false, 128, s, -0.1 + kc * (0.72 + 0.28 * f) * ((w - 1) * 0.477 + last) + w * (3.6 + (grad && !cut ? 8.7 : 0.0) + extra / s) +
+                               (cut ? w * 4.7 * f - 0.8 + 0.2 * s : 0.0));
+    }
+  }
+  return best;
 }
 
 }  // namespace atenia

@@ -418,7 +418,7 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
     ta.v_bytes = (chunks * rows * width * 2 + 1023) / 1024 * 1024;
   }
   int ring = TileSize<BN>::kRing - ta.v_bytes;
-  if (ring < 3 * stage_bytes) ring = TileSize<256>::kRing - ta.v_bytes;  // (many reduced rows: one CTA per SM)
+  if (ring < 2 * stage_bytes) ring = TileSize<256>::kRing - ta.v_bytes;  // (many reduced rows: one CTA per SM)
   ta.stages = ring / stage_bytes;
   if (ta.stages > kTileStages) ta.stages = kTileStages;
   ring = ta.stages * stage_bytes;
@@ -492,7 +492,9 @@ int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   if (dense_gemv_serves(g)) return launch_dense_gemv(g, num_sms, s);
   DenseSize sizes[kMaxDenseProblems];
   for (int i = 0; i < g.problems; ++i) sizes[i] = {g.p[i].M, g.p[i].N, g.p[i].kb};
-  const DensePlan plan = dense_plan(sizes, g.problems, g.epilogue == kDenseSwiGLU, g.a_rows == BM, num_sms);
+  const DensePlan plan =
+      dense_plan(sizes, g.problems, g.a_rows, g.epilogue == kDenseSwiGLU, g.epilogue == kDenseGateGrad, g.a_rows == BM,
+                 g.adapters ? g.adapters->n : 0, num_sms);
   if (plan.pairs) return launch_dense_pairs(g, plan.split, num_sms, s);
   return launch_dense_tiles(g, plan.columns, plan.split, s);
 }

@@ -223,6 +223,8 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   if (!rc && ad2) {
     rc = plan_adapters(&second, {&adapters->down, nullptr}, adapters->ids, adapters->n, h, T, F, d, &ws, true);
     g2.adapters = &second.add;
+    // (h too: the kernel before is the reduction, whose CTAs let this one start when the one that wrote h had completed)
+    g2.a_early = true;
   }
   if (!rc && ad1) rc = launch_adapter_reduce(first.red, sms, s);
   if (!rc) rc = launch_dense_gemm(g1, sms, s);
