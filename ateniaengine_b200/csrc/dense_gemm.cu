@@ -27,7 +27,7 @@ struct TileSize {
   static constexpr int kBBytes = BN * BK * 2;
   static constexpr int kRing = BN == 128 ? 108 * 1024 : 196 * 1024;  // two CTAs per SM, or one
 };
-constexpr int kTileSmemMax = 225 * 1024;
+constexpr int kTileSmemMax = 200 * 1024;
 
 struct __align__(8) TileBars {
   uint64_t full[kTileStages];
@@ -53,13 +53,17 @@ struct Problems {
 
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 4) << 24);
 
+struct TileMasks : TileList {
+  int4 off[BM];  // of the listed adapters: bit set where a row has another one
+};
+
 template <int EPI, bool B_MN, int NP, bool AD, int BN>
 __global__ void __launch_bounds__(TileSize<BN>::kThreads)
 dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant__ TileArgs ta,
                   const __grid_constant__ std::conditional_t<AD, DenseAdapters, NoAdapters> ad) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ TileBars bars;
-  __shared__ std::conditional_t<AD, TileList, NoAdapters> list;
+  __shared__ std::conditional_t<AD, TileMasks, NoAdapters> list;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
   const uint32_t v_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;  // reduced rows, then the ring
   const uint32_t ring = v_smem + (AD ? ta.v_bytes : 0);
@@ -81,6 +85,10 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const int m0 = (tile - nt * m_tiles) * BM, n0 = nt * N_OUT;
   const int rows = min(BM, p.M - m0), cols = min(N_OUT, p.N - n0);
   const int kb_begin = (int)((int64_t)p.kb * rank / split), kb_end = (int)((int64_t)p.kb * (rank + 1) / split);
+  // The adapters' steps come before the last quarter of a long k range: their reduced rows are there by then, and the weights go on
+  // arriving while their short MMAs are issued (48 tokens with 32 adapters, gate and up of 4096 x 14336: 2.5 us of 78).  Behind a short one,
+  // which would wait for the rows half done (64 tokens beside 4096 x 4096, eight k-blocks a CTA: 17.4 / 19.7 us).
+  const int kb_adapters = kb_end - kb_begin < 24 ? kb_end : kb_begin + (kb_end - kb_begin) * 3 / 4;
   const int stages = ta.stages;
   constexpr bool A_MN = NP > 1;
   const int a_bytes = ta.a_rows * BK * 2;
@@ -159,7 +167,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     };
     int ahead = 0;
     if (ta.b_early) {
-      ahead = min(kb_end - kb_begin, stages);
+      ahead = min((AD ? kb_adapters : kb_end) - kb_begin, stages);
       for (int i = 0; i < ahead; ++i) {
         const uint32_t bar = smem_u32(&bars.full[i]), dst = ring + i * stage_bytes;
         mbar_expect_tx_one(bar, stage_bytes);
@@ -168,18 +176,21 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       }
     }
     if (!ta.a_early) chain_wait();
-    for (int kb = kb_begin; kb < kb_end; ++kb) {
-      const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
-      if (kb - kb_begin < ahead) {
-        if (!ta.a_early) load_a(kb, dst, bar);
-      } else {
-        if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2100 + stage))) break;
-        mbar_expect_tx_one(bar, stage_bytes);
-        load_b(kb, dst + a_bytes, bar);
-        load_a(kb, dst, bar);
+    auto load_blocks = [&](int from, int to) {
+      for (int kb = from; kb < to; ++kb) {
+        const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
+        if (kb - kb_begin < ahead) {
+          if (!ta.a_early) load_a(kb, dst, bar);
+        } else {
+          if (!(ok = wait_all(&bars.empty[stage], phase ^ 1u, 2100 + stage))) break;
+          mbar_expect_tx_one(bar, stage_bytes);
+          load_b(kb, dst + a_bytes, bar);
+          load_a(kb, dst, bar);
+        }
+        next_stage();
       }
-      next_stage();
-    }
+    };
+    load_blocks(kb_begin, AD ? kb_adapters : kb_end);
     if constexpr (AD) {
       // (B is not written by the kernel before; the reduced rows, which are, come with another warp)
       ok = ok && wait_all(&bars.listed, 0, 2110);
@@ -223,6 +234,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         }
         left -= here;
       }
+      if (ok) load_blocks(kb_adapters, kb_end);
     }
     chain_wait();
     chain_next();  // (every load is on its way: what follows may be launched)
@@ -252,15 +264,18 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       }
     };
     constexpr uint32_t idesc = kIdesc | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(BN >> 3) << 17);
-    for (int kb = kb_begin; kb < kb_end; ++kb) {
-      if (!filled()) break;
-      const uint32_t sa = ring + stage * stage_bytes;
-      const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sa + a_bytes);
+    auto multiply_blocks = [&](int from, int to) {
+      for (int kb = from; kb < to; ++kb) {
+        if (!filled()) break;
+        const uint32_t sa = ring + stage * stage_bytes;
+        const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sa + a_bytes);
 #pragma unroll
-      for (int k = 0; k < BK / UMMA_K; ++k)
-        tc_mma_bf16_one(tmem, da + k * kOperandStep<A_MN>, db + k * kOperandStep<B_MN>, idesc, kb > kb_begin || k > 0);
-      used();
-    }
+        for (int k = 0; k < BK / UMMA_K; ++k)
+          tc_mma_bf16_one(tmem, da + k * kOperandStep<A_MN>, db + k * kOperandStep<B_MN>, idesc, kb > kb_begin || k > 0);
+        used();
+      }
+    };
+    multiply_blocks(kb_begin, AD ? kb_adapters : kb_end);
     if constexpr (AD) {
       ok = ok && wait_all(&bars.listed, 0, 2210);
       const int count = ok ? list.count : 0;
@@ -270,9 +285,6 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
       uint64_t dv[kMaxChunks];
 #pragma unroll
       for (int c = 0; c < kMaxChunks; ++c) dv[c] = make_smem_desc_width(v_smem + c * v_bytes, ac.width[c]);
-      int32_t id[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) id[w] = ok ? list.id[32 * w + lane] : kNoAdapter;
       auto add_chunk = [&](int c, uint32_t at) {
         constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
         const uint64_t db = make_smem_desc_width(at, ac.width[c]);
@@ -285,7 +297,8 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (group > 0 && !filled()) break;
         uint32_t at = ring + stage * stage_bytes;
         for (int s = 0; s < here; ++s, i += split) {
-          lanes_off(off, id, list.adapter[i]);
+          const int4 m = list.off[i];
+          off[0] = m.x, off[1] = m.y, off[2] = m.z, off[3] = m.w;
 #pragma unroll
           for (int c = 0; c < kMaxChunks; ++c) {
             if (c >= ac.chunks) break;
@@ -301,6 +314,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (group > 0) used();
         left -= here;
       }
+      if (ok) multiply_blocks(kb_adapters, kb_end);
     }
     if (ok) tc_commit_one(smem_u32(&bars.acc_full));
   } else {
@@ -308,6 +322,12 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if constexpr (AD) {
       if (warp < 6) {
         list_adapters(list, ad.ids, m0, rows, ad.n, warp - 2, lane);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int32_t mine = list.id[32 * (warp - 2) + lane];
+        for (int i = 0; i < list.count; ++i) {
+          const uint32_t off = __ballot_sync(0xffffffffu, mine != list.adapter[i]);
+          if (lane == 0) reinterpret_cast<uint32_t*>(&list.off[i])[warp - 2] = off;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars.listed));
       }
