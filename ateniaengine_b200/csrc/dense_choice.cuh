@@ -6,6 +6,7 @@
 //   a wave   : as many CTAs as are resident at once, given how clusters of a size fit the GPU's parts
 //   a k-block: 0.32 us of a pair's 256 x 256 tile, 0.35 of 128 x 256 (its MMAs wait for shared memory), 0.30 of 128 x 128 alone on
 //              its SM and 0.48 beside another
+//   tail     : 2 us for a launch of its own
 //   splits   : what adding the sums through distributed shared memory costs
 //   adapters : 0.1 us of each on a tile of 128 columns (a batch of few rows may have one per row; a tile of a prompt has a few)
 #pragma once
@@ -21,6 +22,7 @@ struct DensePlan {
   bool pairs;    // dense_pair.cu; else tiles of 128 x `columns` (dense_gemm.cu); the reduction cut `split` ways
   int columns;
   int split;
+  int tail_split;  // pairs: of the tiles behind the last whole wave
 };
 
 inline int64_t dense_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -49,13 +51,13 @@ inline DensePlan dense_plan(const DenseSize* sizes, int problems, int rows, bool
   const int most = sizes[0].M > 128 ? 8 : (int)sizes[0].M;
   const double extra = 0.1 * (adapters < most ? adapters : most);
   const double floor = 4.5 + bytes / 5.35e6, f = rows / 128.0;
-  DensePlan best{false, 128, 1};
+  DensePlan best{false, 128, 1, 1};
   double best_us = 1e30;
-  auto offer = [&](bool p, int columns, int split, double us) {
+  auto offer = [&](bool p, int columns, int split, double us, int tail = 1) {
     us = (us > floor ? us : floor) + (adapters ? 0.5 : 0.05) * us;  // (of two that the bytes bound, the one with less to do)
     if (us < best_us) {
       best_us = us;
-      best = {p, columns, split};
+      best = {p, columns, split, tail};
     }
   };
   static const int kSplits[6] = {1, 2, 3, 4, 6, 8};
@@ -65,7 +67,14 @@ inline DensePlan dense_plan(const DenseSize* sizes, int problems, int rows, bool
     const bool cut = s > 1;
     if (full_rows && s <= 4) {
       const double w = (double)dense_ceil(pairs * s, (int64_t)(kAlone[2 * s] * scale) / 2);
-      offer(true, 256, s, 3.2 + w * (0.322 * kc + 1.6 + (cut ? 3.9 : 0.0) + (grad ? 5.5 : 0.0) + 2.5 * extra / s));
+      const double wave = 0.322 * kc + 1.6 + (cut ? 3.9 : 0.0) + (grad ? 5.5 : 0.0) + 2.5 * extra / s;
+      offer(true, 256, s, 3.2 + w * wave);
+      const int64_t room = (int64_t)(kAlone[2] * scale) / 2, whole = pairs / room, rest = pairs - whole * room;
+      if (cut && whole > 0 && rest > 0) {
+        const double full = 0.322 * kb + 1.6 + (grad ? 5.5 : 0.0) + 2.5 * extra;
+        const double tail = (double)dense_ceil(rest * s, (int64_t)(kAlone[2 * s] * scale) / 2);
+        offer(true, 256, 1, 5.2 + whole * full + tail * wave, s);
+      }
     }
     {
       const double w = (double)dense_ceil(tiles256 * s, (int64_t)(kAlone[s] * scale));

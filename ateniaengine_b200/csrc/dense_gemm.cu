@@ -515,7 +515,7 @@ int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
   const DensePlan plan =
       dense_plan(sizes, g.problems, g.a_rows, g.epilogue == kDenseSwiGLU, g.epilogue == kDenseGateGrad, g.a_rows == BM,
                  g.adapters ? g.adapters->n : 0, num_sms);
-  if (plan.pairs) return launch_dense_pairs(g, plan.split, num_sms, s);
+  if (plan.pairs) return launch_dense_pairs(g, plan.split, plan.tail_split, num_sms, s);
   return launch_dense_tiles(g, plan.columns, plan.split, s);
 }
 

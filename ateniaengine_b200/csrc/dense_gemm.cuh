@@ -65,7 +65,7 @@ struct DenseGemm {
 };
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between the two
 int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s);  // dense_gemm.cu
-int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t s);  // dense_pair.cu
+int launch_dense_pairs(const DenseGemm& g, int split, int tail_split, int num_sms, cudaStream_t s);  // dense_pair.cu
 int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_gemv.cu, where it serves the product
 bool dense_gemv_serves(const DenseGemm& g);
 // Two tokens over a large matrix: the tensor-core kernel (dense_gemv.cu has the times).

@@ -6,8 +6,9 @@
 // reads and writes 192 bytes a cycle at full rate, a pair 128).  Persistent: one CTA per SM, two accumulators in tensor memory, so that the epilogue of a tile runs under the MMAs of the next.
 //   k-block : 64; a stage is 16 KiB of A and 16 KiB of B per CTA, six stages
 //   order   : bands of kBand row tiles, column tile by column tile, so that the 74 tiles at work at one time share few operand rows in L2
-//   split   : where the tiles are too few, the pairs of a cluster (two, three or four) share a tile: consecutive k ranges, added through
-//             distributed shared memory in rank order
+//   split   : where the tiles are too few, or the last wave's are, the pairs of a cluster (two, three or four) share a tile: consecutive k
+//             ranges, added through distributed shared memory in rank order.  (The last wave is a launch of its own then: 5000 tokens of
+//             2048 x 5632 have two whole waves of tiles and twelve tiles in the second product.)
 //   epilogue: eight warps; a lane holds a row, so the results go through shared memory to TMA, which writes whole lines (32 bytes a
 //             lane were 32 lines an access, and a tile's 5400 cycles of them hid only behind a reduction of 700 and more)
 //
@@ -57,7 +58,7 @@ struct __align__(8) PairBars {
   int abort_flag;
 };
 struct PairArgs {
-  int problems, tiles, split, b_early, a_early;
+  int problems, first, tiles, split, b_early, a_early;  // tiles first .. tiles - 1
   int tile_end[kMaxDenseProblems];
   DeviceError* err;
 };
@@ -209,7 +210,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   const bool leader = rank == 0;
   // split 1: a pair walks the tiles; else the `split` pairs of a cluster share one tile's reduction
   const int split = pa.split;
-  const int pair = split > 1 ? (int)(blockIdx.x >> 1) / split : (int)(blockIdx.x >> 1);
+  const int pair = pa.first + (split > 1 ? (int)(blockIdx.x >> 1) / split : (int)(blockIdx.x >> 1));
   const int num_pairs = split > 1 ? pa.tiles : (int)(gridDim.x >> 1);
   const int piece = split > 1 ? (int)(in_cluster >> 1) : 0;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? kPairN / 2 : kPairN;
@@ -623,7 +624,8 @@ int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream
   for (int i = 0; i < NP; ++i) ps.p[i] = g.p[i];
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
   if constexpr (AD) ad = *g.adapters;
-  const int pairs = pa.split > 1 ? pa.tiles * pa.split : num_sms / 2 < pa.tiles ? num_sms / 2 : pa.tiles;
+  const int tiles = pa.tiles - pa.first;
+  const int pairs = pa.split > 1 ? tiles * pa.split : num_sms / 2 < tiles ? num_sms / 2 : tiles;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2 * pa.split;
@@ -652,28 +654,7 @@ int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream
   return (int)e;
 }
 
-}  // namespace
-
-int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t s) {
-  if (split < 1 || split > 4) return ATENIA_ERR_SHAPE;
-  PairArgs pa{};
-  int rc = dense_error_word(&pa.err);
-  if (rc) return rc;
-  const int n_out = g.epilogue == kDenseSwiGLU ? kPairN / 2 : kPairN;
-  int64_t tiles = 0;
-  for (int i = 0; i < g.problems; ++i) {
-    const DenseProblem& p = g.p[i];
-    tiles += (int64_t)((p.M + kPairM - 1) / kPairM) * ((p.N + n_out - 1) / n_out);
-    if (tiles > (1 << 26) || p.kb < split) return ATENIA_ERR_SHAPE;
-    pa.tile_end[i] = (int)tiles;
-  }
-  if (tiles == 0) return ATENIA_OK;
-  if (g.a_rows != BM) return ATENIA_ERR_SHAPE;
-  pa.problems = g.problems;
-  pa.tiles = (int)tiles;
-  pa.split = split;
-  pa.b_early = g.b_early;
-  pa.a_early = g.a_early && g.b_early;
+int launch_range(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream_t s) {
   count_launch();
   count_tcgen05_launch();
   const bool ad = g.adapters != nullptr;
@@ -689,6 +670,43 @@ int launch_dense_pairs(const DenseGemm& g, int split, int num_sms, cudaStream_t 
                   : launch_pairs<kDensePlain, false, 1, false>(g, pa, num_sms, s);
   if (g.epilogue == kDenseGateGrad && b_mn && !ad) return launch_pairs<kDenseGateGrad, true, 1, false>(g, pa, num_sms, s);
   return ATENIA_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+int launch_dense_pairs(const DenseGemm& g, int split, int tail_split, int num_sms, cudaStream_t s) {
+  if (split < 1 || split > 4 || tail_split < 1 || tail_split > 4) return ATENIA_ERR_SHAPE;
+  PairArgs pa{};
+  int rc = dense_error_word(&pa.err);
+  if (rc) return rc;
+  const int n_out = g.epilogue == kDenseSwiGLU ? kPairN / 2 : kPairN;
+  int64_t tiles = 0;
+  for (int i = 0; i < g.problems; ++i) {
+    const DenseProblem& p = g.p[i];
+    tiles += (int64_t)((p.M + kPairM - 1) / kPairM) * ((p.N + n_out - 1) / n_out);
+    if (tiles > (1 << 26) || p.kb < split || p.kb < tail_split) return ATENIA_ERR_SHAPE;
+    pa.tile_end[i] = (int)tiles;
+  }
+  if (tiles == 0) return ATENIA_OK;
+  if (g.a_rows != BM) return ATENIA_ERR_SHAPE;
+  pa.problems = g.problems;
+  pa.tiles = (int)tiles;
+  pa.split = split;
+  pa.b_early = g.b_early;
+  pa.a_early = g.a_early && g.b_early;
+  const int waves = (int)tiles / (num_sms / 2);
+  if (split > 1 || tail_split == 1 || waves == 0 || waves * (num_sms / 2) == tiles) return launch_range(g, pa, num_sms, s);
+  // the tiles of whole waves, then the rest with their reductions cut.  The second launch's operands are the first's, so they were there
+  // when the first let it start; its epilogues wait for the first, so what comes behind it waits for both.
+  pa.tiles = waves * (num_sms / 2);
+  if ((rc = launch_range(g, pa, num_sms, s))) return rc;
+  DenseGemm tail = g;
+  tail.chained = true;
+  pa.first = pa.tiles;
+  pa.tiles = (int)tiles;
+  pa.split = tail_split;
+  pa.b_early = pa.a_early = true;
+  return launch_range(tail, pa, num_sms, s);
 }
 
 }  // namespace atenia
