@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["one", "none", "distinct", "runs", "odd"])
 @pytest.mark.parametrize("T,d,out,n,r", [(1, 16, 16, 1, 8), (1, 512, 1408, 4, 16), (5, 272, 144, 3, 24), (33, 64, 272, 40, 8),
                                          (64, 1040, 528, 70, 16), (129, 144, 400, 150, 64), (130, 272, 2064, 9, 128),
-                                         (300, 528, 144, 200, 16), (1021, 1040, 1040, 12, 40), (2100, 512, 1552, 30, 64)])
+                                         (300, 528, 144, 200, 16), (1021, 1040, 1040, 12, 40), (2100, 512, 1552, 30, 64), (2100, 272, 5632, 300, 16), (1500, 144, 5008, 40, 128)])
 def test_linear(T, d, out, n, r, kind):
     from ateniaengine_b200 import adapter_linear
     x, w, low, ids = ref.rand(T, 1.0, T, d), ref.rand(1, d ** -0.5, out, d), ref.low_rank(5, n, r, d, out), ref.ids_of(kind, T, n)
@@ -23,7 +23,9 @@ def test_linear(T, d, out, n, r, kind):
 
 @pytest.mark.parametrize("parts", ["gate,up,down", "gate", "up", "down", "gate,down"])
 @pytest.mark.parametrize("T,d,F,n,ranks,kind", [(1, 64, 96, 2, (8, 16, 24), "one"), (48, 512, 1408, 33, (16, 16, 16), "distinct"),
-                                                (200, 272, 400, 7, (8, 64, 40), "odd"), (1100, 528, 1040, 16, (32, 32, 128), "runs")])
+                                                (200, 272, 400, 7, (8, 64, 40), "odd"), (1100, 528, 1040, 16, (32, 32, 128), "runs"),
+                                                (1500, 272, 3600, 40, (128, 128, 16), "distinct"), (700, 512, 5632, 50, (96, 40, 64), "odd"),
+                                                (1100, 2048, 5632, 16, (24, 8, 32), "runs")])
 def test_block(T, d, F, n, ranks, kind, parts):
     from ateniaengine_b200 import gated_ffn
     x, w, ids = ref.rand(T, 1.0, T, d), ref.block(3, d, F), ref.ids_of(kind, T, n)

@@ -8,7 +8,9 @@ pytestmark = pytest.mark.gpu
 
 SIZES = [(1, 16, 16), (1, 512, 1408), (2, 48, 80), (7, 272, 144), (8, 64, 64), (9, 64, 128), (64, 512, 1408), (100, 16, 2064),
          (127, 1040, 48), (128, 272, 144), (129, 272, 144), (255, 144, 272), (257, 512, 400), (700, 1040, 1424), (1021, 528, 1040),
-         (2100, 768, 1552)]
+         (2100, 768, 1552),
+         # reductions cut over clusters of single CTAs and of pairs, and behind the last whole wave (tests/test_dense_choice.py)
+         (300, 2064, 8208), (1021, 2048, 5632), (2600, 2064, 4112)]
 
 
 @pytest.mark.parametrize("T,d,F", SIZES)
