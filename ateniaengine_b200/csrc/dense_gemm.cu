@@ -289,8 +289,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         constexpr uint32_t idesc_ad = kIdesc | (uint32_t(N_OUT >> 3) << 17);
         const uint64_t db = make_smem_desc_width(at, ac.width[c]);
         const uint32_t d = tmem + (ac.second[c] ? N_OUT : 0);
-#pragma unroll 1
-        for (int k = 0; k < ac.steps[c]; ++k) tc_mma_bf16_lanes_one(d, dv[c] + 2 * k, db + 2 * k, idesc_ad, off);
+        tc_mma_bf16_lanes_one(d, dv[c], db, idesc_ad, ac.steps[c], off);
       };
       for (int i = rank; ok && left > 0;) {
         const int here = group > 0 ? min(left, group) : 1;

@@ -168,15 +168,23 @@ __device__ __forceinline__ void tma_load_3d_one(uint32_t dst, const CUtensorMap*
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-// An accumulating MMA that leaves the lanes whose bit is set in `off` as they are.
-__device__ __forceinline__ void tc_mma_bf16_lanes_one(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+// One to four accumulating MMAs (K = 16 each, 32 bytes apart inside the rows) that leave the lanes whose bit is set in `off` as they are.
+// In one block: the masks go to the registers of the instruction once.
+__device__ __forceinline__ void tc_mma_bf16_lanes_one(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, int steps,
                                                       const uint32_t (&off)[4]) {
   asm volatile(
-      "{\n\t.reg .pred e, t;\n\t"
+      "{\n\t.reg .pred e, t, p;\n\t"
+      ".reg .b64 a, b;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.eq.b32 t, 0, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, t;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, t;\n\t"
+      "setp.gt.and.s32 p, %8, 1, e;\n\tadd.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, {%4, %5, %6, %7}, t;\n\t"
+      "setp.gt.and.s32 p, %8, 2, e;\n\tadd.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, {%4, %5, %6, %7}, t;\n\t"
+      "setp.gt.and.s32 p, %8, 3, e;\n\tadd.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, {%4, %5, %6, %7}, t;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(steps)
       : "memory");
 }
 __device__ __forceinline__ void tc_ld8(uint32_t taddr, uint32_t (&v)[8]) {

@@ -117,14 +117,23 @@ __device__ __forceinline__ void mma_kblock(uint32_t d_tmem, uint64_t a_desc, uin
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
       : "memory");
 }
-__device__ __forceinline__ void mma_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, const uint32_t (&off)[8]) {
+// (see tc_mma_bf16_lanes_one)
+__device__ __forceinline__ void mma_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, int steps,
+                                          const uint32_t (&off)[8]) {
   asm volatile(
-      "{\n\t.reg .pred e, t;\n\t"
+      "{\n\t.reg .pred e, t, p;\n\t"
+      ".reg .b64 a, b;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.eq.b32 t, 0, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, t;\n\t}"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, t;\n\t"
+      "setp.gt.and.s32 p, %12, 1, e;\n\tadd.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+      "@p tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, t;\n\t"
+      "setp.gt.and.s32 p, %12, 2, e;\n\tadd.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+      "@p tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, t;\n\t"
+      "setp.gt.and.s32 p, %12, 3, e;\n\tadd.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+      "@p tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, t;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
-        "r"(off[5]), "r"(off[6]), "r"(off[7])
+        "r"(off[5]), "r"(off[6]), "r"(off[7]), "r"(steps)
       : "memory");
 }
 __device__ __forceinline__ void commit_both(uint32_t bar, uint32_t lead) {
@@ -487,8 +496,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
                   if (c >= r.chunks) break;
                   constexpr uint32_t idesc_ad = kPairIdesc | (uint32_t(N_OUT >> 3) << 17);
                   const uint64_t db = make_smem_desc_width(at, r.width[c]);
-#pragma unroll 1
-                  for (int k = 0; k < r.steps[c]; ++k) mma_lanes(d + (r.second[c] ? N_OUT : 0), dv[c] + 2 * k, db + 2 * k, idesc_ad, off);
+                  mma_lanes(d + (r.second[c] ? N_OUT : 0), dv[c], db, idesc_ad, r.steps[c], off);
                   at += r.b_bytes;
                 }
               }
