@@ -90,4 +90,23 @@ inline DensePlan dense_plan(const DenseSize* sizes, int problems, int rows, bool
   return best;
 }
 
+// dense_rows.cu: row groups, each cut in 1, 2, 4 or 8 pieces of the reduction (of two steps at least), `warps` of them to a block; the
+// cut that leaves the fewest of the `places` for blocks empty in the last wave, the least one of equals.
+struct RowsPlan {
+  int pieces, blocks;
+};
+inline RowsPlan rows_plan(int groups, int steps, int warps, int places) {
+  RowsPlan best{1, (int)dense_ceil(groups, warps)};
+  double best_used = 0;
+  for (int pieces = 1; pieces <= warps && (pieces == 1 || steps >= 2 * pieces); pieces *= 2) {
+    const int64_t blocks = dense_ceil(groups, warps / pieces);
+    const double used = (double)blocks / (double)(dense_ceil(blocks, places) * places);
+    if (used > 1.01 * best_used) {
+      best_used = used;
+      best = {pieces, (int)blocks};
+    }
+  }
+  return best;
+}
+
 }  // namespace atenia

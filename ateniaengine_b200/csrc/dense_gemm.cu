@@ -508,7 +508,7 @@ int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t 
 }
 
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s) {
-  if (dense_gemv_serves(g)) return launch_dense_gemv(g, num_sms, s);
+  if (dense_rows_serve(g)) return launch_dense_rows(g, num_sms, s);
   DenseSize sizes[kMaxDenseProblems];
   for (int i = 0; i < g.problems; ++i) sizes[i] = {g.p[i].M, g.p[i].N, g.p[i].kb};
   const DensePlan plan =

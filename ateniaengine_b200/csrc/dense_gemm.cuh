@@ -27,7 +27,7 @@ struct DenseProblem {
   __nv_bfloat16* out;      // [M, N]
   float* gate;             // kDenseSwiGLU: g and u to be saved, or null; kDenseGateGrad: the saved ones
   float* up;
-  const __nv_bfloat16* a_ptr;     // the same operands for the kernels that read them plainly (dense_gemv.cu)
+  const __nv_bfloat16* a_ptr;     // the same operands for the kernels that read them plainly (dense_rows.cu)
   const __nv_bfloat16* b_ptr[2];
   int K;
   __nv_bfloat16* out_du;   // kDenseGateGrad: du and h [M, N] (dg is `out`)
@@ -66,11 +66,16 @@ struct DenseGemm {
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between the two
 int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s);  // dense_gemm.cu
 int launch_dense_pairs(const DenseGemm& g, int split, int tail_split, int num_sms, cudaStream_t s);  // dense_pair.cu
-int launch_dense_gemv(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_gemv.cu, where it serves the product
-bool dense_gemv_serves(const DenseGemm& g);
-// Two tokens over a large matrix: the tensor-core kernel (dense_gemv.cu has the times).
-constexpr int64_t kGemvTwoElements = (int64_t)1 << 25;
-inline bool dense_gemv_rows(int64_t M, int64_t N, int64_t K) { return M == 1 || (M == 2 && N * K <= kGemvTwoElements); }
+int launch_dense_rows(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_rows.cu, where it serves the product
+bool dense_rows_serve(const DenseGemm& g);
+// Up to 8 rows of a matrix of at most 2^25 elements and up to 16 of one of at most 2^23; one row of any.  Operands on 32-byte boundaries, which the
+// kernel's loads want (any row of a matrix is on one if the first is).  B200, block of 16 tokens, this kernel / dense_gemm.cu's, us: 512 x 1408
+// 5.2 / 8.0, 2048 x 2816 12.5 / 14.8, 2048 x 5632 22.4 / 20.5; of eight 4.6 / 7.8, 10.7 / 14.5, 17.5 / 20.0, 4096 x 14336 65.7 / 61.8; of one
+// 61.0 / 61.8.
+inline bool dense_rows(int64_t M, int64_t N, int64_t K, bool two, const void* x, const void* w0, const void* w1) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w0) | (two ? reinterpret_cast<uintptr_t>(w1) : 0);
+  return (at & 31) == 0 && M <= 16 && (M == 1 || N * K <= (M <= 8 ? (int64_t)1 << 25 : (int64_t)1 << 23));
+}
 
 // Rows of a K-major A box: all of a small batch, so that a call of few tokens moves few token rows.
 inline int dense_a_rows(int64_t rows) { return rows >= 128 ? 128 : (int)((rows + 7) / 8 * 8); }
@@ -93,7 +98,7 @@ struct AdapterReduce {
   bool chained;
 };
 int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s);
-int launch_adapter_gemv(const AdapterReduce& r, cudaStream_t s);  // dense_gemv.cu, for few tokens
+int launch_adapter_gemv(const AdapterReduce& r, cudaStream_t s);  // dense_rows.cu, for few tokens
 // It reads an adapter once per token: up to this many tokens, and elements of A over all of them.
 inline bool adapter_gemv_rows(int64_t M, int64_t rank, int64_t K) { return M <= 128 && M * rank * K <= (int64_t)16 << 20; }
 constexpr int kAdapterMaxRank = 128;

@@ -47,13 +47,18 @@ int matrix_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
   return encode_tmap_bf16(m, base, {(uint64_t)cols, (uint64_t)rows, 0}, {64, (uint32_t)box_rows, 1}, 128);
 }
 
+// Does dense_rows.cu serve the product?  Its kernel reads through plain pointers and needs no maps.
+bool reads_plainly(const DenseProblem& p, const void* a, const void* b0, const void* b1) {
+  return dense_rows(p.M, p.N, p.K, b1 != nullptr, a, b0, b1);
+}
+
 // A [M, K] and B [N, K] of a product without transposed operands: their maps and plain pointers
 int set_operands(DenseProblem* p, const void* a, const void* b0, const void* b1, int a_rows) {
   p->a_ptr = static_cast<const __nv_bfloat16*>(a);
   p->b_ptr[0] = static_cast<const __nv_bfloat16*>(b0);
   p->b_ptr[1] = static_cast<const __nv_bfloat16*>(b1);
   p->kb = p->kb0 = kblocks(p->K);
-  if (dense_gemv_rows(p->M, p->N, p->K)) return ATENIA_OK;
+  if (reads_plainly(*p, a, b0, b1)) return ATENIA_OK;
   int rc = matrix_map(&p->a[0], a, p->M, p->K, a_rows);
   if (!rc) rc = matrix_map(&p->b[0], b0, p->N, p->K, 64);
   if (!rc && b1) rc = matrix_map(&p->b[1], b1, p->N, p->K, 64);
@@ -71,14 +76,13 @@ uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64
 
 // One projection's adapters: the first half's projection and the second half's segment, with v at `v`.
 int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, bool few_reduce,
-                   void* v, AdapterReduce::Projection* red, AdapterSegment* seg) {
+                   bool plain, void* v, AdapterReduce::Projection* red, AdapterSegment* seg) {
   const uint64_t r = (uint64_t)a.rank;
-  const bool few = dense_gemv_rows(T, out, in);  // (the kernels for one or two tokens read through plain pointers)
   int rc = few_reduce ? ATENIA_OK : encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
   const uint32_t width = (uint32_t)adapter_width(a.rank);
   seg->width = (int)width;
-  if (!rc && !few) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {width, (uint32_t)a_rows, 1}, 2 * width);
-  if (!rc && !few) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {width, 64, 1}, 2 * width);
+  if (!rc && !plain) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {width, (uint32_t)a_rows, 1}, 2 * width);
+  if (!rc && !plain) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {width, 64, 1}, 2 * width);
   red->scale = a.scale;
   red->v = static_cast<__nv_bfloat16*>(v);
   red->rank = seg->rank = a.rank;
@@ -88,13 +92,13 @@ int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, i
   return rc;
 }
 
-// The reduced rows of up to two projections of the same input, and what the product needs of them.
+// The reduced rows of up to two projections of the same input, and what the product (which may read `plain`ly) needs of them.
 struct AdapterPlan {
   AdapterReduce red{};
   DenseAdapters add{};
 };
 int plan_adapters(AdapterPlan* p, const AteniaLowRank* const (&sets)[2], const int32_t* ids, int n, const void* x, int64_t T,
-                  int64_t in, int64_t out, uint8_t** ws, bool chained) {
+                  int64_t in, int64_t out, bool plain, uint8_t** ws, bool chained) {
   const int a_rows = dense_a_rows(T);
   p->red.ids = p->add.ids = ids;
   p->red.n = p->add.n = n;
@@ -109,7 +113,7 @@ int plan_adapters(AdapterPlan* p, const AteniaLowRank* const (&sets)[2], const i
   int rc = p->red.few ? ATENIA_OK : matrix_map(&p->red.x, x, T, in, a_rows);
   for (int i = 0; i < 2 && !rc; ++i) {
     if (!sets[i] || sets[i]->rank == 0) continue;
-    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, p->red.few, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
+    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, p->red.few, plain, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
     p->red.projections += 1;
     *ws += reduced_bytes(T, sets[i]->rank);
   }
@@ -216,12 +220,12 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   p2.out = static_cast<__nv_bfloat16*>(y);
   if (!rc) rc = set_operands(&p2, h, w_down, nullptr, g2.a_rows);
   if (!rc && ad1) {
-    rc = plan_adapters(&first, {&adapters->gate, &adapters->up}, adapters->ids, adapters->n, x, T, d, F, &ws, true);
+    rc = plan_adapters(&first, {&adapters->gate, &adapters->up}, adapters->ids, adapters->n, x, T, d, F, reads_plainly(p1, x, w_gate, w_up), &ws, true);
     g1.adapters = &first.add;
     g1.b_early = g1.a_early = true;  // (only the adapters' rows are the kernel before's)
   }
   if (!rc && ad2) {
-    rc = plan_adapters(&second, {&adapters->down, nullptr}, adapters->ids, adapters->n, h, T, F, d, &ws, true);
+    rc = plan_adapters(&second, {&adapters->down, nullptr}, adapters->ids, adapters->n, h, T, F, d, reads_plainly(p2, h, w_down, nullptr), &ws, true);
     g2.adapters = &second.add;
     // (h too: the kernel before is the reduction, whose CTAs let this one start when the one that wrote h had completed)
     g2.a_early = true;
@@ -337,7 +341,6 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AdapterPlan plan;
-  rc = plan_adapters(&plan, {adapter, nullptr}, ids, n, x, T, d_in, d_out, &ws, true);
   DenseGemm g{};
   g.problems = 1;
   g.epilogue = kDensePlain;
@@ -349,6 +352,7 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   p.N = d_out;
   p.K = d_in;
   p.out = static_cast<__nv_bfloat16*>(y);
+  rc = plan_adapters(&plan, {adapter, nullptr}, ids, n, x, T, d_in, d_out, reads_plainly(p, x, weight, nullptr), &ws, true);
   if (!rc) rc = set_operands(&p, x, weight, nullptr, g.a_rows);
   if (!rc) rc = launch_adapter_reduce(plan.red, sms, s);
   if (!rc) rc = launch_dense_gemm(g, sms, s);

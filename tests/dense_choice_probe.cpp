@@ -9,3 +9,9 @@ extern "C" void choice_dense(const long long* sizes, int problems, int rows, int
   const atenia::DensePlan p = atenia::dense_plan(s, problems, rows, two_columns != 0, grad != 0, full_rows != 0, adapters, num_sms);
   out[0] = p.pairs, out[1] = p.columns, out[2] = p.split, out[3] = p.tail_split;
 }
+
+// out: pieces, blocks
+extern "C" void choice_rows(int groups, int steps, int warps, int places, int* out) {
+  const atenia::RowsPlan p = atenia::rows_plan(groups, steps, warps, places);
+  out[0] = p.pieces, out[1] = p.blocks;
+}

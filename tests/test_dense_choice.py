@@ -12,12 +12,15 @@ FORWARD, DOWN, GATE_GRAD, DX, DW = range(5)
 
 
 @pytest.fixture(scope="module")
-def plan(tmp_path_factory):
+def lib(tmp_path_factory):
     so = tmp_path_factory.mktemp("choice") / "libdensechoice.so"
     subprocess.check_call(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", os.path.join(ROOT, "tests", "dense_choice_probe.cpp"),
                            "-o", str(so)])
-    lib = C.CDLL(str(so))
+    return C.CDLL(str(so))
 
+
+@pytest.fixture(scope="module")
+def plan(lib):
     def blocks(k):
         return -(-k // 64)
 
@@ -75,3 +78,21 @@ def test_the_kernel_taken_is_near_the_fastest(plan, kind, T, d, F, us):
 def test_a_last_wave_of_few_tiles_is_cut(plan):
     """5000 x 2048 over 5632: 160 tiles on 74 pairs of SMs."""
     assert plan(DOWN, 5000, 2048, 5632)[:2] == (1, 256) and plan(DOWN, 5000, 2048, 5632)[3] > 1
+
+
+def test_pieces_of_a_few_rows(lib):
+    """Every row group has its warps, every piece its steps; a small matrix is cut as far as that goes, a large one hardly."""
+    out = (C.c_int * 2)()
+
+    def rows(groups, steps, places):
+        lib.choice_rows(groups, steps, 8, places, out)
+        return tuple(out)
+
+    for groups in [*range(1, 70), 128, 1000, 65536, 131072]:
+        for steps in [1, 2, 3, 4, 7, 8, 16, 33, 16384]:
+            for places in (80, 296, 444):
+                pieces, blocks = rows(groups, steps, places)
+                assert pieces in (1, 2, 4, 8) and (pieces == 1 or steps >= 2 * pieces)
+                assert (blocks - 1) * (8 // pieces) < groups <= blocks * (8 // pieces)
+    assert rows(2, 1, 296) == (1, 1) and rows(1, 16384, 296) == (1, 1)
+    assert rows(176, 8, 296) == (4, 88) and rows(65536, 64, 444)[0] <= 2

@@ -6,7 +6,7 @@ import ffn_helpers as ref
 
 pytestmark = pytest.mark.gpu
 
-SIZES = [(1, 16, 16), (1, 512, 1408), (2, 48, 80), (7, 272, 144), (8, 64, 64), (9, 64, 128), (64, 512, 1408), (100, 16, 2064),
+SIZES = [(1, 16, 16), (1, 512, 1408), (2, 48, 80), (7, 272, 144), (8, 64, 64), (9, 64, 128), (16, 1040, 48), (16, 272, 2064), (64, 512, 1408), (100, 16, 2064),
          (127, 1040, 48), (128, 272, 144), (129, 272, 144), (255, 144, 272), (257, 512, 400), (700, 1040, 1424), (1021, 528, 1040),
          (2100, 768, 1552),
          # reductions cut over clusters of single CTAs and of pairs, and behind the last whole wave (tests/test_dense_choice.py)
@@ -138,3 +138,24 @@ def test_captured_and_replayed_beside_another_stream(T):
         torch.cuda.synchronize()
         for _, _, eager, out in steps:
             assert all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+@pytest.mark.parametrize("T", [1, 7, 16, 40])
+def test_operands_on_16_byte_boundaries(T):
+    """Eight elements into an allocation: the kernels that want 32 bytes leave the call to others."""
+    from ateniaengine_b200 import gated_ffn, gated_ffn_backward
+    d, F = 272, 144
+
+    def shifted(t):
+        buf = torch.empty(t.numel() + 8, device="cuda", dtype=t.dtype)
+        buf[8:] = t.flatten()
+        return buf[8:].view(t.shape)
+
+    x, w, dy = ref.rand(1, 1.0, T, d), ref.block(2, d, F), ref.rand(5, 1.0, T, d)
+    sx, sw, sdy = shifted(x), [shifted(t) for t in w], shifted(dy)
+    assert sx.data_ptr() % 32 == 16
+    y, saved = gated_ffn(sx, *sw, save=True, out=shifted(x), sync=True)
+    ref.assert_within(y, ref.forward(x, *w)[0], "y")
+    for got, exp, name in zip(gated_ffn_backward(sdy, sx, *sw, saved, sync=True), ref.backward(dy, x, *w), ("dx", "dgate", "dup", "ddown")):
+        ref.assert_within(got, exp, name)
+    ref.assert_within(gated_ffn(x, *sw), ref.forward(x, *w)[0], "weights alone shifted")
