@@ -52,8 +52,12 @@ __device__ __forceinline__ void add_rows(const AdapterReduce& ar, const RedPart&
     float4 sum = v[0];
 #pragma unroll
     for (int q = 1; q < S; ++q) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
-    *reinterpret_cast<uint2*>(p.v + (int64_t)(m0 + t) * p.rank + at) =
-        make_uint2(pack_bf16x2(sum.x * scale, sum.y * scale), pack_bf16x2(sum.z * scale, sum.w * scale));
+    sum.x *= scale, sum.y *= scale, sum.z *= scale, sum.w *= scale;
+    __nv_bfloat16* to = p.v + (int64_t)(m0 + t) * p.rank + at;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+    if (ar.parts > 1)
+      *reinterpret_cast<uint2*>(to + (int64_t)ar.M * p.rank) = make_uint2(pack_bf16x2(left_of_bf16(sum.x), left_of_bf16(sum.y)),
+                                                                          pack_bf16x2(left_of_bf16(sum.z), left_of_bf16(sum.w)));
   }
 }
 

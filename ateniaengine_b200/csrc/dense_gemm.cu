@@ -65,9 +65,9 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   __shared__ TileBars bars;
   __shared__ std::conditional_t<AD, TileMasks, NoAdapters> list;
   constexpr int N_OUT = EPI == kDenseSwiGLU ? BN / 2 : BN;
-  const uint32_t v_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;  // reduced rows, then the ring
+  const uint32_t v_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;  // reduced rows, then the ring; at the end the sums of a cut reduction
   const uint32_t ring = v_smem + (AD ? ta.v_bytes : 0);
-  float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
+  float* part = reinterpret_cast<float*>(smem_raw + (v_smem - smem_u32(smem_raw)));
   volatile int* abort_flag = &bars.abort_flag;
   const int warp = uniform_warp();
   const int lane = threadIdx.x & 31;
@@ -290,6 +290,7 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         const uint64_t db = make_smem_desc_width(at, ac.width[c]);
         const uint32_t d = tmem + (ac.second[c] ? N_OUT : 0);
         tc_mma_bf16_lanes_one(d, dv[c], db, idesc_ad, ac.steps[c], off);
+        if (ad.parts > 1) tc_mma_bf16_lanes_one(d, dv[c] + (uint32_t)(ac.chunks * v_bytes >> 4), db, idesc_ad, ac.steps[c], off);
       };
       for (int i = rank; ok && left > 0;) {
         const int here = group > 0 ? min(left, group) : 1;
@@ -335,10 +336,11 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
     if constexpr (AD) {
       if (warp == 2 && wait_all(&bars.listed, 0, 2310) && list.count > rank) {
         const uint32_t bar = smem_u32(&bars.v_full);
-        mbar_expect_tx_one(bar, ta.a_rows * 2 * ac.columns);
+        mbar_expect_tx_one(bar, ad.parts * ta.a_rows * 2 * ac.columns);
+        for (int q = 0; q < ad.parts; ++q)
 #pragma unroll
-        for (int c = 0; c < kMaxChunks; ++c)
-          if (c < ac.chunks) tma_load_2d_one(v_smem + c * v_bytes, &ad.seg[ac.second[c]].v, bar, ac.column[c], m0);
+          for (int c = 0; c < kMaxChunks; ++c)
+            if (c < ac.chunks) tma_load_3d_one(v_smem + (q * ac.chunks + c) * v_bytes, &ad.seg[ac.second[c]].v, bar, ac.column[c], m0, q);
         if (*abort_flag)
           for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, 0); ++i) {}
       }
@@ -415,6 +417,19 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
   }
 }
 
+// Of the reduced rows of a tile in shared memory
+int reduced_row_bytes(const DenseGemm& g) {
+  if (!g.adapters) return 0;
+  int chunks = 0, width = 0;
+  for (int i = 0; i < (g.epilogue == kDenseSwiGLU ? 2 : 1); ++i) {
+    const AdapterSegment& seg = g.adapters->seg[i];
+    if (seg.rank == 0) continue;
+    chunks += (seg.rank + seg.width - 1) / seg.width;
+    width = seg.width > width ? seg.width : width;
+  }
+  return (g.adapters->parts * chunks * g.a_rows * width * 2 + 1023) / 1024 * 1024;
+}
+
 template <int EPI, bool B_MN, int NP, bool AD, int BN>
 int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
   auto kernel = dense_tile_kernel<EPI, B_MN, NP, AD, BN>;
@@ -425,24 +440,12 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
   const int rows = g.a_rows;
   const int stage_bytes = rows * BK * 2 + TileSize<BN>::kBBytes;
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};
-  if constexpr (AD) {
-    ad = *g.adapters;
-    int chunks = 0, width = 0;
-    for (int i = 0; i < (EPI == kDenseSwiGLU ? 2 : 1); ++i) {
-      const AdapterSegment& seg = ad.seg[i];
-      if (seg.rank == 0) continue;
-      chunks += (seg.rank + seg.width - 1) / seg.width;
-      width = seg.width > width ? seg.width : width;
-    }
-    ta.v_bytes = (chunks * rows * width * 2 + 1023) / 1024 * 1024;
-  }
+  if constexpr (AD) ad = *g.adapters;
   int ring = TileSize<BN>::kRing - ta.v_bytes;
   if (ring < 2 * stage_bytes) ring = TileSize<256>::kRing - ta.v_bytes;  // (many reduced rows: one CTA per SM)
   ta.stages = ring / stage_bytes;
   if (ta.stages > kTileStages) ta.stages = kTileStages;
-  ring = ta.stages * stage_bytes;
-  const int sums = ta.split > 1 ? rows * kSumsPitch<BN> * 4 : 0;
-  if (ring < sums) ring = sums;
+  const int sums = ta.split > 1 ? rows * kSumsPitch<BN> * 4 : 0, operands = ta.v_bytes + ta.stages * stage_bytes;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ta.split;
@@ -452,7 +455,7 @@ int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles * ta.split);
   cfg.blockDim = dim3(TileSize<BN>::kThreads);
-  cfg.dynamicSmemBytes = 1024 + ta.v_bytes + ring;
+  cfg.dynamicSmemBytes = 1024 + (operands > sums ? operands : sums);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = g.chained ? 2 : 1;
@@ -502,6 +505,9 @@ int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t 
   ta.b_early = g.b_early;
   ta.a_early = g.a_early && g.b_early;
   ta.split = split;
+  ta.v_bytes = reduced_row_bytes(g);
+  // (a ring of two stages at least)
+  if (columns == 256 && ta.v_bytes + 2 * (g.a_rows * BK * 2 + TileSize<256>::kBBytes) > TileSize<256>::kRing) return launch_dense_tiles(g, 128, split, s);
   count_launch();
   count_tcgen05_launch();
   return columns == 256 ? launch_tiles_of<256>(g, ta, (int)tiles, s) : launch_tiles_of<128>(g, ta, (int)tiles, s);

@@ -30,6 +30,7 @@ struct DenseProblem {
   const __nv_bfloat16* a_ptr;     // the same operands for the kernels that read them plainly (dense_rows.cu)
   const __nv_bfloat16* b_ptr[2];
   int K;
+  bool a_rest, out_rest;          // dense_rows.cu, up to kRestMost rows: A, or `out`, is followed by what its rounding to bf16 left
   __nv_bfloat16* out_du;   // kDenseGateGrad: du and h [M, N] (dg is `out`)
   __nv_bfloat16* out_h;
 };
@@ -37,7 +38,7 @@ struct DenseProblem {
 // One projection's adapters beside the product: D[m, :] += B_a v[m, :] for a = ids[m].  (kDenseSwiGLU: segment 0 acts on the
 // gate columns, segment 1 on the up columns; a segment of rank 0 adds nothing.)
 struct AdapterSegment {
-  CUtensorMap v;  // [M, rank] bf16, box {width, rows}, swizzle of the box's width
+  CUtensorMap v;  // [parts, M, rank] bf16, box {width, rows, 1}, swizzle of the box's width
   CUtensorMap b;  // [n, N, rank] bf16, box {width, 64, 1}, likewise
   int rank, width;  // adapter_width(rank)
   const __nv_bfloat16* v_ptr;
@@ -46,10 +47,15 @@ struct AdapterSegment {
 // Rank columns of a box.  TMA takes as long for a row of 32 bytes as for one of 128 (about 4 cycles): boxes are as wide as the rank lets
 // them (columns past it are filled with zeros and left out of the MMAs).
 inline int adapter_width(int rank) { return rank > 32 ? 64 : rank > 16 ? 32 : 16; }
+// The reduced rows are rounded to bf16, the second product's operand.  Where the adapters may make a good part of a sum (its terms are
+// `rank` beside `in`), that rounding would show in the result beside its own; then what the first rounding left is a second operand,
+// multiplied by the same B.  Root mean square of the error, block of 256 x 2048 with rank 128 on all three projections, one part / two:
+// 0.0025 / 0.0023 (0.0017 is the rounding of the result, 0.0017 that of h).
+inline int adapter_parts(int rank, int64_t in) { return (int64_t)32 * rank > in ? 2 : 1; }
 struct DenseAdapters {
   AdapterSegment seg[2];
   const int32_t* ids;  // [M]; an id outside [0, n) means none
-  int n;
+  int n, parts;
 };
 
 constexpr int kMaxDenseProblems = 3;
@@ -68,13 +74,14 @@ int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t 
 int launch_dense_pairs(const DenseGemm& g, int split, int tail_split, int num_sms, cudaStream_t s);  // dense_pair.cu
 int launch_dense_rows(const DenseGemm& g, int num_sms, cudaStream_t s);   // dense_rows.cu, where it serves the product
 bool dense_rows_serve(const DenseGemm& g);
-// Up to 8 rows of a matrix of at most 2^25 elements and up to 16 of one of at most 2^23; one row of any.  Operands on 32-byte boundaries, which the
-// kernel's loads want (any row of a matrix is on one if the first is).  B200, block of 16 tokens, this kernel / dense_gemm.cu's, us: 512 x 1408
-// 5.2 / 8.0, 2048 x 2816 12.5 / 14.8, 2048 x 5632 22.4 / 20.5; of eight 4.6 / 7.8, 10.7 / 14.5, 17.5 / 20.0, 4096 x 14336 65.7 / 61.8; of one
-// 61.0 / 61.8.
+// Up to 8 rows of a matrix of at most 2^25 elements and up to 16 of one of at most 2^23; one row of any.  Operands on 32-byte
+// boundaries, which the kernel's loads want (any row of a matrix is on one if the first is).  B200, block of 16 tokens, this kernel /
+// dense_gemm.cu's, us: 512 x 1408 5.3 / 8.1, 2048 x 2816 12.5 / 14.8, 2048 x 5632 22.4 / 20.5; of eight 5.0 / 7.8, 11.4 / 14.5, 18.9 /
+// 20.1, 4096 x 14336 65.7 / 61.8; of one 61.4 / 61.0.
+constexpr int kRowsMost = 16, kRestMost = 8;
 inline bool dense_rows(int64_t M, int64_t N, int64_t K, bool two, const void* x, const void* w0, const void* w1) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w0) | (two ? reinterpret_cast<uintptr_t>(w1) : 0);
-  return (at & 31) == 0 && M <= 16 && (M == 1 || N * K <= (M <= 8 ? (int64_t)1 << 25 : (int64_t)1 << 23));
+  return (at & 31) == 0 && M <= kRowsMost && (M == 1 || N * K <= (M <= 8 ? (int64_t)1 << 25 : (int64_t)1 << 23));
 }
 
 // Rows of a K-major A box: all of a small batch, so that a call of few tokens moves few token rows.
@@ -85,7 +92,7 @@ struct AdapterReduce {
   struct Projection {
     CUtensorMap a;  // [n, rank, K] bf16, box {64, rank, 1}, 128-byte swizzle
     const float* scale;  // [n]
-    __nv_bfloat16* v;    // [M, rank]
+    __nv_bfloat16* v;    // [parts, M, rank]
     int rank;
     const __nv_bfloat16* a_ptr;
   } p[2];
@@ -93,7 +100,7 @@ struct AdapterReduce {
   CUtensorMap x;  // [M, K], box {64, a_rows}
   const __nv_bfloat16* x_ptr;
   const int32_t* ids;
-  int M, K, kb, n, a_rows;
+  int M, K, kb, n, a_rows, parts;
   bool few;  // adapter_gemv_rows of every projection: the maps are not encoded
   bool chained;
 };
@@ -298,6 +305,11 @@ __device__ __forceinline__ void gate_grad(float dh, float g, float u, float& dg,
 // Four features of a token in the quads of the saved projections
 __device__ __forceinline__ float4* quad(float* base, const DenseProblem& p, int row, int col) {
   return reinterpret_cast<float4*>(base) + (int64_t)(col >> 2) * p.M + row;
+}
+// What rounding `v` to bf16 leaves (nothing of an infinity)
+__device__ __forceinline__ float left_of_bf16(float v) {
+  const float r = v - __bfloat162float(__float2bfloat16(v));
+  return fabsf(r) <= fabsf(v) ? r : 0.f;
 }
 __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));

@@ -358,7 +358,8 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           mbar_arrive(smem_u32(&bars.listed[it & 1]));
         }
         chain_wait();  // v is the kernel before's
-        for (int done = 0; ok && done < found;) {
+        for (int done = 0; ok && done < found * ad.parts;) {
+          const int of = done < found ? 0 : 1, to = (of + 1) * found;  // (which part of the reduced rows, for all adapters)
           // the tile's reduced rows, for the stages of B that follow
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -373,18 +374,18 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 #pragma unroll
             for (int c = 0; c < kMaxChunks; ++c)
               if (c < r.chunks && c >= half * r.v_slots && c < (half + 1) * r.v_slots)
-                load_2d(dst + (c - half * r.v_slots) * r.v_bytes, &ad.seg[r.second[c]].v, bar, r.column[c], t.m0 + (int)rank * BM);
+                load_3d(dst + (c - half * r.v_slots) * r.v_bytes, &ad.seg[r.second[c]].v, bar, r.column[c], t.m0 + (int)rank * BM, of);
             next_stage();
           }
-          for (int b = 0; ok && b < r.b_stages && done < found; ++b) {
+          for (int b = 0; ok && b < r.b_stages && done < to; ++b) {
             if (!free_stage()) break;
-            const int here = min(found - done, r.group);
+            const int here = min(to - done, r.group);
             const uint32_t full = smem_u32(&bars.full[stage]), bar = at_rank(full, lead);
             uint32_t dst = ring + stage * kPairStageBytes;
             if (leader) mbar_expect_tx_one(full, 2 * here * r.columns * r.kRows * 2);
             const int n = t.n0 + (int)rank * (N_OUT / 2);
             for (int q = 0; q < here; ++q) {
-              const int a = lists.adapter[it & 1][done + q];
+              const int a = lists.adapter[it & 1][done - of * found + q];
 #pragma unroll
               for (int c = 0; c < kMaxChunks; ++c) {
                 if (c >= r.chunks) break;
@@ -469,7 +470,8 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
           }
           ok = __all_sync(0xffffffffu, ok);
           const int found = ok ? lists.count[it & 1] : 0;
-          for (int done = 0; ok && done < found;) {
+          for (int done = 0; ok && done < found * ad.parts;) {
+            const int of = done < found ? 0 : 1, to = (of + 1) * found;
             const int v_stage = stage, v_next = stage + 1 == kStages ? 0 : stage + 1;
             const bool two = r.chunks > r.v_slots;
             if (!filled()) break;
@@ -484,13 +486,13 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
               const bool over = c >= r.v_slots;
               dv[c] = make_smem_desc_width(ring + (over ? v_next : v_stage) * kPairStageBytes + (over ? c - r.v_slots : c) * r.v_bytes, r.width[c]);
             }
-            for (int b = 0; ok && b < r.b_stages && done < found; ++b) {
+            for (int b = 0; ok && b < r.b_stages && done < to; ++b) {
               if (!filled()) break;
-              const int here = min(found - done, r.group);
+              const int here = min(to - done, r.group);
               uint32_t at = ring + stage * kPairStageBytes;
               for (int q = 0; q < here; ++q) {
                 uint32_t off[8];
-                lanes_off(off, id, (int32_t)lists.adapter[it & 1][done + q]);
+                lanes_off(off, id, (int32_t)lists.adapter[it & 1][done - of * found + q]);
 #pragma unroll
                 for (int c = 0; c < kMaxChunks; ++c) {
                   if (c >= r.chunks) break;

@@ -6,8 +6,10 @@
 // m16n8k16, the token rows as its n side, 8 or 16 of them.  Lanes take 32 bytes of a row each, 64 of k a step: that orders k inside a
 // step differently from the instruction's operands, for weights and tokens alike, which a sum does not mind.  Two or three steps are on
 // their way (RowsShape).  A block's eight warps are row groups times pieces of the reduction (rows_plan), which are added in order.
-// B200, weights out of L2, us, this kernel / dense_gemm.cu's: block of 1 token, 512 x 1408 4.4 / 7.5, 2048 x 2816 10.4 / 14.3, 2048 x 5632
-// 16.6 / 19.6; of 16, 5.2 / 8.1, 12.5 / 14.8; one product 4096 x 4096 8.2 / 11.1 (1 token), 8.5 / 11.9 (8).  The bytes of a block
+// h of a block of up to eight tokens comes in two parts, its rounding to bf16 and what that left, as twice the tokens of the second
+// product: their columns would be empty, and the result is as exact as its own rounding (its error is 1.42 times that otherwise).
+// B200, weights out of L2, us, this kernel / dense_gemm.cu's: block of 1 token, 512 x 1408 4.5 / 7.5, 2048 x 2816 10.4 / 14.3, 2048 x 5632
+// 16.4 / 19.6; of 16, 5.3 / 8.1, 12.5 / 14.8; one product 4096 x 4096 8.2 / 11.1 (1 token), 8.5 / 11.9 (8).  The bytes of a block
 // of 2048 x 2816 take 5.4 us at the copy rate: what is left is the two launches and their first loads.
 //
 // Adapters: a warp adds its piece of the rank columns, v[t, j] B[a, n, j] for the tokens and rows that its lanes hold.  A token reads its
@@ -43,13 +45,14 @@ struct VecArgs {
   float* up;
   int T, N, K, pieces;
   bool early;               // the weights are not the kernel before's
+  bool x_rest, out_rest;    // behind x, and behind out, comes what rounding them left
 };
 struct VecAdapters {
-  const __nv_bfloat16* v[2];  // [T, rank]
+  const __nv_bfloat16* v[2];  // [parts, T, rank]
   const __nv_bfloat16* b[2];  // [n, N, rank]
   int rank[2];
   const int32_t* ids;
-  int n;
+  int n, parts;
 };
 struct NoVecAdapters {};
 
@@ -93,7 +96,7 @@ __device__ __forceinline__ void mma_rows(float (&c)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: tiles of eight tokens.  Lane 4 g + i holds 32 bytes (piece i of a step) of weight rows g and g + 8 and of tokens g, g + 8, and sums
+// NT: tiles of eight tokens (x in two parts: the first half of them the tokens, the other half what their rounding left).  Lane 4 g + i holds 32 bytes (piece i of a step) of weight rows g and g + 8 and of tokens g, g + 8, and sums
 // of those rows for tokens 2 i and 2 i + 1 of a tile.
 template <int EPI, int NT, bool AD, bool LARGE>
 __global__ void __launch_bounds__(kVecThreads, RowsShape<LARGE>::kBlocks)
@@ -127,7 +130,11 @@ dense_rows_kernel(const __grid_constant__ VecArgs va, const __grid_constant__ st
   float c[NT][4] = {};
   const __nv_bfloat16* x[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) x[t] = va.x + (int64_t)min(8 * t + g, va.T - 1) * va.K + 16 * i4;
+  for (int t = 0; t < NT; ++t) {
+    const int column = 8 * t + g;
+    const bool rest = va.x_rest && column >= 4 * NT;
+    x[t] = va.x + ((int64_t)min(rest ? column - 4 * NT : column, va.T - 1) + (rest ? va.T : 0)) * va.K + 16 * i4;
+  }
   for (int s0 = begin; s0 < end; s0 += kAhead) {
     if (s0 > begin) fetch(s0);
     Words xv[NT][kAhead];
@@ -146,6 +153,10 @@ dense_rows_kernel(const __grid_constant__ VecArgs va, const __grid_constant__ st
         for (int q = 0; q < 8; q += 2)
           mma_rows(c[t], a[s].w[q], b[s].w[q], a[s].w[q + 1], b[s].w[q + 1], xv[t][s].w[q], xv[t][s].w[q + 1]);
   }
+  if (va.x_rest) {  // both parts of a token's x
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[0][q] += NT == 1 ? __shfl_xor_sync(0xffffffffu, c[0][q], 2) : c[NT - 1][q];
+  }
   if constexpr (AD) {
     if (live) {
 #pragma unroll
@@ -161,7 +172,11 @@ dense_rows_kernel(const __grid_constant__ VecArgs va, const __grid_constant__ st
             const int r = ad.rank[seg];
             const __nv_bfloat16* bp = ad.b[seg] + ((int64_t)id * va.N + (h ? n1 : n0)) * r;
             const __nv_bfloat16* vp = ad.v[seg] + (int64_t)token * r;
-            for (int j = 8 * piece; j < r; j += 8 * va.pieces) c[t][2 * h + q] = dot8(load16(vp + j), load16(bp + j), c[t][2 * h + q]);
+            for (int j = 8 * piece; j < r; j += 8 * va.pieces) {
+              const uint4 bv = load16(bp + j);
+              c[t][2 * h + q] = dot8(load16(vp + j), bv, c[t][2 * h + q]);
+              if (ad.parts > 1) c[t][2 * h + q] = dot8(load16(vp + (int64_t)va.T * r + j), bv, c[t][2 * h + q]);
+            }
           }
         }
     }
@@ -188,7 +203,9 @@ dense_rows_kernel(const __grid_constant__ VecArgs va, const __grid_constant__ st
       if (token >= va.T) continue;
       __nv_bfloat16* out = va.out + (int64_t)token * va.N;
       if constexpr (EPI == kDenseSwiGLU) {
-        out[n0] = __float2bfloat16(silu_mul(c[t][q], c[t][2 + q]));
+        const float o = silu_mul(c[t][q], c[t][2 + q]);
+        out[n0] = __float2bfloat16(o);
+        if (va.out_rest) out[(int64_t)va.T * va.N + n0] = __float2bfloat16(left_of_bf16(o));
         if (va.gate) {
           const int64_t kept = ((int64_t)(n0 / 4) * va.T + token) * 4 + n0 % 4;  // (in quads: [N / 4][T][4])
           va.gate[kept] = c[t][q];
@@ -212,7 +229,7 @@ struct VecReduce {
   } p[2];
   const __nv_bfloat16* x;
   const int32_t* ids;
-  int K, n;
+  int T, K, n, parts;
 };
 __global__ void __launch_bounds__(kVecThreads) adapter_gemv_kernel(const __grid_constant__ VecReduce vr) {
   __shared__ float part[kVecWarps][kRankGroup];
@@ -247,7 +264,10 @@ __global__ void __launch_bounds__(kVecThreads) adapter_gemv_kernel(const __grid_
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kVecWarps; ++i) sum += part[i][threadIdx.x];
-    p.v[(int64_t)t * p.rank + j0 + threadIdx.x] = __float2bfloat16(sum * p.scale[id]);
+    sum *= p.scale[id];
+    __nv_bfloat16* to = p.v + (int64_t)t * p.rank + j0 + threadIdx.x;
+    *to = __float2bfloat16(sum);
+    if (vr.parts > 1) to[(int64_t)vr.T * p.rank] = __float2bfloat16(left_of_bf16(sum));
   }
 }
 
@@ -262,12 +282,15 @@ int launch_rows(const DenseGemm& g, const VecArgs& va, int blocks, cudaStream_t 
     }
     ad.ids = g.adapters->ids;
     ad.n = g.adapters->n;
+    ad.parts = g.adapters->parts;
   }
   return launch_chained(g.chained, dense_rows_kernel<EPI, NT, AD, LARGE>, dim3(blocks), dim3(kVecThreads), 0, s, va, ad);
 }
 template <int EPI, bool AD>
 int launch_rows_tokens(const DenseGemm& g, const VecArgs& va, bool large, int blocks, cudaStream_t s) {
-  if (va.T > 8) return launch_rows<EPI, 2, AD, false>(g, va, blocks, s);  // (dense_rows: no large ones)
+  if constexpr (EPI == kDensePlain)
+    if (large && va.x_rest && va.T > 4) return launch_rows<EPI, 2, AD, true>(g, va, blocks, s);
+  if (va.T > 8 || (va.x_rest && va.T > 4)) return launch_rows<EPI, 2, AD, false>(g, va, blocks, s);  // (dense_rows: more than 8 of no large one)
   return large ? launch_rows<EPI, 1, AD, true>(g, va, blocks, s) : launch_rows<EPI, 1, AD, false>(g, va, blocks, s);
 }
 
@@ -294,6 +317,8 @@ int launch_dense_rows(const DenseGemm& g, int num_sms, cudaStream_t s) {
   va.N = p.N;
   va.K = p.K;
   va.early = g.b_early;
+  va.x_rest = p.a_rest;
+  va.out_rest = p.out_rest;
   const int groups = g.epilogue == kDenseSwiGLU ? p.N / 8 : p.N / 16;
   const bool large = dense_elements(g) > kLargeElements;
   const RowsPlan plan = rows_plan(groups, (p.K + kStep - 1) / kStep, kVecWarps,
@@ -319,7 +344,9 @@ int launch_adapter_gemv(const AdapterReduce& r, cudaStream_t s) {
   }
   vr.x = r.x_ptr;
   vr.ids = r.ids;
+  vr.T = r.M;
   vr.K = r.K;
+  vr.parts = r.parts;
   vr.n = r.n;
   count_launch();
   return launch_chained(r.chained, adapter_gemv_kernel, dim3(rank / kRankGroup, r.M, r.projections), dim3(kVecThreads), 0, s, vr);

@@ -65,6 +65,9 @@ int set_operands(DenseProblem* p, const void* a, const void* b0, const void* b1,
   return rc;
 }
 
+// h of a call's tokens; of a few it may come in two parts (dense_rows.cu)
+uint64_t h_bytes(int64_t T, int64_t d_ff) { return align256((uint64_t)T * d_ff * (T <= kRestMost ? 4 : 2)); }
+
 bool rank_ok(int r) { return r >= 8 && r <= kAdapterMaxRank && r % 8 == 0; }
 int check_adapter(const AteniaLowRank& a) {
   if (!rank_ok(a.rank)) return ATENIA_ERR_SHAPE;
@@ -72,16 +75,17 @@ int check_adapter(const AteniaLowRank& a) {
   if (!aligned16(a.a) || !aligned16(a.b)) return ATENIA_ERR_SHAPE;
   return ATENIA_OK;
 }
-uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64_t)T * rank * 2) : 0; }
+// (room for two parts: the calls that ask for the size do not all know the width that decides)
+uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64_t)T * rank * 4) : 0; }
 
 // One projection's adapters: the first half's projection and the second half's segment, with v at `v`.
-int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, bool few_reduce,
+int encode_adapter(const AteniaLowRank& a, int64_t T, int64_t in, int64_t out, int n, int a_rows, int parts, bool few_reduce,
                    bool plain, void* v, AdapterReduce::Projection* red, AdapterSegment* seg) {
   const uint64_t r = (uint64_t)a.rank;
   int rc = few_reduce ? ATENIA_OK : encode_tmap_bf16(&red->a, a.a, {(uint64_t)in, r, (uint64_t)n}, {64, (uint32_t)r, 1}, 128);
   const uint32_t width = (uint32_t)adapter_width(a.rank);
   seg->width = (int)width;
-  if (!rc && !plain) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, 0}, {width, (uint32_t)a_rows, 1}, 2 * width);
+  if (!rc && !plain) rc = encode_tmap_bf16(&seg->v, v, {r, (uint64_t)T, (uint64_t)parts}, {width, (uint32_t)a_rows, 1}, 2 * width);
   if (!rc && !plain) rc = encode_tmap_bf16(&seg->b, a.b, {r, (uint64_t)out, (uint64_t)n}, {width, 64, 1}, 2 * width);
   red->scale = a.scale;
   red->v = static_cast<__nv_bfloat16*>(v);
@@ -108,12 +112,14 @@ int plan_adapters(AdapterPlan* p, const AteniaLowRank* const (&sets)[2], const i
   p->red.x_ptr = static_cast<const __nv_bfloat16*>(x);
   p->red.a_rows = a_rows;
   p->red.chained = chained;
-  p->red.few = true;
-  for (const AteniaLowRank* a : sets) p->red.few = p->red.few && (!a || adapter_gemv_rows(T, a->rank, in));
+  int rank = 0;
+  for (const AteniaLowRank* a : sets) rank = a && a->rank > rank ? a->rank : rank;
+  p->red.few = adapter_gemv_rows(T, rank, in);
+  p->red.parts = p->add.parts = adapter_parts(rank, in);
   int rc = p->red.few ? ATENIA_OK : matrix_map(&p->red.x, x, T, in, a_rows);
   for (int i = 0; i < 2 && !rc; ++i) {
     if (!sets[i] || sets[i]->rank == 0) continue;
-    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, p->red.few, plain, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
+    rc = encode_adapter(*sets[i], T, in, out, n, a_rows, p->red.parts, p->red.few, plain, *ws, &p->red.p[p->red.projections], &p->add.seg[i]);
     p->red.projections += 1;
     *ws += reduced_bytes(T, sets[i]->rank);
   }
@@ -163,7 +169,7 @@ uint64_t atenia_gated_ffn_workspace_bytes(int T, int d_model, int d_ff, const At
   if (check_sizes(T, d_model, d_ff)) return 0;
   const uint64_t rows = align256((uint64_t)T * d_ff * 2);
   if (backward) return 3 * rows;  // dg, du, h
-  uint64_t n = rows;              // h
+  uint64_t n = h_bytes(T, d_ff);
   if (adapters) n += reduced_bytes(T, adapters->gate.rank) + reduced_bytes(T, adapters->up.rank) + reduced_bytes(T, adapters->down.rank);
   return n;
 }
@@ -190,7 +196,7 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(ws);
-  ws += align256((uint64_t)T * d_ff * 2);
+  ws += h_bytes(T, d_ff);
   const int64_t d = d_model, F = d_ff;
 
   AdapterPlan first, second;
@@ -219,6 +225,7 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   p2.K = d_ff;
   p2.out = static_cast<__nv_bfloat16*>(y);
   if (!rc) rc = set_operands(&p2, h, w_down, nullptr, g2.a_rows);
+  p1.out_rest = p2.a_rest = T <= kRestMost && reads_plainly(p1, x, w_gate, w_up) && reads_plainly(p2, h, w_down, nullptr);
   if (!rc && ad1) {
     rc = plan_adapters(&first, {&adapters->gate, &adapters->up}, adapters->ids, adapters->n, x, T, d, F, reads_plainly(p1, x, w_gate, w_up), &ws, true);
     g1.adapters = &first.add;
@@ -255,6 +262,18 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!aligned16(p)) return ATENIA_ERR_SHAPE;
   if (workspace_bytes < atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, nullptr, 1)) return ATENIA_ERR_CAPACITY;
+  const uint64_t row = (uint64_t)T * d * 2, weight = (uint64_t)d * F * 2, kept = (uint64_t)T * F * 4;
+  const struct {
+    const void* p;
+    uint64_t bytes;
+  } outs[4] = {{dx, row}, {dw_gate, weight}, {dw_up, weight}, {dw_down, weight}},
+    ins[7] = {{dy, row}, {x, row}, {w_gate, weight}, {w_up, weight}, {w_down, weight}, {saved_gate, kept}, {saved_up, kept}};
+  for (int i = 0; i < 4; ++i) {
+    for (const auto& in : ins)
+      if (overlap(outs[i].p, outs[i].bytes, in.p, in.bytes)) return ATENIA_ERR_SHAPE;
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return ATENIA_ERR_SHAPE;
+  }
   int sms = 0;
   if ((rc = num_sms_of_current_device(&sms))) return rc;
   const uint64_t rows = align256((uint64_t)T * F * 2);

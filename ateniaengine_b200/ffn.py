@@ -140,7 +140,7 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
 
     `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
     the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
-    [2, F / 4, T, 4], the two projections before the activation.  `sync=True` waits and raises what the kernels recorded."""
+    [2, F / 4, T, 4], the two projections before the activation.  `out` may be x.  `sync=True` waits and raises what the kernels recorded."""
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     ad, ranks = None, (0, 0, 0)

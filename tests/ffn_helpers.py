@@ -2,7 +2,8 @@
 
 Roundings: a bf16 rounding is off by at most 2^-8 of the value (half a step), every sum is f32: 2^-24 a term of the sum of the
 magnitudes, whatever the order, doubled for tensor cores that truncate.  The exponential and the quotient of the activation are
-within 2^-18 of the value.  What a rounded operand is off goes through the next product with the magnitudes of its weights."""
+within 2^-18 of the value.  What a rounded operand is off goes through the next product with the magnitudes of its weights.  An adapter's
+reduced rows are one bf16 operand, or two (what the first leaves is rounded once more) where 32 of its rank exceed its input's width."""
 import torch
 
 BF = 2.0 ** -8
@@ -27,7 +28,7 @@ def project(x, w, low=None, ids=None, dx=None):
                 continue
             s = scale[i]
             v = s * (x[rows] @ a[i].T)
-            dv = v.abs() * BF + s.abs() * f32_sum(x[rows], a[i]) + 2.0 ** -22 * v.abs()
+            dv = v.abs() * (BF if 32 * a.shape[1] <= x.shape[1] else BF * BF) + s.abs() * f32_sum(x[rows], a[i]) + 2.0 ** -22 * v.abs()
             if dx is not None:
                 dv = dv + s.abs() * dx[rows] @ a[i].abs().T
             y[rows] += v @ b[i].T
@@ -40,7 +41,7 @@ def adapter_linear(x, w, low, ids):
     return y, e + (y.abs() + e) * BF
 
 
-def forward(x, gate, up, down, adapters=None, ids=None):
+def forward(x, gate, up, down, adapters=None, ids=None, h_rounding=BF):
     """(y, bound of y), and what the backward pass needs of the way there."""
     low = adapters or {}
     x = x.double()
@@ -48,7 +49,7 @@ def forward(x, gate, up, down, adapters=None, ids=None):
     u, eu = project(x, up.double(), low.get("up"), ids)
     s = torch.sigmoid(g)
     h = g * s * u
-    dh = h.abs() * (BF + ACT) + 1.1 * u.abs() * eg + (g * s).abs() * eu + 1.1 * eg * eu  # |silu'| <= 1.1
+    dh = h.abs() * (h_rounding + ACT) + 1.1 * u.abs() * eg + (g * s).abs() * eu + 1.1 * eg * eu  # |silu'| <= 1.1
     y, e = project(h, down.double(), low.get("down"), ids, dx=dh)
     return (y, e + (y.abs() + e) * BF), (g, eg, u, eu, s, h, dh)
 

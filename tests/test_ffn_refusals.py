@@ -65,6 +65,16 @@ def test_pointers_of_one_direction(lib):
         assert _backward(lib, **{name: P + 4}) == -2, name
 
 
+def test_gradients_over_inputs_or_one_another(lib):
+    apart = {n: P + (i << 16) for i, n in enumerate(("dy", "x", "gate", "up", "down", "sg", "su", "dx", "dg", "du", "dd"))}
+    sizes = dict(dy=512, x=512, gate=12288, up=12288, down=12288, sg=1536, su=1536, dx=512, dg=12288, du=12288, dd=12288)
+    for out in ("dx", "dg", "du", "dd"):
+        for other in apart:
+            if other != out:
+                assert _backward(lib, **{**apart, out: apart[other]}) == -2, (out, other)
+                assert _backward(lib, **{**apart, out: apart[other] + sizes[other] - 16}) == -2, (out, other)
+
+
 def test_adapters_of_the_block(lib):
     from ateniaengine_b200 import _lib
     def call(**kw):

@@ -159,3 +159,21 @@ def test_operands_on_16_byte_boundaries(T):
     for got, exp, name in zip(gated_ffn_backward(sdy, sx, *sw, saved, sync=True), ref.backward(dy, x, *w), ("dx", "dgate", "dup", "ddown")):
         ref.assert_within(got, exp, name)
     ref.assert_within(gated_ffn(x, *sw), ref.forward(x, *w)[0], "weights alone shifted")
+
+
+@pytest.mark.parametrize("d,F", [(16, 16), (272, 144), (528, 2064), (2048, 5632)])
+@pytest.mark.parametrize("T", [1, 3, 4, 5, 8])
+def test_few_tokens_are_as_exact_as_their_last_rounding(T, d, F):
+    """What the rounding of h left goes through the second product too."""
+    from ateniaengine_b200 import gated_ffn
+    x, w = ref.rand(T, 1.0, T, d), ref.block(2, d, F)
+    ref.assert_within(gated_ffn(x, *w, sync=True), ref.forward(x, *w, h_rounding=ref.BF ** 2)[0], "y")
+
+
+@pytest.mark.parametrize("T", [5, 40, 600])
+def test_in_place(T):
+    from ateniaengine_b200 import gated_ffn
+    d, F = 272, 2064
+    x, w = ref.rand(T, 1.0, T, d), ref.block(2, d, F)
+    y = gated_ffn(x, *w)
+    assert gated_ffn(x, *w, out=x, sync=True).data_ptr() == x.data_ptr() and torch.equal(x, y)
