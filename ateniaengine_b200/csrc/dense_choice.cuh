@@ -8,7 +8,9 @@
 //              its SM and 0.48 beside another
 //   tail     : 2 us for a launch of its own
 //   splits   : what adding the sums through distributed shared memory costs
-//   adapters : 0.1 us of each on a tile of 128 columns (a batch of few rows may have one per row; a tile of a prompt has a few)
+//   adapters : 0.1 us of each on a tile of 128 columns (a batch of few rows may have one per row; up to 512 rows are taken for a decode
+//              batch with up to 64 a tile, 300 rows of 90 requests beside 4096 x 4096 50 -> 27 us, of five 29 -> 23; more for prompts, of
+//              which a tile has a few: 4000 rows of 90 requests through a block of 2048 x 5632 would go from 247 to 298)
 #pragma once
 #include <stdint.h>
 
@@ -48,7 +50,7 @@ inline DensePlan dense_plan(const DenseSize* sizes, int problems, int rows, bool
     least_kb = s.kb < least_kb ? s.kb : least_kb;
     bytes += 128.0 * s.kb * (s.M + (two_columns ? 2 : 1) * s.N) + (grad ? 14.0 : 2.0) * s.M * s.N;
   }
-  const int most = sizes[0].M > 128 ? 8 : (int)sizes[0].M;
+  const int most = sizes[0].M > 512 ? 8 : sizes[0].M > 128 ? 64 : (int)sizes[0].M;
   const double extra = 0.1 * (adapters < most ? adapters : most);
   const double floor = 4.5 + bytes / 5.35e6, f = rows / 128.0;
   DensePlan best{false, 128, 1, 1};
