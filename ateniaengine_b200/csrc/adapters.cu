@@ -6,6 +6,7 @@
 // decode batch in which every row has its own adapter reads each A once, which is what bounds it, and a tensor core has the
 // products to spare (64 rows, rank 16: 1 GFLOP instead of 8 MFLOP per 4096 inputs).  A cluster of up to 8 CTAs cuts the reduction
 // and adds in rank order.
+#include "dense_choice.cuh"
 #include "dense_gemm.cuh"
 
 namespace atenia {
@@ -34,18 +35,18 @@ struct RedPart {
   int first, count, rank0, cols;  // projections first .. first + count - 1; rank rows of the first and of all
 };
 
-// This rank's share of the tile's sums, four rank rows a thread, added in rank order.
+// This rank's share of the tile's sums, four rank rows a thread, added in rank order.  The threads of all ranks take neighbouring pieces,
+// since a pass's rows, those of one or two adapters, are neighbours more often than not.
 template <int S>
-__device__ __forceinline__ void add_rows(const AdapterReduce& ar, const RedPart& rp, int m0, int rows, uint32_t part, const TileList& list,
-                                         const int16_t* slot, int begin_slot, int end_slot, int rank) {
+__device__ __forceinline__ void add_rows(const AdapterReduce& ar, const RedPart& rp, int m0, int rows, uint32_t part,
+                                         const float (*scales)[BM], const int16_t* slot, int begin_slot, int end_slot, int rank) {
   const int quads = rp.cols / 4, total = rows * quads;
-  const int begin = total * rank / S, end = total * (rank + 1) / S;
-  for (int i = begin + (int)threadIdx.x; i < end; i += kRedThreads) {
+  for (int i = rank * kRedThreads + (int)threadIdx.x; i < total; i += S * kRedThreads) {
     const int t = i / quads, j = 4 * (i - t * quads);
     if (slot[t] < begin_slot || slot[t] >= end_slot) continue;
     const AdapterReduce::Projection& p = ar.p[rp.first + (j >= rp.rank0)];
     const int at = j >= rp.rank0 ? j - rp.rank0 : j;
-    const float scale = p.scale[list.id[t]];
+    const float scale = scales[j >= rp.rank0][t];
     float4 v[S];
 #pragma unroll
     for (int q = 0; q < S; ++q) v[q] = ld_cluster_f32x4(part + (t * kRedPitch + j) * 4, q);
@@ -67,6 +68,7 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int l
   __shared__ RedBars bars;
   __shared__ TileList list;
   __shared__ int16_t slot[BM];  // of a row's adapter in the list, -1 where it has none
+  __shared__ float scales[2][BM];  // ... and its scales
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   float* part = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
   volatile int* abort_flag = &bars.abort_flag;
@@ -185,6 +187,8 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int l
     } else {
       const int quarter = warp & 3;
       const int row = quarter * 32 + lane;
+      if (pass == first_pass && slot[row] >= 0)  // (behind the pass's loads; what follows waits for them)
+        for (int i = 0; i < rp.count; ++i) scales[i][row] = ar.p[rp.first + i].scale[list.id[row]];
       const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full), acc_phase, abort_flag));
       if (!ready) {
         if (lane == 0) report_error(err, ATENIA_ERR_DEVICE_TIMEOUT, 2600);
@@ -196,15 +200,19 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int l
         for (int i = 0; i < here; ++i) {
           if (!__any_sync(0xffffffffu, mine == i)) continue;
 #pragma unroll 1
-          for (int j = 0; j < rp.cols; j += 8) {
-            uint32_t v[8];
-            tc_ld8(taddr + i * rp.cols + j, v);
+          for (int j = 0; j < rp.cols; j += 32) {
+            uint32_t v[4][8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (j + 8 * q < rp.cols) tc_ld8(taddr + i * rp.cols + j + 8 * q, v[q]);
             tc_ld_wait();
-            if (mine == i) {
-              uint4* dst = reinterpret_cast<uint4*>(part + row * kRedPitch + j);
-              dst[0] = make_uint4(v[0], v[1], v[2], v[3]);
-              dst[1] = make_uint4(v[4], v[5], v[6], v[7]);
-            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (mine == i && j + 8 * q < rp.cols) {
+                uint4* dst = reinterpret_cast<uint4*>(part + row * kRedPitch + j + 8 * q);
+                dst[0] = make_uint4(v[q][0], v[q][1], v[q][2], v[q][3]);
+                dst[1] = make_uint4(v[q][4], v[q][5], v[q][6], v[q][7]);
+              }
           }
         }
         tc_fence_before();
@@ -215,10 +223,10 @@ adapter_reduce_kernel(const __grid_constant__ AdapterReduce ar, int split, int l
     if (split > 1) cluster_barrier();
     if (!*abort_flag) {
       const uint32_t sums = smem_u32(part);
-      if (split == 1) add_rows<1>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
-      else if (split == 2) add_rows<2>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
-      else if (split == 4) add_rows<4>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
-      else add_rows<8>(ar, rp, m0, rows, sums, list, slot, begin, begin + here, rank);
+      if (split == 1) add_rows<1>(ar, rp, m0, rows, sums, scales, slot, begin, begin + here, rank);
+      else if (split == 2) add_rows<2>(ar, rp, m0, rows, sums, scales, slot, begin, begin + here, rank);
+      else if (split == 4) add_rows<4>(ar, rp, m0, rows, sums, scales, slot, begin, begin + here, rank);
+      else add_rows<8>(ar, rp, m0, rows, sums, scales, slot, begin, begin + here, rank);
     }
     __syncthreads();
     if (split > 1) cluster_barrier();  // no CTA goes on, or leaves, while another reads its sums
@@ -240,20 +248,13 @@ int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s) {
   DeviceError* err = nullptr;
   int rc = dense_error_word(&err);
   if (rc) return rc;
-  // a tile has no more distinct adapters than rows
-  const int most = r.n < BM ? (r.M < r.n ? r.M : r.n) : (r.M < BM ? r.M : BM);
   const bool together = r.projections > 1 && r.p[0].rank + r.p[1].rank <= kRankRows;
   int widest = 0;
   for (int i = 0; i < r.projections; ++i) widest = together ? widest + r.p[i].rank : (r.p[i].rank > widest ? r.p[i].rank : widest);
-  const int passes = (most + kRankRows / widest - 1) / (kRankRows / widest);
   const int64_t tiles = (int64_t)m_tiles * (together ? 1 : r.projections);
   if (tiles > (1 << 24)) return ATENIA_ERR_SHAPE;
-  // the reduction over a cluster until every SM has two CTAs, each with two k-blocks at least; then the passes that a tile can have side by side
-  // (most tiles of a prompt have one, and the CTAs of the others leave at once)
-  int split = 1;
-  while (split < 8 && tiles * split < 2 * num_sms && r.kb >= 4 * split) split *= 2;
-  int64_t lanes = 2 * num_sms / (tiles * split);
-  lanes = lanes < 1 ? 1 : lanes > passes ? passes : lanes;
+  const ReducePlan plan = reduce_plan(r.M, tiles, r.kb, r.n, kRankRows / widest, num_sms);
+  const int split = plan.split, lanes = plan.lanes;
   const int64_t units = tiles * lanes;
   const int stage_bytes = r.a_rows * BK * 2 + kRankRows * BK * 2;
   int stages = kRedRingBytes / stage_bytes;
@@ -277,7 +278,7 @@ int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s) {
   cfg.numAttrs = r.chained ? 2 : 1;
   count_launch();
   count_tcgen05_launch();
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_reduce_kernel, r, split, (int)lanes, (int)together, stages, err);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_reduce_kernel, r, split, lanes, (int)together, stages, err);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return (int)e;
 }

@@ -92,6 +92,34 @@ inline DensePlan dense_plan(const DenseSize* sizes, int problems, int rows, bool
   return best;
 }
 
+// adapters.cu: a tile of 128 token rows takes passes of so many adapters; CTAs side by side take the passes (lanes) or share one's reduction
+// (split).  Microseconds: a pass's loads, sums and stores 2, a cluster's two barriers 2.2, a k-block 0.23; measured with clock64.  How many
+// passes a tile has only the device knows: one per row in a decode batch, a few in a prompt.
+// B200, whole calls: 2000 rows of 90 requests, rank 128 of 1024 inputs beside 4096 outputs 87.5 us with the greatest split, 77.3 so; a block of
+// 1024 x 4096 with rank 64, 500 rows of 90 requests 95.1 and 87.8.
+struct ReducePlan {
+  int split, lanes;
+};
+inline ReducePlan reduce_plan(int64_t rows, int64_t tiles, int kb, int n, int per_pass, int num_sms) {
+  const int64_t most = n < 128 ? (rows < n ? rows : n) : (rows < 128 ? rows : 128);
+  const int64_t likely = rows > 512 ? 4 : rows > 128 ? 16 : rows;
+  const int64_t passes = dense_ceil(most, per_pass), expected = dense_ceil(most < likely ? most : likely, per_pass);
+  const int64_t places = 2 * num_sms;
+  ReducePlan best{1, 1};
+  double best_us = 1e30;
+  for (int split = 1; split <= 8 && (split == 1 || kb >= 2 * split); split *= 2) {
+    int64_t lanes = places / (tiles * split);
+    lanes = lanes < 1 ? 1 : lanes > passes ? passes : lanes;
+    const double waves = (double)dense_ceil(tiles * split * lanes, places), rounds = (double)dense_ceil(expected, lanes);
+    const double us = waves * (1.6 + rounds * (0.23 * kb / split + 2.0 + (split > 1 ? 2.2 : 0.0)));
+    if (us < best_us) {
+      best_us = us;
+      best = {split, (int)lanes};
+    }
+  }
+  return best;
+}
+
 // dense_rows.cu: row groups, each cut in 1, 2, 4 or 8 pieces of the reduction (of two steps at least), `warps` of them to a block; the
 // cut that leaves the fewest of the `places` for blocks empty in the last wave, the least one of equals.
 struct RowsPlan {

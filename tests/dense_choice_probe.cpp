@@ -15,3 +15,9 @@ extern "C" void choice_rows(int groups, int steps, int warps, int places, int* o
   const atenia::RowsPlan p = atenia::rows_plan(groups, steps, warps, places);
   out[0] = p.pieces, out[1] = p.blocks;
 }
+
+// out: split, lanes
+extern "C" void choice_reduce(long long rows, long long tiles, int kb, int n, int per_pass, int num_sms, int* out) {
+  const atenia::ReducePlan p = atenia::reduce_plan(rows, tiles, kb, n, per_pass, num_sms);
+  out[0] = p.split, out[1] = p.lanes;
+}

@@ -96,3 +96,22 @@ def test_pieces_of_a_few_rows(lib):
                 assert (blocks - 1) * (8 // pieces) < groups <= blocks * (8 // pieces)
     assert rows(2, 1, 296) == (1, 1) and rows(1, 16384, 296) == (1, 1)
     assert rows(176, 8, 296) == (4, 88) and rows(65536, 64, 444)[0] <= 2
+
+
+def test_cut_and_lanes_of_the_reduced_rows(lib):
+    out = (C.c_int * 2)()
+
+    def reduce(rows, kb, n, per_pass, projections=1):
+        tiles = -(-rows // 128) * projections
+        lib.choice_reduce(C.c_longlong(rows), C.c_longlong(tiles), kb, n, per_pass, 148, out)
+        split, lanes = out
+        assert split in (1, 2, 4, 8) and (split == 1 or kb >= 2 * split) and 1 <= lanes <= max(1, -(-min(n, rows, 128) // per_pass))
+        assert tiles * split * lanes < 1 << 31
+        return split, lanes
+
+    for rows in (1, 17, 128, 129, 500, 513, 5000, 1 << 24):
+        for kb in (1, 2, 3, 16, 64, 16384):
+            for n in (1, 3, 90, 65536):
+                for per_pass in (1, 2, 16):
+                    reduce(rows, kb, n, per_pass, 2)
+    assert reduce(1100, 32, 16, 2) == (8, 4) and reduce(2000, 16, 60, 1) == (4, 4)
