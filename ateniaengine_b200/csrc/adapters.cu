@@ -1,11 +1,13 @@
-// First half of the low-rank adapters: v[t, :] = scale[a] * (A_a x[t, :]) with a = ids[t], rounded to bf16 (the second product's
-// operand; the sums, over CTAs too, are f32).
+// First half of the low-rank adapters: v[t, :] = scale[a] * (A_a x[t, :]) with a = ids[t], in one or two bf16 parts (adapter_parts; the
+// second product's operand; the sums, over CTAs too, are f32).
 //
 // A tile is 128 token rows; its distinct adapters, in the order of their first rows, are taken up to 128 rank rows at a time (of gate
-// and up together where they fit) as the N side of one MMA, and a row keeps the columns of its own adapter.  Rows of other adapters are computed and dropped: a
-// decode batch in which every row has its own adapter reads each A once, which is what bounds it, and a tensor core has the
-// products to spare (64 rows, rank 16: 1 GFLOP instead of 8 MFLOP per 4096 inputs).  A cluster of up to 8 CTAs cuts the reduction
-// and adds in rank order.
+// and up together where they fit) as the N side of one MMA, and a row keeps the columns of its own adapter.  Rows of other adapters are
+// computed and dropped: each A is read once a tile, and a tensor core has the products to spare (128 rows, rank 16 of 4096 inputs: 2 GFLOP
+// for 128 adapters instead of 17 MFLOP).  CTAs side by side take passes of adapters, and a cluster of up to 8 cuts the reduction and adds in
+// rank order (reduce_plan).  What bounds it is latency: of 6.3 us inside the kernel (1100 rows, rank 64 of 2048 inputs, a pass, four
+// k-blocks a CTA) the list of adapters takes 1.0, the first load 0.8, the MMAs behind the loads 0.9, the two barriers of the cluster
+// 1.0 each and the sums 0.7.
 #include "dense_choice.cuh"
 #include "dense_gemm.cuh"
 
@@ -18,7 +20,7 @@ constexpr int kRedStages = 6;       // at most
 constexpr int kRedThreads = 192;
 constexpr int kRedTmemCols = 128;
 constexpr int kRedRingBytes = 100 * 1024;
-constexpr int kRedPitch = kAdapterMaxRank + 4;  // floats (see kPartPitch)
+constexpr int kRedPitch = kAdapterMaxRank + 4;  // floats (see kSumsPitch)
 constexpr int kRedPartBytes = BM * kRedPitch * 4;  // f32 sums [row][rank row]
 static_assert(kRedPartBytes <= kRedRingBytes, "");
 

@@ -1,13 +1,15 @@
-// Dense products on one CTA per tile (tcgen05 cta_group::1): 128 rows x 128 columns, the reduction cut over a cluster.
+// Dense products on one CTA per tile (tcgen05 cta_group::1): 128 rows x 128 or 256 columns, the reduction cut over a cluster.
 //
 // D[m, n] = sum_k A[m, k] B[n, k]; a lane of tensor memory holds a row of D, so the epilogue of a row (gate and up of a feature,
 // the saved values, 32 contiguous bytes of the result) stays in one thread.
-//   k-block: 64; a stage holds the A rows the call has (8 .. 128) and 128 B rows (kDenseSwiGLU: 64 gate and 64 up rows)
-//   split  : the CTAs of a cluster (1, 2, 4, 8) take consecutive k ranges of one tile and add their f32 sums through distributed
+//   k-block: 64; a stage holds the A rows the call has (8 .. 128) and the tile's B rows (kDenseSwiGLU: half gate and half up rows)
+//   split  : the CTAs of a cluster (1, 2, 3, 4, 6, 8) take consecutive k ranges of one tile and add their f32 sums through distributed
 //            shared memory in rank order, so results do not depend on timing and nothing is kept in global memory
-// What bounds it: for few rows the weights' bytes (two CTAs per SM, 80 to 100 KiB of loads in flight each).
+// What bounds it: for few rows the weights' bytes (two CTAs per SM with 100 KiB of loads in flight each, or one with 190: 37 rows, gate and
+// up of 4096 x 14336 235 MB in 41 us, 5.7 TB/s); for some hundred rows the MMAs, which wait for shared memory (333 rows, 2048 x 5632: 11 of
+// 17 us), and the 5 us before the first and after the last of them.
 //
-// Adapters: after its k range a CTA takes its share of the tile's adapters (ascending ids, dealt over the ranks).  For adapter a it
+// Adapters: a CTA takes its share of the tile's adapters (in the order of their first rows, dealt over the ranks).  For adapter a it
 // multiplies the tile's reduced rows v (K = 16 steps) by B_a with the lanes of all other rows disabled, so a row only ever adds
 // its own adapter: no row is multiplied by zero for another one's, and infinities or NaN in an adapter stay with its own rows.
 #include <type_traits>
@@ -22,7 +24,7 @@ constexpr int kTileStages = 8;   // at most
 
 template <int BN>
 struct TileSize {
-  static constexpr int kEpiWarps = BN / 32;  // 128 columns a warp and lane quarter at most... two warps a quarter for 256
+  static constexpr int kEpiWarps = BN / 32;  // a warp has 128 columns of a quarter of the lanes
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kBBytes = BN * BK * 2;
   static constexpr int kRing = BN == 128 ? 108 * 1024 : 196 * 1024;  // two CTAs per SM, or one

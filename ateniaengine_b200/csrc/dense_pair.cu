@@ -3,8 +3,9 @@
 // Two CTAs on the two SMs of a TPC stage 128 A rows and half of the 256 B rows each (kDenseSwiGLU: rank 0 the gate rows of 128
 // features, rank 1 their up rows) and the leader issues M256 x N256 x K16 MMAs over both CTAs' shared memory, so that a byte
 // brought to an SM is used for twice the products of a single CTA's tile (whose MMAs wait for shared memory: 128 x 256 of one CTA
-// reads and writes 192 bytes a cycle at full rate, a pair 128).  Persistent: one CTA per SM, two accumulators in tensor memory, so that the epilogue of a tile runs under the MMAs of the next.
-//   k-block : 64; a stage is 16 KiB of A and 16 KiB of B per CTA, six stages
+// reads and writes 192 bytes a cycle at full rate, a pair 128).  Persistent: one CTA per SM, two accumulators in tensor memory, so that the
+// epilogue of a tile runs under the MMAs of the next.
+//   k-block : 64; a stage is 16 KiB of A and 16 KiB of B per CTA, six stages (kDenseGateGrad five)
 //   order   : bands of kBand row tiles, column tile by column tile, so that the 74 tiles at work at one time share few operand rows in L2
 //   split   : where the tiles are too few, or the last wave's are, the pairs of a cluster (two, three or four) share a tile: consecutive k
 //             ranges, added through distributed shared memory in rank order.  (The last wave is a launch of its own then: 5000 tokens of
@@ -13,7 +14,9 @@
 //             lane were 32 lines an access, and a tile's 5400 cycles of them hid only behind a reduction of 700 and more)
 //
 // Adapters as in dense_gemm.cu: behind the k-blocks of a tile come the steps of the adapters that its rows have, with the lanes
-// of other rows disabled.
+// of other rows disabled.  What an adapter costs is its MMAs over all 256 rows and their masks (about 600 cycles a tile and adapter at
+// rank 32 of gate and up).  What bounds the rest: the power cap (5000 tokens of 2048 x 5632: 223 us cold, 1.55 PFLOP/s; 270 in a loop, at the
+// rate that the library's product sustains), and whole waves of tiles for some thousand rows.
 //
 // No TMA multicast is used: every CTA fetches its own tiles (cp.async.bulk.tensor ... cta_group::2 only routes the completion to
 // the leader's mbarrier).  Barriers: full[s] lives in the leader and collects the bytes of both CTAs; empty[s] and acc_full[b] exist
@@ -196,7 +199,7 @@ struct AdapterRounds : AdapterChunks<EPI> {
     b_stages = kPairStages - (this->chunks > v_slots ? 2 : 1);
   }
 };
-// The adapters of two tiles, found by the producer between its loads (in ascending order; of a split reduction every split-th)
+// The adapters of two tiles, found by the producer between its loads (in ascending order; of a cut reduction every split-th)
 struct PairLists {
   uint16_t adapter[2][kPairM];
   int count[2];
