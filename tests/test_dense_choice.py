@@ -77,7 +77,8 @@ def test_the_kernel_taken_is_near_the_fastest(plan, kind, T, d, F, us):
 
 def test_a_last_wave_of_few_tiles_is_cut(plan):
     """5000 x 2048 over 5632: 160 tiles on 74 pairs of SMs."""
-    assert plan(DOWN, 5000, 2048, 5632)[:2] == (1, 256) and plan(DOWN, 5000, 2048, 5632)[3] > 1
+    for adapters in (0, 9):
+        assert plan(DOWN, 5000, 2048, 5632, adapters)[:2] == (1, 256) and plan(DOWN, 5000, 2048, 5632, adapters)[3] > 1
 
 
 def test_pieces_of_a_few_rows(lib):

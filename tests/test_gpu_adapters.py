@@ -10,7 +10,9 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["one", "none", "distinct", "runs", "odd"])
 @pytest.mark.parametrize("T,d,out,n,r", [(1, 16, 16, 1, 8), (1, 512, 1408, 4, 16), (5, 272, 144, 3, 24), (8, 512, 400, 5, 128), (13, 528, 144, 20, 40), (33, 64, 272, 40, 8),
                                          (64, 1040, 528, 70, 16), (129, 144, 400, 150, 64), (130, 272, 2064, 9, 128),
-                                         (300, 528, 144, 200, 16), (1021, 1040, 1040, 12, 40), (2100, 512, 1552, 30, 64), (2100, 272, 5632, 300, 16), (1500, 144, 5008, 40, 128)])
+                                         (300, 528, 144, 200, 16), (1021, 1040, 1040, 12, 40), (2100, 512, 1552, 30, 64), (2100, 272, 5632, 300, 16), (1500, 144, 5008, 40, 128),
+                                         # reduced rows by the tensor cores beside the kernel of a few rows; a cut last wave of CTA pairs
+                                         (8, 32768, 512, 3, 128), (5000, 5632, 2048, 9, 16)])
 def test_linear(T, d, out, n, r, kind):
     from ateniaengine_b200 import adapter_linear
     x, w, low, ids = ref.rand(T, 1.0, T, d), ref.rand(1, d ** -0.5, out, d), ref.low_rank(5, n, r, d, out), ref.ids_of(kind, T, n)
@@ -25,7 +27,10 @@ def test_linear(T, d, out, n, r, kind):
 @pytest.mark.parametrize("T,d,F,n,ranks,kind", [(1, 64, 96, 2, (8, 16, 24), "one"), (11, 272, 144, 4, (24, 8, 128), "odd"), (48, 512, 1408, 33, (16, 16, 16), "distinct"),
                                                 (200, 272, 400, 7, (8, 64, 40), "odd"), (1100, 528, 1040, 16, (32, 32, 128), "runs"),
                                                 (1500, 272, 3600, 40, (128, 128, 16), "distinct"), (700, 512, 5632, 50, (96, 40, 64), "odd"),
-                                                (1100, 2048, 5632, 16, (24, 8, 32), "runs")])
+                                                (1100, 2048, 5632, 16, (24, 8, 32), "runs"),
+                                                # two parts of many reduced rows beside the ring, and under the sums of a cut reduction
+                                                (100, 1024, 14336, 6, (128, 128, 16), "distinct"), (128, 2048, 512, 5, (128, 128, 64), "runs"),
+                                                (4, 512, 1408, 3, (128, 64, 128), "distinct")])
 def test_block(T, d, F, n, ranks, kind, parts):
     from ateniaengine_b200 import gated_ffn
     x, w, ids = ref.rand(T, 1.0, T, d), ref.block(3, d, F), ref.ids_of(kind, T, n)
