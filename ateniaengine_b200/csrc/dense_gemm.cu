@@ -42,7 +42,7 @@ struct __align__(8) TileBars {
 };
 
 struct TileArgs {
-  int problems, a_rows, stages, split, b_early, a_early;
+  int problems, a_rows, stages, split, b_early, a_early, next_early;
   int v_bytes;                      // of the reduced rows, ahead of the ring
   int tile_end[kMaxDenseProblems];  // tiles of the problems up to and including this one
   DeviceError* err;
@@ -177,7 +177,10 @@ dense_tile_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (ta.a_early) load_a(kb_begin + i, dst, bar);
       }
     }
-    if (!ta.a_early) chain_wait();
+    if (!ta.a_early) {
+      chain_wait();
+      if (ta.next_early) chain_next();
+    }
     auto load_blocks = [&](int from, int to) {
       for (int kb = from; kb < to; ++kb) {
         const uint32_t bar = smem_u32(&bars.full[stage]), dst = ring + stage * stage_bytes;
@@ -506,6 +509,7 @@ int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t 
   ta.a_rows = g.a_rows;
   ta.b_early = g.b_early;
   ta.a_early = g.a_early && g.b_early;
+  ta.next_early = g.next_early;
   ta.split = split;
   ta.v_bytes = reduced_row_bytes(g);
   // (a ring of two stages at least)

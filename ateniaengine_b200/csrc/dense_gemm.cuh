@@ -67,7 +67,9 @@ struct DenseGemm {
   int a_rows;                    // rows of A a stage holds: of a K-major A's box (dense_a_rows), else 128
   bool chained;                  // see launch_chained
   bool b_early;                  // B is not written by the kernel before: its first tiles are requested before the wait
-  bool a_early;                  // neither is A: only the adapters' v is waited for
+  bool a_early;                  // neither is A: only the adapters' v, and the stores, wait
+  bool next_early;               // what follows reads nothing of this product's: it may start on SMs that this one leaves
+                                 // free (a launch of pairs on all of them does not let it: 4096 tokens, 2048 x 5632 420 / 425 us)
 };
 int launch_dense_gemm(const DenseGemm& g, int num_sms, cudaStream_t s);   // chooses between them
 int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t s);  // dense_gemm.cu

@@ -61,7 +61,7 @@ struct __align__(8) PairBars {
   int abort_flag;
 };
 struct PairArgs {
-  int problems, first, tiles, split, b_early, a_early;  // tiles first .. tiles - 1
+  int problems, first, tiles, split, b_early, a_early, next_early;  // tiles first .. tiles - 1
   int tile_end[kMaxDenseProblems];
   DeviceError* err;
 };
@@ -311,7 +311,10 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         if (pa.a_early) load_a(p, t, kb0 + i, dst, bar);
       }
     }
-    if (!(AD && pa.a_early)) chain_wait();
+    if (!pa.a_early) {
+      chain_wait();
+      if (pa.next_early) chain_next();
+    }
     const std::conditional_t<AD, AdapterRounds<EPI>, NoAdapters> r(ad);
     int it = 0;
     for (int i = pair; ok && i < pa.tiles; i += num_pairs, ++it) {
@@ -404,6 +407,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
         }
       }
     }
+    chain_wait();
     chain_next();  // (every load is on its way: what follows may be launched)
     if (*abort_flag && leader && lane == 0) {
       // let the copies already issued (both CTAs') land before the pair's shared memory is released
@@ -627,7 +631,7 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 }
 
 template <int EPI, bool B_MN, int NP, bool AD>
-int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream_t s) {
+int launch_pairs(const DenseGemm& g, PairArgs pa, int num_sms, cudaStream_t s) {
   auto kernel = dense_pair_kernel<EPI, B_MN, NP, AD>;
   static bool attr_set[kMaxDevices] = {};
   if (first_use_on_current_device(attr_set)) {
@@ -639,6 +643,7 @@ int launch_pairs(const DenseGemm& g, const PairArgs& pa, int num_sms, cudaStream
   if constexpr (AD) ad = *g.adapters;
   const int tiles = pa.tiles - pa.first;
   const int pairs = pa.split > 1 ? tiles * pa.split : num_sms / 2 < tiles ? num_sms / 2 : tiles;
+  pa.next_early = g.next_early && 2 * pairs < num_sms;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2 * pa.split;

@@ -305,6 +305,7 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   g2.epilogue = kDensePlain;
   g2.a_rows = g1.a_rows;
   g2.chained = g2.b_early = true;
+  g2.next_early = true;  // (backward pass of 64 tokens, 512 x 1408 17.8 -> 17.0 us, of 1021, 2048 x 5632 132.4 -> 129.4)
   DenseProblem& p2 = g2.p[0];
   p2.M = T;
   p2.N = d_model;
@@ -321,7 +322,7 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   g3.problems = 3;
   g3.epilogue = kDensePlain;
   g3.a_rows = tc::BM;
-  g3.chained = true;
+  g3.chained = g3.b_early = g3.a_early = true;  // (its operands are older than the kernel before it, which waited for them)
   const void* lhs[3] = {dg, du, dy};
   const void* rhs[3] = {x, x, h};
   void* out[3] = {dw_gate, dw_up, dw_down};
