@@ -41,7 +41,7 @@ def test_block(T, d, F, n, ranks, kind, parts):
     assert torch.equal(y, gated_ffn(x, *w, adapters=sets, adapter_ids=ids))
 
 
-@pytest.mark.parametrize("T,r", [(40, 16), (40, 40), (600, 64)])
+@pytest.mark.parametrize("T,r", [(6, 16), (13, 128), (40, 16), (40, 40), (600, 64)])
 def test_a_broken_adapter_stays_with_its_requests(T, r):
     """NaN and infinities in one adapter's matrices: every other row is as it is without them."""
     from ateniaengine_b200 import adapter_linear, gated_ffn
@@ -109,3 +109,38 @@ def test_beside_the_block_it_adapts():
         ref.assert_within(a, ref.adapter_linear(x, wo, low, ids), "projection")
         ref.assert_within(b, ref.forward(a, *w, sets, ids)[0], "block")
         ref.assert_within(c, ref.adapter_linear(b, wo, low, ids), "second projection")
+
+
+def test_threads_with_streams_of_their_own():
+    """Four host threads, each its own sizes on its own stream, at the same time: the bits that each has alone."""
+    import threading
+    from ateniaengine_b200 import adapter_linear, gated_ffn, gated_ffn_backward
+    d, F, n, r = 528, 1040, 7, 16
+    w, low = ref.block(3, d, F), ref.low_rank(50, n, r, d, d)
+    wo = ref.rand(9, d ** -0.5, d, d)
+
+    def step(x, dy, ids):
+        a = adapter_linear(x, wo, low, ids)
+        y, saved = gated_ffn(a, *w, save=True)
+        return [a, y, *gated_ffn_backward(dy, a, *w, saved)]
+
+    jobs = []
+    for i, T in enumerate((3, 48, 300, 1100)):
+        args = ref.rand(T, 1.0, T, d), ref.rand(T + 1, 1.0, T, d), ref.ids_of("odd" if i % 2 else "runs", T, n, i)
+        jobs.append((args, step(*args)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(args, alone):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = step(*args)
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(not torch.equal(p, q) for p, q in zip(got, alone))
+
+    threads = [threading.Thread(target=run, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(wrong) == 6 * len(jobs) and not any(wrong)
