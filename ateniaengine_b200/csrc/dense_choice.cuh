@@ -124,17 +124,14 @@ inline ReducePlan reduce_plan(int64_t rows, int64_t tiles, int kb, int n, int pe
 // cut that leaves the fewest of the `places` for blocks empty in the last wave, the least one of equals.
 struct RowsPlan {
   int pieces, blocks;
+  double used;  // of the places in all waves
 };
 inline RowsPlan rows_plan(int groups, int steps, int warps, int places) {
-  RowsPlan best{1, (int)dense_ceil(groups, warps)};
-  double best_used = 0;
+  RowsPlan best{1, (int)dense_ceil(groups, warps), 0.0};
   for (int pieces = 1; pieces <= warps && (pieces == 1 || steps >= 2 * pieces); pieces *= 2) {
     const int64_t blocks = dense_ceil(groups, warps / pieces);
     const double used = (double)blocks / (double)(dense_ceil(blocks, places) * places);
-    if (used > 1.01 * best_used) {
-      best_used = used;
-      best = {pieces, (int)blocks};
-    }
+    if (used > 1.01 * best.used) best = {pieces, (int)blocks, used};
   }
   return best;
 }

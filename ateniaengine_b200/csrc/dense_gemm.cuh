@@ -78,8 +78,8 @@ int launch_dense_rows(const DenseGemm& g, int num_sms, cudaStream_t s);   // den
 bool dense_rows_serve(const DenseGemm& g);
 // Up to 8 rows of a matrix of at most 2^25 elements and up to 16 of one of at most 2^23; one row of any.  Operands on 32-byte
 // boundaries, which the kernel's loads want (any row of a matrix is on one if the first is).  B200, block of 16 tokens, this kernel /
-// dense_gemm.cu's, us: 512 x 1408 5.3 / 8.1, 2048 x 2816 12.5 / 14.8, 2048 x 5632 22.4 / 20.5; of eight 5.0 / 7.8, 11.4 / 14.5, 18.9 /
-// 20.1, 4096 x 14336 65.7 / 61.8; of one 61.4 / 61.0.
+// dense_gemm.cu's, us: 512 x 1408 5.3 / 8.1, 2048 x 2816 12.5 / 14.8, 2048 x 5632 22.4 / 20.5; of eight 5.0 / 7.8, 11.4 / 14.5, 18.8 /
+// 20.1, 4096 x 14336 65.7 / 61.8; of one 60.1 / 61.0.
 constexpr int kRowsMost = 16, kRestMost = 8;
 inline bool dense_rows(int64_t M, int64_t N, int64_t K, bool two, const void* x, const void* w0, const void* w1) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w0) | (two ? reinterpret_cast<uintptr_t>(w1) : 0);

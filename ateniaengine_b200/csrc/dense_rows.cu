@@ -26,9 +26,10 @@ using namespace tc;
 constexpr int kVecWarps = 8;
 constexpr int kVecThreads = 32 * kVecWarps;
 constexpr int kStep = 64;  // k of a step: 32 bytes a lane
-// Steps on their way and blocks an SM holds: more of a warp for a matrix that is read in a round or two, more warps for a large one.
-// B200, blocks of one / eight tokens, us: 512 x 1408 4.5 / 4.7 with three steps and two blocks, 5.1 / 5.4 with two and three, 2048 x 5632
-// 19.0 / 19.6 and 17.5 / 19.0, 4096 x 14336 62.0 / 62.5 and 60.4 / 65.7.
+// Steps on their way and blocks an SM holds: more of a warp, or more warps for gate and up of a large matrix, where these fill the last
+// wave about as well.  B200, blocks of one token, all products with three steps and two blocks / gate and up with two and three, us: 512 x
+// 1408 4.5 / 5.1, 2048 x 5632 19.3 / 16.4, 1024 x 16384 31.8 / 26.9, 4096 x 14336 63.5 / 60.8, 4096 x 8192 (filled to 0.87 and 0.77) 36.0 /
+// 38.3.  One product with three steps and two blocks / two and three, four tokens: 4096 x 8192 14.1 / 17.4, 5120 x 5120 13.0 / 13.1.
 template <bool LARGE>
 struct RowsShape {
   static constexpr int kAhead = LARGE ? 2 : 3;
@@ -288,15 +289,14 @@ int launch_rows(const DenseGemm& g, const VecArgs& va, int blocks, cudaStream_t 
 }
 template <int EPI, bool AD>
 int launch_rows_tokens(const DenseGemm& g, const VecArgs& va, bool large, int blocks, cudaStream_t s) {
-  if constexpr (EPI == kDensePlain)
-    if (large && va.x_rest && va.T > 4) return launch_rows<EPI, 2, AD, true>(g, va, blocks, s);
-  if (va.T > 8 || (va.x_rest && va.T > 4)) return launch_rows<EPI, 2, AD, false>(g, va, blocks, s);  // (dense_rows: more than 8 of no large one)
-  return large ? launch_rows<EPI, 1, AD, true>(g, va, blocks, s) : launch_rows<EPI, 1, AD, false>(g, va, blocks, s);
+  // two tiles of eight: more than eight tokens, or more than four in two parts
+  if (va.T > 8 || (va.x_rest && va.T > 4)) return launch_rows<EPI, 2, AD, false>(g, va, blocks, s);
+  if constexpr (EPI == kDenseSwiGLU)
+    if (large) return launch_rows<EPI, 1, AD, true>(g, va, blocks, s);
+  return launch_rows<EPI, 1, AD, false>(g, va, blocks, s);
 }
 
 }  // namespace
-
-static int64_t dense_elements(const DenseGemm& g) { return (int64_t)g.p[0].N * g.p[0].K * (g.epilogue == kDenseSwiGLU ? 2 : 1); }
 
 bool dense_rows_serve(const DenseGemm& g) {
   const DenseProblem& p = g.p[0];
@@ -320,9 +320,11 @@ int launch_dense_rows(const DenseGemm& g, int num_sms, cudaStream_t s) {
   va.x_rest = p.a_rest;
   va.out_rest = p.out_rest;
   const int groups = g.epilogue == kDenseSwiGLU ? p.N / 8 : p.N / 16;
-  const bool large = dense_elements(g) > kLargeElements;
-  const RowsPlan plan = rows_plan(groups, (p.K + kStep - 1) / kStep, kVecWarps,
-                                  (large ? RowsShape<true>::kBlocks : RowsShape<false>::kBlocks) * num_sms);
+  const int steps = (p.K + kStep - 1) / kStep;
+  const RowsPlan few = rows_plan(groups, steps, kVecWarps, RowsShape<false>::kBlocks * num_sms);
+  const RowsPlan many = rows_plan(groups, steps, kVecWarps, RowsShape<true>::kBlocks * num_sms);
+  const bool large = g.epilogue == kDenseSwiGLU && (int64_t)2 * p.N * p.K > kLargeElements && p.M <= 8 && many.used >= 0.92 * few.used;
+  const RowsPlan& plan = large ? many : few;
   const int blocks = plan.blocks;
   va.pieces = plan.pieces;
   count_launch();
