@@ -261,10 +261,8 @@ int launch_adapter_reduce(const AdapterReduce& r, int num_sms, cudaStream_t s) {
   const int stage_bytes = r.a_rows * BK * 2 + kRankRows * BK * 2;
   int stages = kRedRingBytes / stage_bytes;
   if (stages > kRedStages) stages = kRedStages;
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(adapter_reduce_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRedRingBytes + 1024));
-  }
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, adapter_reduce_kernel, kRedRingBytes + 1024)) return rc;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = split;

@@ -658,12 +658,9 @@ constexpr int kFixupMaxRows = 32;  // rows (tokens x top-k) up to which the kern
 
 template <int MODE, bool I8, bool FEW>
 int launch_dec_one(const GroupedGemmArgs& a, int num_sms, cudaStream_t s) {
-  static bool attr_set[kMaxDevices] = {};
+  static FirstUse ready[kMaxDevices];
   constexpr int kSmem = DecRing<I8, FEW>::SMEM_BYTES;
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(grouped_gemm_decode_kernel<MODE, I8, FEW>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  }
+  if (const int rc = allow_shared_memory(ready, grouped_gemm_decode_kernel<MODE, I8, FEW>, kSmem)) return rc;
   // stream-K where a workspace slot can hold every piece (bf16: every group fits one 128-token tile;
   // INT8: tiles are 32 tokens) and the tiles that can exist are too few to balance the SMs
   constexpr int BN_OUT = (MODE == kSwiGLU) ? DROWS : 2 * DROWS;

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "../../include/atenia_moe.h"
+#include "first_use.cuh"
 #include "kernel_choice.cuh"
 #include "pair_tiles.cuh"
 
@@ -37,15 +38,19 @@ void count_launch(int n = 1);
 void count_tcgen05_launch();
 void count_bytes(int which, uint64_t n);
 
-// One-time kernel attributes are per device: `flags` is a per-kernel array indexed by device ordinal.
-// Returns true exactly once per (kernel, device); a benign double set under a race is harmless.
+// Dynamic shared memory above 48 KiB has to be allowed per kernel and device before the first launch there: `of` is a per-kernel
+// array indexed by device ordinal.
 constexpr int kMaxDevices = 64;
-inline bool first_use_on_current_device(bool (&flags)[kMaxDevices]) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return true;
-  if (flags[dev]) return false;
-  flags[dev] = true;
-  return true;
+template <typename K>
+int allow_shared_memory(FirstUse (&of)[kMaxDevices], K* kernel, int bytes) {
+  auto set = [&] {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) (void)cudaGetLastError();  // returned here: not again by the next plain launch's check
+    return (int)e;
+  };
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return set();
+  return of[dev](set);
 }
 
 // ---- chained launches --------------------------------------------------------------------------

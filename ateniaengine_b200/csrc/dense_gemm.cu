@@ -438,10 +438,8 @@ int reduced_row_bytes(const DenseGemm& g) {
 template <int EPI, bool B_MN, int NP, bool AD, int BN>
 int launch_tiles(const DenseGemm& g, TileArgs ta, int tiles, cudaStream_t s) {
   auto kernel = dense_tile_kernel<EPI, B_MN, NP, AD, BN>;
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmemMax));
-  }
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, kernel, kTileSmemMax)) return rc;
   const int rows = g.a_rows;
   const int stage_bytes = rows * BK * 2 + TileSize<BN>::kBBytes;
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};

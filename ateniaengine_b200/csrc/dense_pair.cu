@@ -633,10 +633,8 @@ dense_pair_kernel(const __grid_constant__ Problems<NP> ps, const __grid_constant
 template <int EPI, bool B_MN, int NP, bool AD>
 int launch_pairs(const DenseGemm& g, PairArgs pa, int num_sms, cudaStream_t s) {
   auto kernel = dense_pair_kernel<EPI, B_MN, NP, AD>;
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairSize<EPI>::kSmem));
-  }
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, kernel, PairSize<EPI>::kSmem)) return rc;
   Problems<NP> ps;
   for (int i = 0; i < NP; ++i) ps.p[i] = g.p[i];
   std::conditional_t<AD, DenseAdapters, NoAdapters> ad{};

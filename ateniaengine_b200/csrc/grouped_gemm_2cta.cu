@@ -511,11 +511,8 @@ grouped_gemm_2cta_kernel(const __grid_constant__ PairRowMaps tmaps_x, const CUte
 
 template <int MODE, int TOK, bool EX, typename E>
 int launch_2cta_form(const GroupedGemmArgs& a, int num_sms, cudaStream_t s, const E& ex) {
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(grouped_gemm_2cta_kernel<MODE, TOK, EX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         PairRing<TOK>::SMEM_BYTES));
-  }
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, grouped_gemm_2cta_kernel<MODE, TOK, EX>, PairRing<TOK>::SMEM_BYTES)) return rc;
   const int grid = num_sms & ~1;  // whole pairs
   return launch_chained(a.chained, grouped_gemm_2cta_kernel<MODE, TOK, EX>, dim3(grid), dim3(NUM_THREADS2),
                         PairRing<TOK>::SMEM_BYTES, s, *a.pair_rows, a.tmap_b0, MODE == kSwiGLU ? a.tmap_b1 : a.tmap_b0,

@@ -320,11 +320,8 @@ grouped_gemm_pair_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const 
 
 template <int MODE>
 int launch_pair_rows_one(const GroupedGemmArgs& a, int num_sms, cudaStream_t s) {
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(grouped_gemm_pair_rows_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         SMEM_BYTES2));
-  }
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, grouped_gemm_pair_rows_kernel<MODE>, SMEM_BYTES2)) return rc;
   const int grid = num_sms & ~1;  // whole pairs
   return launch_chained(a.chained, grouped_gemm_pair_rows_kernel<MODE>, dim3(grid), dim3(NUM_THREADS2), SMEM_BYTES2, s, a.tmap_a,
                         a.tmap_b0, MODE == kSwiGLU ? a.tmap_b1 : a.tmap_b0, a.group_offsets, a.num_groups, a.N, a.K,

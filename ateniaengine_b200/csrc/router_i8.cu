@@ -558,9 +558,8 @@ __global__ void __launch_bounds__(256) router_digits_kernel(const float* __restr
 
 template <int CTAS>
 int launch_form(const RouterArgs& a, cudaStream_t s) {
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set))
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(router_i8_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, R_SMEM));
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, router_i8_kernel<CTAS>, R_SMEM)) return rc;
   router_i8_kernel<CTAS><<<(a.T + RM - 1) / RM * CTAS, R_THREADS, R_SMEM, s>>>(a, *a.digit_map, a.digit_scale);
   return (int)cudaGetLastError();
 }

@@ -333,11 +333,8 @@ grouped_gemm_w8_m256_kernel(const __grid_constant__ CUtensorMap tmap_a, const CU
 
 template <int MODE>
 int launch_m256_one(const GroupedGemmArgs& a, int num_sms, cudaStream_t s) {
-  static bool attr_set[kMaxDevices] = {};
-  if (first_use_on_current_device(attr_set)) {
-    ATENIA_CUDA_TRY(cudaFuncSetAttribute(grouped_gemm_w8_m256_kernel<MODE>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, M_SMEM_BYTES));
-  }
+  static FirstUse ready[kMaxDevices];
+  if (const int rc = allow_shared_memory(ready, grouped_gemm_w8_m256_kernel<MODE>, M_SMEM_BYTES)) return rc;
   grouped_gemm_w8_m256_kernel<MODE><<<dim3(num_sms), dim3(M_THREADS), M_SMEM_BYTES, s>>>(
       a.tmap_a, a.tmap_b0, MODE == kSwiGLU ? a.tmap_b1 : a.tmap_b0, a.group_offsets, a.num_groups, a.N, a.K, a.out,
       a.scale0, a.scale1, a.err);
