@@ -461,18 +461,18 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 static EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
+  static FirstUse found;
+  static std::atomic<EncodeTiledFn> fn{nullptr};
+  found([] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-    }
-  }
-  return fn;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+    if (e != cudaSuccess) (void)cudaGetLastError();  // (the caller returns ATENIA_ERR_DRIVER)
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess) return 1;
+    fn.store(reinterpret_cast<EncodeTiledFn>(p), std::memory_order_relaxed);
+    return 0;
+  });
+  return fn.load(std::memory_order_relaxed);
 }
 
 int encode_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
