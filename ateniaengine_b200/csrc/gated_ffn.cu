@@ -11,13 +11,15 @@
 #include <mutex>
 
 #include "dense_gemm.cuh"
+#include "error_word.cuh"
 
 namespace atenia {
 
 namespace {
 
 static __device__ DeviceError g_dense_error;
-std::mutex g_mu;
+static __device__ DeviceError g_taken_error;  // by a check
+std::mutex g_mu, g_check_mu[kMaxDevices];
 DeviceError* g_error_addr[kMaxDevices] = {};
 int g_sms[kMaxDevices] = {};
 
@@ -381,15 +383,16 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
 
 int atenia_ffn_check(void* stream) {
   using namespace atenia;
-  DeviceError* err = nullptr;
-  int rc = dense_error_word(&err);
+  DeviceError* word = nullptr;
+  int rc = dense_error_word(&word);
   if (rc) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int dev = -1;
+  void* taken = nullptr;
+  ATENIA_CUDA_TRY(cudaGetDevice(&dev));
+  ATENIA_CUDA_TRY(cudaGetSymbolAddress(&taken, g_taken_error));
   DeviceError e{};
-  ATENIA_CUDA_TRY(cudaMemcpyAsync(&e, err, sizeof e, cudaMemcpyDeviceToHost, s));
-  ATENIA_CUDA_TRY(cudaStreamSynchronize(s));
-  if (e.code) ATENIA_CUDA_TRY(cudaMemsetAsync(err, 0, sizeof e, s));
-  return e.code;
+  rc = take_device_error(word, static_cast<DeviceError*>(taken), g_check_mu[dev], static_cast<cudaStream_t>(stream), &e);
+  return rc ? rc : e.code;
 }
 
 }  // extern "C"

@@ -474,7 +474,8 @@ ATENIA_API uint64_t atenia_adapter_linear_workspace_bytes(int T, int rank);
 ATENIA_API int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, int d_out, const AteniaLowRank* adapter,
                                      const int32_t* ids, int n, void* y, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Waits for the stream and returns the first error that kernels of the calls above recorded on this device since the last check
- * (ATENIA_ERR_DEVICE_TIMEOUT: a bounded wait gave up); the word is cleared. */
+ * (ATENIA_ERR_DEVICE_TIMEOUT: a bounded wait gave up), and clears it.  The word is the device's, not the stream's: of several checks one
+ * returns an error, whichever stream it came from. */
 ATENIA_API int atenia_ffn_check(void* stream);
 
 /* ---- expert parallelism ------------------------------------------------------------------- */
