@@ -172,12 +172,16 @@ uint64_t atenia_gated_ffn_workspace_bytes(int T, int d_model, int d_ff, const At
   const uint64_t rows = align256((uint64_t)T * d_ff * 2);
   if (backward) return 3 * rows;  // dg, du, h
   uint64_t n = h_bytes(T, d_ff);
-  if (adapters) n += reduced_bytes(T, adapters->gate.rank) + reduced_bytes(T, adapters->up.rank) + reduced_bytes(T, adapters->down.rank);
+  if (adapters)
+    for (const AteniaLowRank* a : {&adapters->gate, &adapters->up, &adapters->down}) {
+      if (a->rank != 0 && !rank_ok(a->rank)) return 0;
+      n += reduced_bytes(T, a->rank);
+    }
   return n;
 }
 
 uint64_t atenia_adapter_linear_workspace_bytes(int T, int rank) {
-  return T < 0 || !atenia::rank_ok(rank) ? 0 : atenia::reduced_bytes(T, rank);
+  return T < 0 || T > atenia::kMaxRows || !atenia::rank_ok(rank) ? 0 : atenia::reduced_bytes(T, rank);
 }
 
 int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up, const void* w_down, int T, int d_model, int d_ff,
