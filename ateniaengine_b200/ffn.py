@@ -17,6 +17,7 @@ from .moe import _launching
 
 BF16 = torch.bfloat16
 _PARTS = {"gate", "up", "down"}
+_MAX_ROWS, _MAX_WIDTH = 1 << 24, 1 << 20  # (the library's sizes are 32 bits: larger ones would come to it as others)
 
 
 class LowRankAdapters(NamedTuple):
@@ -48,6 +49,8 @@ def _rows(x, name="x"):
         raise TypeError(f"{name} must be a bf16 tensor")
     if x.dim() != 2:
         raise ValueError(f"{name} must be [tokens, width], got {tuple(x.shape)}")
+    if x.shape[0] > _MAX_ROWS:
+        raise ValueError(f"{name}: at most 2^24 tokens, got {x.shape[0]}")
     if not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     return x if x.is_contiguous() else x.contiguous()
@@ -100,13 +103,26 @@ def _workspace(nbytes, x):
     return x.new_empty(nbytes // 2 or 1)  # (bf16 elements; the sizes are multiples of 256)
 
 
+def _check_widths(a, b, what):
+    if a < 16 or b < 16 or a % 16 or b % 16 or a > _MAX_WIDTH or b > _MAX_WIDTH:
+        raise ValueError(f"{what} must be multiples of 16, at most 2^20, got {a} and {b}")
+
+
+def _projection(x, weight):
+    """in, out and the checked weight [out, in] of adapter_linear."""
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be [out, in]")
+    n_in, n_out = x.shape[1], weight.shape[0]
+    _check_widths(n_in, n_out, "the projection's sizes")
+    return n_in, n_out, _operand(weight, "weight", (n_out, n_in), BF16, x.device)
+
+
 def _block(x, gate, up, down):
     if not isinstance(gate, torch.Tensor) or gate.dim() != 2:
         raise ValueError("gate must be [d_ff, d_model]")
     T, d = x.shape
     F = gate.shape[0]
-    if d < 16 or F < 16 or d % 16 or F % 16:
-        raise ValueError(f"d_model and d_ff must be multiples of 16, got {d} and {F}")
+    _check_widths(d, F, "d_model and d_ff")
     return (T, d, F, _operand(gate, "gate", (F, d), BF16, x.device), _operand(up, "up", (F, d), BF16, x.device),
             _operand(down, "down", (d, F), BF16, x.device))
 
@@ -136,7 +152,7 @@ def _block_adapters(adapters, adapter_ids, T, d, F, save, device):
 
 
 def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, out=None, sync=False):
-    """y = (silu(x gate^T) * (x up^T)) down^T.  x: CUDA bf16 [T, d], any T; gate, up: bf16 [F, d]; down: bf16 [d, F].
+    """y = (silu(x gate^T) * (x up^T)) down^T.  x: CUDA bf16 [T, d], T up to 2^24; gate, up: bf16 [F, d]; down: bf16 [d, F].
 
     `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
     the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
@@ -192,13 +208,8 @@ def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
     adapters of many requests.  x: CUDA bf16 [T, in]; weight: bf16 [out, in]; adapters: LowRankAdapters; adapter_ids: int32 [T].
     `out` must not overlap x."""
     x = _rows(x)
-    T, n_in = x.shape
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
-        raise ValueError("weight must be [out, in]")
-    n_out = weight.shape[0]
-    if n_in < 16 or n_out < 16 or n_in % 16 or n_out % 16:
-        raise ValueError(f"the projection's sizes must be multiples of 16, got {n_out} x {n_in}")
-    weight = _operand(weight, "weight", (n_out, n_in), BF16, x.device)
+    T = x.shape[0]
+    n_in, n_out, weight = _projection(x, weight)
     ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, x.device)
     low, n, keep = _low_rank(adapters, "adapters", n_in, n_out, x.device)
     y = _output(out, (T, n_out), x)
