@@ -148,6 +148,8 @@ def _block_adapters(adapters, adapter_ids, T, d, F, save, device):
         fields += low
         ranks.append(low[3])
         keep.append(tensors)
+    if n == 0:
+        raise ValueError("adapter_ids without adapters")
     return _FFN_ADAPTERS.pack(*fields, ids.data_ptr(), n, 0), ranks, keep
 
 

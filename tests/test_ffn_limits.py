@@ -62,3 +62,11 @@ def test_python_entries_refuse_sizes_that_the_library_does_not_take():
             ffn._projection(z(4, 16), z(wide, 16))
         with pytest.raises(ValueError, match="at most"):
             ffn._projection(z(4, wide), z(16, wide))
+
+
+@pytest.mark.parametrize("adapters", [{"gate": None}, {"gate": None, "up": None, "down": None}])
+def test_a_dict_of_no_adapters_is_refused_in_python(adapters):
+    import torch
+    from ateniaengine_b200 import ffn
+    with pytest.raises(ValueError, match="without adapters"):
+        ffn._block_adapters(adapters, torch.zeros(4, dtype=torch.int32), 4, 64, 96, False, torch.device("cpu"))
