@@ -38,9 +38,24 @@ constexpr int kMaxAdapters = ATENIA_ADAPTER_MAX_COUNT;
 
 uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + nb && y < x + na;
+struct Range {
+  const void* p;  // (null: none)
+  uint64_t bytes;
+};
+bool overlap(const Range& a, const Range& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+}
+// Does an output lie over an input or over another output?
+template <int O, int I>
+bool overlap_any(const Range (&outs)[O], const Range (&ins)[I]) {
+  for (int i = 0; i < O; ++i) {
+    for (const Range& in : ins)
+      if (overlap(outs[i], in)) return true;
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return true;
+  }
+  return false;
 }
 int kblocks(int64_t k) { return (int)((k + tc::BK - 1) / tc::BK); }
 
@@ -77,6 +92,16 @@ int check_adapter(const AteniaLowRank& a) {
   if (!aligned16(a.a) || !aligned16(a.b)) return ATENIA_ERR_SHAPE;
   return ATENIA_OK;
 }
+// What a projection's adapters are read from
+struct AdapterRanges {
+  Range a, b, scale;
+  AdapterRanges(const AteniaLowRank* s, int64_t in, int64_t out, int n) : a{}, b{}, scale{} {
+    if (!s || s->rank == 0) return;
+    a = {s->a, (uint64_t)n * s->rank * in * 2};
+    b = {s->b, (uint64_t)n * s->rank * out * 2};
+    scale = {s->scale, (uint64_t)n * 4};
+  }
+};
 // (room for two parts: the calls that ask for the size do not all know the width that decides)
 uint64_t reduced_bytes(int64_t T, int rank) { return rank > 0 ? align256((uint64_t)T * rank * 4) : 0; }
 
@@ -196,7 +221,20 @@ int atenia_gated_ffn_forward(const void* x, const void* w_gate, const void* w_up
   if (!x || !y || !workspace) return ATENIA_ERR_NULL;
   for (const void* p : {x, w_gate, w_up, w_down, (const void*)y, (const void*)saved_gate, (const void*)saved_up, (const void*)workspace})
     if (!aligned16(p)) return ATENIA_ERR_SHAPE;
-  if (workspace_bytes < atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, adapters, 0)) return ATENIA_ERR_CAPACITY;
+  const uint64_t need = atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, adapters, 0);
+  if (workspace_bytes < need) return ATENIA_ERR_CAPACITY;
+  {
+    const uint64_t row = (uint64_t)T * d_model * 2, weight = (uint64_t)d_model * d_ff * 2, kept = (uint64_t)T * d_ff * 4;
+    const int n = adapters ? adapters->n : 0;
+    const AdapterRanges gate(adapters ? &adapters->gate : nullptr, d_model, d_ff, n), up(adapters ? &adapters->up : nullptr, d_model, d_ff, n),
+        down(adapters ? &adapters->down : nullptr, d_ff, d_model, n);
+    const Range outs[4] = {{y, row}, {saved_gate, kept}, {saved_up, kept}, {workspace, need}};
+    const Range ins[13] = {{w_gate, weight}, {w_up, weight}, {w_down, weight}, gate.a, gate.b, gate.scale, up.a, up.b, up.scale,
+                           down.a, down.b, down.scale, {adapters ? adapters->ids : nullptr, (uint64_t)T * 4}};
+    if (overlap_any(outs, ins)) return ATENIA_ERR_SHAPE;
+    for (int i = 1; i < 4; ++i)  // (y may be x: the products that write it read h)
+      if (overlap(outs[i], {x, row})) return ATENIA_ERR_SHAPE;
+  }
   int sms = 0;
   if ((rc = num_sms_of_current_device(&sms))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -267,18 +305,13 @@ int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate,
   for (const void* p : {dy, x, w_gate, w_up, w_down, (const void*)saved_gate, (const void*)saved_up, (const void*)dx, (const void*)dw_gate,
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!aligned16(p)) return ATENIA_ERR_SHAPE;
-  if (workspace_bytes < atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, nullptr, 1)) return ATENIA_ERR_CAPACITY;
-  const uint64_t row = (uint64_t)T * d * 2, weight = (uint64_t)d * F * 2, kept = (uint64_t)T * F * 4;
-  const struct {
-    const void* p;
-    uint64_t bytes;
-  } outs[4] = {{dx, row}, {dw_gate, weight}, {dw_up, weight}, {dw_down, weight}},
-    ins[7] = {{dy, row}, {x, row}, {w_gate, weight}, {w_up, weight}, {w_down, weight}, {saved_gate, kept}, {saved_up, kept}};
-  for (int i = 0; i < 4; ++i) {
-    for (const auto& in : ins)
-      if (overlap(outs[i].p, outs[i].bytes, in.p, in.bytes)) return ATENIA_ERR_SHAPE;
-    for (int j = 0; j < i; ++j)
-      if (overlap(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return ATENIA_ERR_SHAPE;
+  const uint64_t need = atenia_gated_ffn_workspace_bytes(T, d_model, d_ff, nullptr, 1);
+  if (workspace_bytes < need) return ATENIA_ERR_CAPACITY;
+  {
+    const uint64_t row = (uint64_t)T * d * 2, weight = (uint64_t)d * F * 2, kept = (uint64_t)T * F * 4;
+    const Range outs[5] = {{dx, row}, {dw_gate, weight}, {dw_up, weight}, {dw_down, weight}, {workspace, need}};
+    const Range ins[7] = {{dy, row}, {x, row}, {w_gate, weight}, {w_up, weight}, {w_down, weight}, {saved_gate, kept}, {saved_up, kept}};
+    if (overlap_any(outs, ins)) return ATENIA_ERR_SHAPE;
   }
   int sms = 0;
   if ((rc = num_sms_of_current_device(&sms))) return rc;
@@ -360,8 +393,14 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   if (!x || !ids || !y || !workspace) return ATENIA_ERR_NULL;
   for (const void* p : {x, weight, (const void*)y, (const void*)workspace})
     if (!aligned16(p)) return ATENIA_ERR_SHAPE;
-  if (overlap(x, (uint64_t)T * d_in * 2, y, (uint64_t)T * d_out * 2)) return ATENIA_ERR_SHAPE;
-  if (workspace_bytes < atenia_adapter_linear_workspace_bytes(T, adapter->rank)) return ATENIA_ERR_CAPACITY;
+  const uint64_t need = atenia_adapter_linear_workspace_bytes(T, adapter->rank);
+  if (workspace_bytes < need) return ATENIA_ERR_CAPACITY;
+  {
+    const AdapterRanges ad(adapter, d_in, d_out, n);
+    const Range outs[2] = {{y, (uint64_t)T * d_out * 2}, {workspace, need}};
+    const Range ins[6] = {{x, (uint64_t)T * d_in * 2}, {weight, (uint64_t)d_in * d_out * 2}, ad.a, ad.b, ad.scale, {ids, (uint64_t)T * 4}};
+    if (overlap_any(outs, ins)) return ATENIA_ERR_SHAPE;
+  }
   int sms = 0;
   if ((rc = num_sms_of_current_device(&sms))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

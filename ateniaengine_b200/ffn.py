@@ -158,7 +158,7 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
 
     `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
     the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
-    [2, F / 4, T, 4], the two projections before the activation.  `out` may be x.  `sync=True` waits and raises what the kernels recorded."""
+    [2, F / 4, T, 4], the two projections before the activation.  `out` may be x, and overlaps nothing else that is read.  `sync=True` waits and raises what the kernels recorded."""
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     ad, ranks = None, (0, 0, 0)
@@ -208,7 +208,7 @@ def gated_ffn_backward(dy, x, gate, up, down, saved, sync=False):
 def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
     """y = x weight^T + scale[i] * (x A_i^T) B_i^T with i = adapter_ids[t], outside [0, n) for none: one shared projection with the
     adapters of many requests.  x: CUDA bf16 [T, in]; weight: bf16 [out, in]; adapters: LowRankAdapters; adapter_ids: int32 [T].
-    `out` must not overlap x."""
+    `out` must not overlap what is read."""
     x = _rows(x)
     T = x.shape[0]
     n_in, n_out, weight = _projection(x, weight)

@@ -427,7 +427,8 @@ ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
 /* ---- dense gated feed-forward block, its backward pass, low-rank adapters ------------------- */
 
 /* y = (silu(x Wg^T) * (x Wu^T)) Wd^T for the dense layers beside the MoE ones.  x [T, d_model], w_gate and w_up [d_ff, d_model],
- * w_down [d_model, d_ff], y [T, d_model]: device, bf16, row-major; y may be x.  The sums are f32; h = silu(g) u is rounded to bf16
+ * w_down [d_model, d_ff], y [T, d_model]: device, bf16, row-major; y may be x, else no output (the workspace among them) overlaps
+ * an input or another output (ATENIA_ERR_SHAPE).  The sums are f32; h = silu(g) u is rounded to bf16
  * between the products (of up to 8 tokens, what that leaves is multiplied too where the call's kernels can).  d_model and d_ff are multiples of 16 (at most 2^20), T at most 2^24 (0 is allowed); matrices and the workspace are
  * 16-byte aligned (else ATENIA_ERR_SHAPE).  `workspace` (device) has at least the bytes the size function returns (else
  * ATENIA_ERR_CAPACITY); its content need not be kept between calls, and calls that may run at the same time, captured ones
@@ -463,13 +464,14 @@ ATENIA_API int atenia_gated_ffn_forward(const void* x, const void* w_gate, const
                                         void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients of the block without adapters, from dy [T, d_model] and what the forward call saved: dx [T, d_model], dw_gate and
  * dw_up [d_ff, d_model], dw_down [d_model, d_ff], bf16, all written (none is added to; zero for T = 0).  dg, du and h are rounded
- * to bf16 as operands of the second products.  Nothing saved is changed: the call can be repeated.  No output overlaps
- * an input or another output (ATENIA_ERR_SHAPE). */
+ * to bf16 as operands of the second products.  Nothing saved is changed: the call can be repeated.  No output, the
+ * workspace among them, overlaps an input or another output (ATENIA_ERR_SHAPE). */
 ATENIA_API int atenia_gated_ffn_backward(const void* dy, const void* x, const void* w_gate, const void* w_up, const void* w_down,
                                          const float* saved_gate, const float* saved_up, int T, int d_model, int d_ff, void* dx,
                                          void* dw_gate, void* dw_up, void* dw_down, void* workspace, uint64_t workspace_bytes,
                                          void* stream);
-/* y = x W^T plus the tokens' adapters: any one projection (W [d_out, d_in]).  y does not overlap x (ATENIA_ERR_SHAPE). */
+/* y = x W^T plus the tokens' adapters: any one projection (W [d_out, d_in]).  Neither y nor the workspace overlaps what is read
+ * (ATENIA_ERR_SHAPE). */
 ATENIA_API uint64_t atenia_adapter_linear_workspace_bytes(int T, int rank);
 ATENIA_API int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, int d_out, const AteniaLowRank* adapter,
                                      const int32_t* ids, int n, void* y, void* workspace, uint64_t workspace_bytes, void* stream);

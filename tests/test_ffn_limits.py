@@ -3,6 +3,8 @@ import ctypes as C
 
 import pytest
 
+from test_ffn_refusals import _backward, _forward, _linear
+
 P = 1 << 20  # an aligned address that nothing reads
 
 
@@ -70,3 +72,64 @@ def test_a_dict_of_no_adapters_is_refused_in_python(adapters):
     from ateniaengine_b200 import ffn
     with pytest.raises(ValueError, match="without adapters"):
         ffn._block_adapters(adapters, torch.zeros(4, dtype=torch.int32), 4, 64, 96, False, torch.device("cpu"))
+
+
+def _over(call, lib, sizes, out, other):
+    """The call with `out` on `other`, and with it on its last 16 bytes; everything else apart."""
+    apart = {name: P + (i << 24) for i, name in enumerate(sizes)}
+    return [call(lib, **{**apart, out: apart[other] + at}) for at in (0, (sizes[other] - 1) // 16 * 16)]
+
+
+def test_outputs_of_the_block_over_what_it_reads_or_writes(lib):
+    """T = 4, d = 64, F = 96.  (The output over x is allowed and not called here: the addresses are nobody's.)"""
+    kept, w = 4 * 96 * 4, 64 * 96 * 2
+    need = lib.atenia_gated_ffn_workspace_bytes(4, 64, 96, None, 0)
+    sizes = dict(x=512, gate=w, up=w, down=w, y=512, sg=kept, su=kept, ws=need)
+    for out, others in (("y", ("gate", "up", "down", "sg", "su", "ws")), ("sg", ("x", "gate", "up", "down", "y", "su", "ws")),
+                        ("su", ("x", "gate", "up", "down", "y", "sg", "ws")), ("ws", ("x", "gate", "up", "down", "y", "sg", "su"))):
+        for other in others:
+            assert _over(_forward, lib, sizes, out, other) == [-2, -2], (out, other)
+
+
+def test_outputs_of_the_block_over_its_adapters(lib):
+    from ateniaengine_b200 import _lib
+    n, r, T, d, F = 3, 16, 4, 64, 96
+    places, sizes = {}, {}
+    for i, part in enumerate(("gate", "up", "down")):
+        n_in, n_out = (F, d) if part == "down" else (d, F)
+        for j, (name, size) in enumerate((("a", n * r * n_in * 2), ("b", n * r * n_out * 2), ("scale", n * 4))):
+            places[part, name], sizes[part, name] = (1 << 30) + ((3 * i + j) << 20), size
+    sets = {p: _lib.LowRank(rank=r, **{k: places[p, k] for k in ("a", "b", "scale")}) for p in ("gate", "up", "down")}
+    ad = _lib.FfnAdapters(ids=(1 << 30) + (10 << 20), n=n, **sets)
+    places["ids"], sizes["ids"] = ad.ids, T * 4
+    apart = {name: P + (i << 24) for i, name in enumerate(("x", "gate", "up", "down", "y", "ws"))}
+    for other in places:
+        for out in ("y", "ws"):
+            for at in (0, (sizes[other] - 1) // 16 * 16):
+                assert _forward(lib, adapters=C.byref(ad), **{**apart, out: places[other] + at}) == -2, (out, other, at)
+
+
+def test_workspace_of_the_backward_pass_over_its_operands(lib):
+    w, kept = 12288, 1536
+    sizes = dict(dy=512, x=512, gate=w, up=w, down=w, sg=kept, su=kept, dx=512, dg=w, du=w, dd=w,
+                 ws=lib.atenia_gated_ffn_workspace_bytes(4, 64, 96, None, 1))
+    for other in sizes:
+        if other != "ws":
+            assert _over(_backward, lib, sizes, "ws", other) == [-2, -2], other
+
+
+def test_output_of_the_projection_over_what_it_reads(lib):
+    """T = 4, 64 -> 96, two adapters of rank 8."""
+    from ateniaengine_b200 import _lib
+    low = dict(a=2 * 8 * 64 * 2, b=2 * 8 * 96 * 2, scale=8)
+    at = {name: (1 << 30) + (i << 20) for i, name in enumerate(low)}
+    sizes = dict(x=512, w=12288, ids=16, y=768, ws=lib.atenia_adapter_linear_workspace_bytes(4, 8))
+    for out in ("y", "ws"):
+        for other in sizes:
+            if other != out:
+                call = lambda lib, **kw: _linear(lib, low=_lib.LowRank(rank=8, **at), **kw)
+                assert _over(call, lib, sizes, out, other) == [-2, -2], (out, other)
+        for name in low:
+            apart = {k: P + (i << 24) for i, k in enumerate(sizes)}
+            for shift in (0, (low[name] - 1) // 16 * 16):
+                assert _linear(lib, low=_lib.LowRank(rank=8, **at), **{**apart, out: at[name] + shift}) == -2, (out, name)
