@@ -27,6 +27,10 @@ struct DensePlan {
   int tail_split;  // pairs: of the tiles behind the last whole wave
 };
 
+// Tiles of a launch, times the CTAs or pairs that share one, at most: grids and tile indices are 32 bits.  No plan of sizes that the entry
+// points take has more (2^24 rows of 2^20 columns of gate and up are 2^29 pair tiles).
+constexpr int64_t kDenseMostTiles = (int64_t)1 << 29;
+
 inline int64_t dense_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // rows: of A a stage holds (128 = all); two_columns: gate and up of a feature (kDenseSwiGLU); grad: kDenseGateGrad; full_rows: the

@@ -498,7 +498,7 @@ int launch_dense_tiles(const DenseGemm& g, int columns, int split, cudaStream_t 
   for (int i = 0; i < g.problems; ++i) {
     const DenseProblem& p = g.p[i];
     tiles += (int64_t)((p.M + BM - 1) / BM) * ((p.N + n_out - 1) / n_out);
-    if (tiles * split > (1 << 28)) return ATENIA_ERR_SHAPE;
+    if (tiles * split > kDenseMostTiles) return ATENIA_ERR_SHAPE;
     if (p.kb < split) return ATENIA_ERR_SHAPE;
     ta.tile_end[i] = (int)tiles;
   }

@@ -700,7 +700,7 @@ int launch_dense_pairs(const DenseGemm& g, int split, int tail_split, int num_sm
   for (int i = 0; i < g.problems; ++i) {
     const DenseProblem& p = g.p[i];
     tiles += (int64_t)((p.M + kPairM - 1) / kPairM) * ((p.N + n_out - 1) / n_out);
-    if (tiles > (1 << 26) || p.kb < split || p.kb < tail_split) return ATENIA_ERR_SHAPE;
+    if (tiles * split > kDenseMostTiles || p.kb < split || p.kb < tail_split) return ATENIA_ERR_SHAPE;
     pa.tile_end[i] = (int)tiles;
   }
   if (tiles == 0) return ATENIA_OK;

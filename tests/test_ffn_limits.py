@@ -133,3 +133,30 @@ def test_output_of_the_projection_over_what_it_reads(lib):
             apart = {k: P + (i << 24) for i, k in enumerate(sizes)}
             for shift in (0, (low[name] - 1) // 16 * 16):
                 assert _linear(lib, low=_lib.LowRank(rank=8, **at), **{**apart, out: at[name] + shift}) == -2, (out, name)
+
+
+def test_no_product_of_allowed_sizes_has_more_tiles_than_a_launch_takes(tmp_path):
+    """Or it would be refused behind products that have run."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    so = tmp_path / "libdenselimits.so"
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", os.path.join(root, "tests", "dense_limits_probe.cpp"), "-o", str(so)])
+    probe = C.CDLL(str(so))
+    probe.limits_work_items.restype = probe.limits_most.restype = C.c_longlong
+    most = probe.limits_most()
+    assert most * 2 < 1 << 31  # (two CTAs a pair)
+    widths = [16, 48, 64, 80, 128, 144, 256, 272, 1024, 1 << 14, 1 << 17, (1 << 20) - 16, 1 << 20]
+    seen = 0
+    for T in (1, 17, 127, 128, 129, 4096, (1 << 20) + 1, 1 << 22, (1 << 24) - 1, 1 << 24):
+        for d in widths:
+            for F in widths:
+                blocks = [-(-v // 64) for v in (T, d, F)]
+                few, gw = min(128, -(-T // 8) * 8), [F, d, blocks[0], F, d, blocks[0], d, F, blocks[0]]
+                for sizes, rows, two, grad, adapters in (([T, F, blocks[1]], few, 1, 0, (0, 1, 65536)), ([T, d, blocks[2]], few, 0, 0, (0, 1, 65536)),
+                                                         ([T, F, blocks[1]], few, 0, 1, (0,)), ([T, d, 2 * blocks[2]], few, 0, 0, (0,)), (gw, 128, 0, 0, (0,))):
+                    for n in adapters:
+                        items = probe.limits_work_items((C.c_longlong * 9)(*sizes), len(sizes) // 3, rows, two, grad, n)
+                        assert items <= most, (T, d, F, two, grad, n, items)
+                        seen = max(seen, items)
+    assert seen > 1 << 28  # (the sizes do come near it)
