@@ -3,7 +3,8 @@
 The dense counterpart of an MoE layer's expert (gate, up, SwiGLU, down) for the layers of a model that have no router, for training
 it, and for serving it with one adapter per request.  Every computation runs in the CUDA library; torch owns the memory (the
 calls take their workspace from its allocator, on the current stream) and nothing is recorded for torch's autograd: a training
-step calls `gated_ffn_backward` itself.
+step calls `gated_ffn_backward` itself, or wraps the two calls in a torch.autograd.Function of its own.  An x that requires a gradient is
+refused while torch records.
 """
 import ctypes as C
 import functools
@@ -54,6 +55,14 @@ def _rows(x, name="x"):
     if not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     return x if x.is_contiguous() else x.contiguous()
+
+
+def _check_unrecorded(x):
+    """The result has no history: where x has one, its gradient would be lost without a word.  (Parameters are ordinary arguments: a
+    program that calls gated_ffn_backward itself passes them.)"""
+    if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
+        raise ValueError("x requires a gradient, which this call does not record: detach it, call under torch.no_grad(), or from a "
+                         "torch.autograd.Function")
 
 
 def _output(out, shape, x):
@@ -154,11 +163,12 @@ def _block_adapters(adapters, adapter_ids, T, d, F, save, device):
 
 
 def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, out=None, sync=False):
-    """y = (silu(x gate^T) * (x up^T)) down^T.  x: CUDA bf16 [T, d], T up to 2^24; gate, up: bf16 [F, d]; down: bf16 [d, F].
+    """y = (silu(x gate^T) * (x up^T)) down^T, not recorded for autograd.  x: CUDA bf16 [T, d], T up to 2^24; gate, up: bf16 [F, d]; down: bf16 [d, F].
 
     `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
     the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
     [2, F / 4, T, 4], the two projections before the activation.  `out` may be x, and overlaps nothing else that is read.  `sync=True` waits and raises what the kernels recorded."""
+    _check_unrecorded(x)
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     ad, ranks = None, (0, 0, 0)
@@ -209,6 +219,7 @@ def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
     """y = x weight^T + scale[i] * (x A_i^T) B_i^T with i = adapter_ids[t], outside [0, n) for none: one shared projection with the
     adapters of many requests.  x: CUDA bf16 [T, in]; weight: bf16 [out, in]; adapters: LowRankAdapters; adapter_ids: int32 [T].
     `out` must not overlap what is read."""
+    _check_unrecorded(x)
     x = _rows(x)
     T = x.shape[0]
     n_in, n_out, weight = _projection(x, weight)
