@@ -56,17 +56,22 @@ int allow_shared_memory(FirstUse (&of)[kMaxDevices], K* kernel, int bytes) {
 // ---- chained launches --------------------------------------------------------------------------
 // The kernels of a forward are launched so that each may start while the one before it on the stream still runs
 // (programmatic dependent launch).  Every kernel launched with launch_chained therefore calls chain_wait() before it
-// touches global memory at all: it returns once the kernel before has completed and its stores are visible -- and that
+// touches global memory, three exceptions apart: it returns once the kernel before has completed and its stores are visible -- and that
 // one's chain_wait() has waited for the kernel before it, so nothing earlier is in flight either.  chain_next() lets
 // the next kernel's blocks start: what overlaps is its launch, not its work.  Kernels without chain_wait() are
 // launched plainly and wait for everything before them as usual.
-// Two exceptions.  The cluster router requests rows of the layer's own copies of the router matrix and the gate vector, which
+// The exceptions.  The cluster router requests rows of the layer's own copies of the router matrix and the gate vector, which
 // no kernel writes (set_weights synchronises).  And a GEMM takes the group offsets and requests its first weight tiles before
 // its chain_wait().  The kernel before it writes neither (it gathers rows, makes digits, or is the GEMM before) and comes to
 // chain_next() only past its own chain_wait() -- or, between two GEMMs, was launched by one that had passed its -- so
 // whatever wrote them has completed before the GEMM's blocks start.  Under expert parallelism every kernel of ep.cu is launched
 // plainly and calls no chain_next(), and one of them (the scatter, or the host's read of the counts) comes between the kernel
 // that writes the offsets and the GEMM, whatever the collective right before it does.
+// Third, the products of the dense block and the adapters (dense_rows.cu, dense_gemm.cu, dense_pair.cu) request their weights before their
+// chain_wait() (DenseGemm::b_early) and, beside adapters, in the weights' gradients and in a cut last wave, their rows and ids too
+// (a_early).  Such a launch is never a call's first.  The launch before it is of the same call, writes none of these, and comes to
+// chain_next() only past its own chain_wait(): whatever wrote them has completed.  What it does write (h; the adapters' reduced rows)
+// is read past the wait, and so are all stores.
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // A kernel that takes whole SMs must not sit there waiting while another stream's work could run.  So the kernels
