@@ -429,7 +429,9 @@ ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
 /* y = (silu(x Wg^T) * (x Wu^T)) Wd^T for the dense layers beside the MoE ones.  x [T, d_model], w_gate and w_up [d_ff, d_model],
  * w_down [d_model, d_ff], y [T, d_model]: device, bf16, row-major; y may be x, else no output (the workspace among them) overlaps
  * an input or another output (ATENIA_ERR_SHAPE).  The sums are f32; h = silu(g) u is rounded to bf16
- * between the products (of up to 8 tokens, what that leaves is multiplied too where the call's kernels can).  d_model and d_ff are multiples of 16 (at most 2^20), T at most 2^24 (0 is allowed); matrices and the workspace are
+ * between the products; of up to 8 tokens, what that leaves is multiplied by w_down too where the call's kernels can (the adapters of the
+ * down projection take the rounded h).  Which kernels a call takes, and with them the last bits of a token's row, goes by the sizes of
+ * the whole call.  d_model and d_ff are multiples of 16 (at most 2^20), T at most 2^24 (0 is allowed); matrices and the workspace are
  * 16-byte aligned (else ATENIA_ERR_SHAPE).  `workspace` (device) has at least the bytes the size function returns (else
  * ATENIA_ERR_CAPACITY); its content need not be kept between calls, and calls that may run at the same time, captured ones
  * included, need one each.  Asynchronous on `stream`; the calls allocate nothing and can be captured in a graph (make the first call
@@ -440,7 +442,8 @@ ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
  * Adapters: token t adds scale[a] * B_a (A_a x_t) to a projection W x_t, where a = ids[t]; an id outside [0, n) means none.
  * A is [n, rank, in], B [n, out, rank] (device, bf16, 16-byte aligned), scale [n] and ids [T] device.  A rank is a multiple of 8
  * up to ATENIA_ADAPTER_MAX_RANK (zero-pad A's rows and B's columns otherwise); rank 0 = this projection has none.  The reduced
- * rows scale A x are rounded to bf16, and where 32 rank > in what that leaves is multiplied by B too.  A token reads its own adapter only: infinities and NaN in another one's do not reach it. */
+ * rows scale A x are rounded to bf16, and where 32 rank > in what that leaves is multiplied by B too (of gate and up: the greater rank).
+ * A token reads its own adapter only: infinities and NaN in another one's do not reach it. */
 #define ATENIA_ADAPTER_MAX_RANK 128
 #define ATENIA_ADAPTER_MAX_COUNT 65536 /* n at most */
 typedef struct AteniaLowRank {
