@@ -475,53 +475,50 @@ static EncodeTiledFn get_encode_fn() {
   return fn.load(std::memory_order_relaxed);
 }
 
+// A host thread without a context (one that has made no runtime call yet; torch's backward threads start so) is refused by the
+// encoder, where a launch would bind the current device's: then that is done here.
+static int encode_tiled(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* size, const cuuint64_t* strides,
+                        const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  const EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return ATENIA_ERR_DRIVER;
+  const cuuint32_t estr[3] = {1, 1, 1};
+  auto encode = [&] {
+    return fn(out, type, (cuuint32_t)rank, const_cast<void*>(base), size, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    int dev = -1;
+    ATENIA_CUDA_TRY(cudaGetDevice(&dev));
+    ATENIA_CUDA_TRY(cudaSetDevice(dev));
+    r = encode();
+  }
+  return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
+}
+
 int encode_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
                       uint32_t box_cols, int swizzle64) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return ATENIA_ERR_DRIVER;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || cols % 16 != 0) return ATENIA_ERR_SHAPE;
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle64 == 2 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                 : (swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  return encode_tiled(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box,
+                      swizzle64 == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : (swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE));
 }
 
 int encode_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
                         uint32_t box_cols) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return ATENIA_ERR_DRIVER;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (cols * 2) % 16 != 0) return ATENIA_ERR_SHAPE;
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols * 2};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * 2};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  return encode_tiled(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int encode_tmap_bf16(CUtensorMap* out, const void* base, const uint64_t (&dims)[3], const uint32_t (&box)[3], int swizzle_bytes) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return ATENIA_ERR_DRIVER;
-  const int rank = dims[2] ? 3 : 2;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (dims[0] * 2) % 16 != 0) return ATENIA_ERR_SHAPE;
-  cuuint64_t size[3] = {dims[0], dims[1], dims[2]};
-  cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
-  cuuint32_t boxes[3] = {box[0], box[1], box[2]};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), size, strides, boxes, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
-                                                 : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                                       : CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? ATENIA_OK : ATENIA_ERR_DRIVER;
+  const cuuint64_t size[3] = {dims[0], dims[1], dims[2]}, strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
+  const cuuint32_t boxes[3] = {box[0], box[1], box[2]};
+  return encode_tiled(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims[2] ? 3 : 2, base, size, strides, boxes,
+                      swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace atenia
