@@ -97,8 +97,9 @@ __device__ __forceinline__ void mma_rows(float (&c)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: tiles of eight tokens (x in two parts: the first half of them the tokens, the other half what their rounding left).  Lane 4 g + i holds 32 bytes (piece i of a step) of weight rows g and g + 8 and of tokens g, g + 8, and sums
-// of those rows for tokens 2 i and 2 i + 1 of a tile.
+// NT: tiles of eight tokens (x in two parts: the first half of them the tokens, the other half what their rounding left).  Lane 4 g + i
+// holds 32 bytes (piece i of a step) of weight rows g and g + 8 and of tokens g, g + 8, and sums of those rows for tokens 2 i and 2 i + 1
+// of a tile.
 template <int EPI, int NT, bool AD, bool LARGE>
 __global__ void __launch_bounds__(kVecThreads, RowsShape<LARGE>::kBlocks)
 dense_rows_kernel(const __grid_constant__ VecArgs va, const __grid_constant__ std::conditional_t<AD, VecAdapters, NoVecAdapters> ad) {
