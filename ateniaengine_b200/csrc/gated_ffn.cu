@@ -38,6 +38,7 @@ constexpr int kMaxAdapters = ATENIA_ADAPTER_MAX_COUNT;
 
 uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 struct Range {
   const void* p;  // (null: none)
   uint64_t bytes;
@@ -89,7 +90,7 @@ bool rank_ok(int r) { return r >= 8 && r <= kAdapterMaxRank && r % 8 == 0; }
 int check_adapter(const AteniaLowRank& a) {
   if (!rank_ok(a.rank)) return ATENIA_ERR_SHAPE;
   if (!a.a || !a.b || !a.scale) return ATENIA_ERR_NULL;
-  if (!aligned16(a.a) || !aligned16(a.b)) return ATENIA_ERR_SHAPE;
+  if (!aligned16(a.a) || !aligned16(a.b) || !aligned4(a.scale)) return ATENIA_ERR_SHAPE;
   return ATENIA_OK;
 }
 // What a projection's adapters are read from
@@ -160,7 +161,7 @@ int check_sizes(int64_t T, int64_t d, int64_t f) {
 
 int check_ffn_adapters(const AteniaFfnAdapters* ad) {
   if (!ad->ids) return ATENIA_ERR_NULL;
-  if (ad->n < 1 || ad->n > kMaxAdapters) return ATENIA_ERR_SHAPE;
+  if (ad->n < 1 || ad->n > kMaxAdapters || !aligned4(ad->ids)) return ATENIA_ERR_SHAPE;
   const AteniaLowRank* sets[3] = {&ad->gate, &ad->up, &ad->down};
   for (const AteniaLowRank* a : sets) {
     if (a->rank == 0) continue;
@@ -393,6 +394,7 @@ int atenia_adapter_linear(const void* x, const void* weight, int T, int d_in, in
   if (!x || !ids || !y || !workspace) return ATENIA_ERR_NULL;
   for (const void* p : {x, weight, (const void*)y, (const void*)workspace})
     if (!aligned16(p)) return ATENIA_ERR_SHAPE;
+  if (!aligned4(ids)) return ATENIA_ERR_SHAPE;
   const uint64_t need = atenia_adapter_linear_workspace_bytes(T, adapter->rank);
   if (workspace_bytes < need) return ATENIA_ERR_CAPACITY;
   {

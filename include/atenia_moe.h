@@ -440,7 +440,7 @@ ATENIA_API int atenia_moe_stack_destroy(AteniaMoeStack* stack);
  * four features of a token side by side.
  *
  * Adapters: token t adds scale[a] * B_a (A_a x_t) to a projection W x_t, where a = ids[t]; an id outside [0, n) means none.
- * A is [n, rank, in], B [n, out, rank] (device, bf16, 16-byte aligned), scale [n] and ids [T] device.  A rank is a multiple of 8
+ * A is [n, rank, in], B [n, out, rank] (device, bf16, 16-byte aligned), scale [n] and ids [T] device, 4-byte aligned.  A rank is a multiple of 8
  * up to ATENIA_ADAPTER_MAX_RANK (zero-pad A's rows and B's columns otherwise); rank 0 = this projection has none.  The reduced
  * rows scale A x are rounded to bf16, and where 32 rank > in what that leaves is multiplied by B too (of gate and up: the greater rank).
  * A token reads its own adapter only: infinities and NaN in another one's do not reach it. */

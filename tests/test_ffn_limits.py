@@ -160,3 +160,14 @@ def test_no_product_of_allowed_sizes_has_more_tiles_than_a_launch_takes(tmp_path
                         assert items <= most, (T, d, F, two, grad, n, items)
                         seen = max(seen, items)
     assert seen > 1 << 28  # (the sizes do come near it)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_scales_and_ids_off_their_type_are_refused(lib, shift):
+    """The kernels read them as 32-bit words: an address in between would be a fault on the device."""
+    from ateniaengine_b200 import _lib
+    low = _lib.LowRank(a=P, b=P, scale=P + shift, rank=8)
+    assert _linear(lib, low=low) == -2 and _linear(lib, ids=P + shift) == -2
+    good = dict(gate=_low(8), up=_low(8), down=_low(8), ids=P, n=2)
+    for bad in (dict(gate=low), dict(up=low), dict(down=low), dict(ids=P + shift)):
+        assert _forward(lib, adapters=C.byref(_lib.FfnAdapters(**{**good, **bad})), nbytes=0) == -2, bad
