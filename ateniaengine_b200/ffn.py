@@ -45,24 +45,22 @@ def _operand(t, name, shape, dtype, device):
     raise ValueError(f"{name} is on {t.device}, x on {device}")
 
 
-def _rows(x, name="x"):
+def _rows(x, recorded=False):
+    """x, contiguous.  `recorded` False: the result has no history, so that an x that has one would lose its gradient without a word.
+    (Parameters are ordinary arguments: a program that calls gated_ffn_backward itself passes them.)"""
     if not isinstance(x, torch.Tensor) or x.dtype is not BF16:
-        raise TypeError(f"{name} must be a bf16 tensor")
-    if x.dim() != 2:
-        raise ValueError(f"{name} must be [tokens, width], got {tuple(x.shape)}")
-    if x.shape[0] > _MAX_ROWS:
-        raise ValueError(f"{name}: at most 2^24 tokens, got {x.shape[0]}")
-    if not x.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    return x if x.is_contiguous() else x.contiguous()
-
-
-def _check_unrecorded(x):
-    """The result has no history: where x has one, its gradient would be lost without a word.  (Parameters are ordinary arguments: a
-    program that calls gated_ffn_backward itself passes them.)"""
-    if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
+        raise TypeError("x must be a bf16 tensor")
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError(f"x must be [tokens, width], got {tuple(shape)}")
+    if shape[0] > _MAX_ROWS:
+        raise ValueError(f"x: at most 2^24 tokens, got {shape[0]}")
+    if not recorded and x.requires_grad and torch.is_grad_enabled():
         raise ValueError("x requires a gradient, which this call does not record: detach it, call under torch.no_grad(), or from a "
                          "torch.autograd.Function")
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _output(out, shape, x):
@@ -118,12 +116,13 @@ def _check_widths(a, b, what):
 
 
 def _projection(x, weight):
-    """in, out and the checked weight [out, in] of adapter_linear."""
+    """tokens, in, out and the checked weight [out, in] of adapter_linear."""
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be [out, in]")
-    n_in, n_out = x.shape[1], weight.shape[0]
+    T, n_in = x.shape
+    n_out = weight.shape[0]
     _check_widths(n_in, n_out, "the projection's sizes")
-    return n_in, n_out, _operand(weight, "weight", (n_out, n_in), BF16, x.device)
+    return T, n_in, n_out, _operand(weight, "weight", (n_out, n_in), BF16, x.device)
 
 
 def _block(x, gate, up, down):
@@ -132,8 +131,9 @@ def _block(x, gate, up, down):
     T, d = x.shape
     F = gate.shape[0]
     _check_widths(d, F, "d_model and d_ff")
-    return (T, d, F, _operand(gate, "gate", (F, d), BF16, x.device), _operand(up, "up", (F, d), BF16, x.device),
-            _operand(down, "down", (d, F), BF16, x.device))
+    device = x.device
+    return (T, d, F, _operand(gate, "gate", (F, d), BF16, device), _operand(up, "up", (F, d), BF16, device),
+            _operand(down, "down", (d, F), BF16, device))
 
 
 def _block_adapters(adapters, adapter_ids, T, d, F, save, device):
@@ -163,12 +163,13 @@ def _block_adapters(adapters, adapter_ids, T, d, F, save, device):
 
 
 def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, out=None, sync=False):
-    """y = (silu(x gate^T) * (x up^T)) down^T, not recorded for autograd.  x: CUDA bf16 [T, d], T up to 2^24; gate, up: bf16 [F, d]; down: bf16 [d, F].
+    """y = (silu(x gate^T) * (x up^T)) down^T, not recorded for autograd.  x: CUDA bf16 [T, d], T up to 2^24; gate, up: bf16 [F, d];
+    down: bf16 [d, F].
 
     `adapters`: a dict of LowRankAdapters for any of "gate", "up", "down" (the same number in each), with `adapter_ids` int32 [T]:
     the adapter of each token, outside [0, n) for none.  `save=True` returns (y, saved) for gated_ffn_backward; saved is f32
-    [2, F / 4, T, 4], the two projections before the activation.  `out` may be x, and overlaps nothing else that is read.  `sync=True` waits and raises what the kernels recorded."""
-    _check_unrecorded(x)
+    [2, F / 4, T, 4], the two projections before the activation.  `out` may be x, and overlaps nothing else that is read.
+    `sync=True` waits and raises what the kernels recorded."""
     x = _rows(x)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     ad, ranks = None, (0, 0, 0)
@@ -196,7 +197,7 @@ def gated_ffn(x, gate, up, down, adapters=None, adapter_ids=None, save=False, ou
 def gated_ffn_backward(dy, x, gate, up, down, saved, sync=False):
     """Gradients of gated_ffn(x, gate, up, down) for the gradient dy [T, d] of its output, from what save=True returned:
     (dx [T, d], dgate [F, d], dup [F, d], ddown [d, F]), bf16.  `saved` is left as it is."""
-    x = _rows(x)
+    x = _rows(x, recorded=True)  # (nothing is asked of autograd here)
     T, d, F, gate, up, down = _block(x, gate, up, down)
     dy = _operand(dy, "dy", (T, d), BF16, x.device)
     saved = _operand(saved, "saved", (2, F // 4, T, 4), torch.float32, x.device)
@@ -219,17 +220,16 @@ def adapter_linear(x, weight, adapters, adapter_ids, out=None, sync=False):
     """y = x weight^T + scale[i] * (x A_i^T) B_i^T with i = adapter_ids[t], outside [0, n) for none: one shared projection with the
     adapters of many requests.  x: CUDA bf16 [T, in]; weight: bf16 [out, in]; adapters: LowRankAdapters; adapter_ids: int32 [T].
     `out` must not overlap what is read."""
-    _check_unrecorded(x)
     x = _rows(x)
-    T = x.shape[0]
-    n_in, n_out, weight = _projection(x, weight)
-    ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, x.device)
-    low, n, keep = _low_rank(adapters, "adapters", n_in, n_out, x.device)
+    T, n_in, n_out, weight = _projection(x, weight)
+    device = x.device
+    ids = _operand(adapter_ids, "adapter_ids", (T,), torch.int32, device)
+    low, n, keep = _low_rank(adapters, "adapters", n_in, n_out, device)
     y = _output(out, (T, n_out), x)
     nbytes = _linear_bytes(T, low[3])
     ws = _workspace(nbytes, x)
     lib = _lib.lib()
-    with _launching(x.device) as st:
+    with _launching(device) as st:
         rc = lib.atenia_adapter_linear(x.data_ptr(), weight.data_ptr(), T, n_in, n_out, _LOW_RANK.pack(*low), ids.data_ptr(), n, y.data_ptr(),
                                        ws.data_ptr(), nbytes, st)
         if rc or sync:

@@ -122,7 +122,7 @@ def check_sum(a, b, unit, what):
 
 
 def check_bf16(t, what):
-    assert torch.equal(t.to(torch.bfloat16).double(), t), what
+    assert torch.equal(t.to(torch.bfloat16).to(t.dtype), t), what
 
 
 def delta(x, low, ids, what, unit_x=1.0):

@@ -30,10 +30,9 @@ def without(a, b, part):
 @pytest.mark.parametrize("T,d,F", ex.BLOCKS)
 def test_block(T, d, F):
     rows = min(max(T, 16), ROWS if d * F < 1e7 else ROWS // 2)  # (of a shorter call the inputs of 16)
-    x, w, dy = ex.make_x(rows, d, T, "cpu"), ex.make_block(d, F, 1, "cpu"), ex.make_dy(rows, d, 5, "cpu")
-    y, g, u, h = ex.forward(x, *w)
-    dx, dgate, dup, ddown = ex.backward(dy, x, *w, u, h)
-    x, dy, g, u, h, gate, up, down = (t.float() for t in (x, dy, g, u, h, *w))  # (exact too)
+    x, gate, up, down, dy = (t.float() for t in (ex.make_x(rows, d, T, "cpu"), *ex.make_block(d, F, 1, "cpu"), ex.make_dy(rows, d, 5, "cpu")))
+    y, g, u, h = ex.forward(x, gate, up, down)  # (f32 holds what ffn_exact asserts)
+    dx, dgate, dup, ddown = ex.backward(dy, x, gate, up, down, u, h)
     dh = dy @ down
     dg, du = dh * u, dh * 64
 
